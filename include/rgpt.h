@@ -52,8 +52,12 @@ enum RgptEpilogue {
   RGPT_EPI_POLY_BF16 = 6,  /* D bf16 = beta*C + alpha*acc, C bf16                   */
   RGPT_EPI_BIAS_SIGMOID_BF16 = 7, /* D bf16 = sigmoid(alpha*acc + colscale[n]) (G1 gate)  */
   RGPT_EPI_POLY_F32 = 8,   /* D f32  = beta*C + alpha*acc, C f32 (fp32 Newton-Schulz)  */
-  RGPT_EPI_ARGMAX_BF16 = 9 /* no D: per row and column tile, the first maximum of bf16(alpha*acc) and its
+  RGPT_EPI_ARGMAX_BF16 = 9, /* no D: per row and column tile, the first maximum of bf16(alpha*acc) and its
                               column (rgpt_gemm_argmax only)                          */
+  RGPT_EPI_LSE_F32 = 10,   /* no D: per row and column tile, the maximum and the sum of e^{acc - maximum}
+                              (rgpt_linear_logprobs only)                             */
+  RGPT_EPI_SOFTMAX_GRAD_BF16 = 11 /* D bf16 = coef[m]*([n = label[m]] - e^{acc - lse[m]})
+                              (rgpt_linear_logprobs_dlogits only)                     */
 };
 enum RgptActivation { RGPT_ACT_NONE = 0, RGPT_ACT_SQUARED_RELU = 1, RGPT_ACT_GELU = 2, RGPT_ACT_SILU = 3, RGPT_ACT_MISH = 4,
                       /* squared ReLU, post-activation only: ACT_FWD writes D = relu(acc)^2 and no D2 (pass
@@ -214,6 +218,63 @@ int rgpt_cross_entropy(void* logits, long long ld, int M, int V, const long long
  * start at zero; each call rewrites what it reads. No cudaMalloc/cudaFree is made. */
 int rgpt_cross_entropy_noalloc(void* logits, long long ld, int M, int V, const long long* labels, int ignore_index,
                                float grad_scale, float* loss_out, int* argmax, int write_grad, void* stream);
+/* ------------------------------------------------------------------ post-training losses
+ * No counterpart in the reference, which only pre-trains (its loss is the cross entropy above).
+ * Logits: bf16, fp16 or fp32 (RgptDtype), row (b, t) of a [B, T] grid at element b*sb + t*st, unit stride along the
+ * vocabulary, any alignment of the type; labels [B, T] int64, contiguous. A token is scored when its label lies in
+ * [0, V) and is not ignore_index; an unscored row is not read, has log-probability 0 and a zero gradient row.
+ * dlogits has the logits' type and its own strides db, dt; it may be the logits themselves (same pointer and
+ * strides), which are then overwritten. B*T < 2^31. Sums are fp32 or wider, and in a fixed order: equal calls give
+ * equal bits. */
+enum RgptDtype { RGPT_DTYPE_BF16 = 0, RGPT_DTYPE_F16 = 1, RGPT_DTYPE_F32 = 2 };
+/* logps [B, T] = logits[label] - lse, lse [B, T] (optional) = log sum_j e^{logits_j}; 0 where not scored. */
+int rgpt_token_logprobs(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,
+                        const long long* labels, long long ignore_index, float* logps, float* lse, void* stream);
+/* dlogits = dlogps * ([j = label] - e^{logits_j - lse}); lse as rgpt_token_logprobs wrote it (a row whose |lse| is
+ * above 64, where fp32 would round it too coarsely, is summed again). */
+int rgpt_token_logprobs_bwd(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,
+                            const long long* labels, long long ignore_index, const float* lse, const float* dlogps,
+                            void* dlogits, long long db, long long dt, void* stream);
+/* Paired preference loss over 2P sequences: sequence p < P is the chosen one of pair p, P + p the rejected one.
+ *   s = sum of the sequence's scored log-probabilities (their mean with `average`)
+ *   h = beta * ((s_chosen - ref_chosen) - (s_rejected - ref_rejected)) - margin   (ref_logps [2P], null = 0)
+ *   SIGMOID: -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h);  HINGE: max(0, 1 - h);
+ *   SQUARED: (h - 1/2)^2;   loss[0] = mean over the pairs.
+ * Writes token_logps, lse [2P, T], seq_logps [2P] (s), margins [P] (h), coef [2P] (grad_scale * d loss / d a scored
+ * token's log-probability) and, when dlogits is not null, grad_scale * d loss / d logits. scratch [2P, T] fp64: the
+ * log-probabilities before their rounding to fp32, whose errors the difference of two long sums would show. */
+enum RgptPreference { RGPT_PREF_SIGMOID = 0, RGPT_PREF_HINGE = 1, RGPT_PREF_SQUARED = 2 };
+int rgpt_preference_loss(const void* logits, int dtype, long long sb, long long st, int P, int T, int V,
+                         const long long* labels, long long ignore_index, const float* ref_logps, int kind, float beta,
+                         float margin, float label_smoothing, int average, float grad_scale, float* token_logps,
+                         float* lse, float* seq_logps, float* margins, float* coef, float* loss, double* scratch,
+                         void* dlogits, long long db, long long dt, void* stream);
+/* Clipped policy loss with a KL term, per scored token with log-probability lp and ratio r = e^{lp - old}:
+ *   pg = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A),  kl = e^{ref - lp} - (ref - lp) - 1 (ref_logps null: 0)
+ *   loss = sum_t w (pg + kl_coef kl),  w = 1 / (scored tokens), or with by_sequence
+ *   1 / (sequences with a scored token * scored tokens of the token's sequence).
+ * old_logps, ref_logps [B, T]; advantages [B], or [B, T] with adv_per_token. Writes token_logps [B, T], counts [B]
+ * (scored tokens of each sequence), stats [4] = {loss, sum w pg, sum w kl, weighted share of clipped tokens}, the
+ * optional lse [B, T] and coef [B, T] (grad_scale * d loss / d lp, 0 where not scored), and, when dlogits is not null,
+ * grad_scale * d loss / d logits. Without any scored token everything is 0. */
+int rgpt_policy_loss(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,
+                     const long long* labels, long long ignore_index, const float* old_logps, const float* ref_logps,
+                     const float* advantages, int adv_per_token, float clip_low, float clip_high, float kl_coef,
+                     int by_sequence, float grad_scale, float* token_logps, int* counts, float* stats, float* lse,
+                     float* coef, void* dlogits, long long db, long long dt, void* stream);
+/* Log-probabilities straight from hidden states, logits = X @ W^T never stored: X [M, K], W [V, K] bf16, K-major,
+ * 16-byte aligned rows; labels [M]. logps [M], lse [M] (optional, written for every row) as rgpt_token_logprobs over
+ * the fp32 product (round_bf16: over the product rounded to bf16, which is what a stored bf16 product gives).
+ * part: scratch of part_floats >= 2 * M * ceil(V/128) floats, 8-byte aligned. */
+int rgpt_linear_logprobs(const void* X, long long ldx, const void* W, long long ldw, int M, int V, int K,
+                         const long long* labels, long long ignore_index, int round_bf16, float* part,
+                         long long part_floats, float* logps, float* lse, void* stream);
+/* The gradient of those logits for M rows, from the recomputed product: dlogits [M, >= V] bf16 =
+ * dlogps * ([j = label] - e^{logit_j - lse}), zero rows where not scored. The gradients of X and W follow by
+ * rgpt_gemm_bf16 (dX = dlogits W, dW += dlogits^T X). */
+int rgpt_linear_logprobs_dlogits(const void* X, long long ldx, const void* W, long long ldw, int M, int V, int K,
+                                 const long long* labels, long long ignore_index, const float* lse,
+                                 const float* dlogps, void* dlogits, long long ldd, void* stream);
 /* rGPT halting losses (model/gpt.py:105-141, trainer.py:150-162): q [R, M, 2], argmax [R, M].
  * losses[0] += halt BCE mean, losses[1] += q_continue BCE mean; dq = grad_scale * d(total)/dq. */
 int rgpt_halt_losses(const float* q, const int* argmax, const long long* labels, int R, int M, float grad_scale,
@@ -266,6 +327,26 @@ int rgpt_segment_copy(const RgptSegment* table, const int* chunk_seg, const long
 int rgpt_adamw(const RgptAdamwTensor* table, const int* chunk_tensor, const long long* chunk_start, int n_chunks,
                int chunk_elems, float lr, float wd, float beta1, float beta2, float eps, int step, const float* hp,
                void* stream);
+/* AdamW with both moments in 8 bits (no counterpart in the reference, whose moments are fp32). Each block of 256
+ * consecutive elements of a tensor (the last one may be shorter) has two fp32 scales:
+ *   m = mq * m_scale[block],      mq float8 e4m3,  m_scale = max|m| / 448
+ *   v = (vq * r_scale[block])^2,  vq unsigned, 3 bits of exponent and 5 of mantissa: q / 2048 for q < 32, else
+ *       2^(q/32 - 7) * (1 + (q%32)/32); r = sqrt(v), r_scale = max r / 1.96875. A nonzero r never takes code 0.
+ * Codes round to nearest, ties to even; a block whose largest moment is not above 2^-100 holds zeros. The update:
+ *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr ((m / (sqrt(v) inv_sqrt_bc2 + eps)) inv_bc1)
+ * from the moments before they are rounded to codes, every operation one fp32 rounding. chunk_elems: a multiple of
+ * 256, and every chunk_start too. */
+#define RGPT_ADAMW8_BLOCK 256
+typedef struct RgptAdamw8Tensor {
+  float* p; const float* g; unsigned char* mq; float* m_scale; unsigned char* vq; float* r_scale;
+  unsigned short* shadow; long long n;
+} RgptAdamw8Tensor;
+int rgpt_adamw8(const RgptAdamw8Tensor* table, const int* chunk_tensor, const long long* chunk_start, int n_chunks,
+                int chunk_elems, float lr, float wd, float beta1, float beta2, float eps, int step, const float* hp,
+                void* stream);
+/* The fp32 moments m, v [n] that codes and scales stand for. */
+int rgpt_adamw8_moments(const unsigned char* mq, const float* m_scale, const unsigned char* vq, const float* r_scale,
+                        float* m, float* v, long long n, void* stream);
 /* muon_update's momentum/Nesterov/transposition (optimizer.py:51-69, :23-26) for n same-shape [R, C]
  * matrices into the bf16 NS stack X (zero-padded, leading dim ldx); sumsq[n] ACCUMULATES ||X||_F^2. */
 int rgpt_muon_prep(const RgptMuonTensor* table, int n, int R, int C, void* X, long long x_bstride, int ldx,

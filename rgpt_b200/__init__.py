@@ -4,6 +4,7 @@ Sub-modules:
   _lib       ctypes binding of librgpt_kernels.so (C ABI in include/rgpt.h)
   native     torch-tensor wrappers of each native entry point
   model      GPT / rGPT modules with the reference's Python API
+  losses     differentiable post-training losses on logits and hidden states
   optimizer  Muon / DistMuon (NorMuon / DistNorMuon aliases)
   trainer    the training-step driver
 """

@@ -64,6 +64,26 @@ _SIGNATURES: dict[str, list] = {
     "rgpt_cross_entropy_noalloc": [_c_vp, _c_ll, _c_int, _c_int, _c_vp, _c_int, _c_float, _c_vp, _c_vp, _c_int,
                                    _c_vp],
     "rgpt_halt_losses": [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_float, _c_vp, _c_vp, _c_vp],
+    "rgpt_token_logprobs": [_c_vp, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_vp, _c_vp, _c_vp],
+    "rgpt_token_logprobs_bwd": [_c_vp, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_vp, _c_vp, _c_vp,
+                                _c_ll, _c_ll, _c_vp],
+    "rgpt_preference_loss": [
+        _c_vp, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll,  # logits .. V, labels, ignore_index
+        _c_vp, _c_int, _c_float, _c_float, _c_float, _c_int, _c_float,  # ref, kind, beta, margin, smoothing, average, scale
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_ll, _c_ll, _c_vp,  # outputs, scratch, dlogits, stream
+    ],
+    "rgpt_policy_loss": [
+        _c_vp, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll,  # logits .. V, labels, ignore_index
+        _c_vp, _c_vp, _c_vp, _c_int, _c_float, _c_float, _c_float, _c_int, _c_float,  # old, ref, adv .. grad_scale
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_ll, _c_ll, _c_vp,  # outputs, dlogits and its strides, stream
+    ],
+    "rgpt_linear_logprobs": [_c_vp, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_vp, _c_ll,
+                             _c_vp, _c_vp, _c_vp],
+    "rgpt_linear_logprobs_dlogits": [_c_vp, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_vp, _c_vp,
+                                     _c_vp, _c_ll, _c_vp],
+    "rgpt_adamw8": [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float, _c_float, _c_int,
+                    _c_vp, _c_vp],
+    "rgpt_adamw8_moments": [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_ll, _c_vp],
     "rgpt_adamw": [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float, _c_float, _c_int,
                    _c_vp, _c_vp],
     "rgpt_muon_prep": [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_float, _c_int, _c_vp, _c_vp, _c_vp],
@@ -128,7 +148,7 @@ def last_error() -> str:
 
 # Kernels each entry point enqueues (rgpt_cross_entropy: up to 3, counted by its wrapper).
 _KERNELS_PER_CALL = {"rgpt_last_error": 0, "rgpt_device_error": 0, "rgpt_version": 0,
-                     "rgpt_cross_entropy_noalloc": 3}
+                     "rgpt_cross_entropy_noalloc": 3, "rgpt_linear_logprobs": 2}
 launch_count = 0  # native kernels enqueued by this process (read by the benchmark)
 
 

@@ -31,6 +31,10 @@
 //   POLY_F32     the same in fp32 (C and D fp32)     (fp32 Newton-Schulz on split bf16 operands)
 //   ARGMAX_BF16  per row and column tile: the first maximum of bf16(acc) and its column; no output
 //                matrix (the rGPT per-step lm_head argmax, model/gpt.py:119-120)
+//   LSE_F32      per row and column tile: maximum and sum of exponentials, and the label's value; no output
+//                matrix (log-probabilities from hidden states)
+//   SOFTMAX_GRAD coef[row] * ([column = label] - e^{acc - lse[row]}): the gradient tiles of those
+//                log-probabilities, from the recomputed product
 //   BIAS_SIGMOID sigmoid(acc + bias)                 (model/attention.py:45-48, G1 gate)
 //   ACCUM_F32    grad += acc (bulk reduce-add, so split-K needs no separate reduction)
 #include <cudaTypedefs.h>
@@ -67,6 +71,14 @@ struct EpiParams {
   float* amax_val;
   int* amax_idx;
   long long amax_ld;
+  // LSE_F32 / SOFTMAX_GRAD_BF16: each row's label (scored when in [0, N) and not ignore_index)
+  const long long* labels;
+  long long ignore_index;
+  float2* lse_part;        // LSE_F32: [column tile][M] (maximum, sum of e^{v - maximum}) of the tile's columns
+  float* label_logit;      // LSE_F32: [M], the label's value, written for scored rows only
+  int round_bf16;          // LSE_F32: the values are rounded to bf16 first (what a stored bf16 product would hold)
+  const float* row_lse;    // SOFTMAX_GRAD_BF16: [M]
+  const float* row_coef;   // SOFTMAX_GRAD_BF16: [M]
 };
 
 constexpr int GEMM_BM = 128;
@@ -379,7 +391,8 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
     uint8_t* buf1 = buf0 + EPI_STAGE_BYTES;
     int which = 0;
     constexpr bool bf16_out = (EPI == RGPT_EPI_STORE_BF16 || EPI == RGPT_EPI_ACT_FWD || EPI == RGPT_EPI_ACT_BWD ||
-                               EPI == RGPT_EPI_POLY_BF16 || EPI == RGPT_EPI_BIAS_SIGMOID_BF16);
+                               EPI == RGPT_EPI_POLY_BF16 || EPI == RGPT_EPI_BIAS_SIGMOID_BF16 ||
+                               EPI == RGPT_EPI_SOFTMAX_GRAD_BF16);
     constexpr bool act_two_out = EPI == RGPT_EPI_ACT_FWD && ACT != ACT_SQRELU_POST;  // pre and post
     const bool dual = act_two_out || (EPI == RGPT_EPI_RESID_F32 && ep.has_d2);
     const float alpha = ep.alpha_dev ? ep.alpha * __ldg(ep.alpha_dev) : ep.alpha;
@@ -465,7 +478,72 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
           ep.amax_val[(long long)row * ep.amax_ld + nt] = best;
           ep.amax_idx[(long long)row * ep.amax_ld + nt] = besti;
         }
+      } else if constexpr (EPI == RGPT_EPI_LSE_F32) {
+        // this thread's row: a running maximum and sum of exponentials over the tile's columns (fp32), and the
+        // label's value when it lies in this tile
+        const int row = row0 + lane;
+        const long long label = row < sh.M ? ep.labels[row] : -1;
+        const bool scored = label >= 0 && label < sh.N && label != ep.ignore_index;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+        for (int c0 = cbeg; c0 < cend; c0 += 32) {
+          const int gn0 = nt * BN + c0;
+          uint32_t rr[32];
+          tmem_ld32(t_row + c0, rr);
+          tmem_wait_ld();
+          if (gn0 >= sh.N) continue;
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]);
+          if (ep.round_bf16) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = bf16_round(v[j]);
+          }
+          if (gn0 + 32 > sh.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = gn0 + j < sh.N ? v[j] : -INFINITY;
+          }
+          if (scored && label >= gn0 && label < gn0 + 32) {
+            const int at = (int)label - gn0;
+            float x = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) x = j == at ? v[j] : x;
+            ep.label_logit[row] = x;
+          }
+          __syncwarp();
+          float cm = v[0];
+#pragma unroll
+          for (int j = 1; j + 1 < 32; j += 2) cm = fmax3(cm, v[j], v[j + 1]);
+          cm = fmaxf(cm, v[31]);
+          const float nm = fmaxf(m, cm);
+          const float r = nm == -INFINITY ? 0.f : nm;  // only -inf so far: e^{-inf - 0} = 0, not a NaN
+          s *= ex2_approx((m - r) * 1.4426950408889634f);
+          m = nm;
+          const float2 nr = make_float2(-r, -r), l2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+          float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float2 t0 = fmul2(fadd2(make_float2(v[j], v[j + 1]), nr), l2e);
+            const float2 t1 = fmul2(fadd2(make_float2(v[j + 2], v[j + 3]), nr), l2e);
+            a0 = fadd2(a0, make_float2(ex2_approx(t0.x), ex2_approx(t0.y)));
+            a1 = fadd2(a1, make_float2(ex2_approx(t1.x), ex2_approx(t1.y)));
+          }
+          s += (a0.x + a0.y) + (a1.x + a1.y);
+        }
+        if (row < sh.M) ep.lse_part[(long long)nt * sh.M + row] = make_float2(m, s);
       } else if constexpr (bf16_out) {
+        // SOFTMAX_GRAD: this thread's row of labels, log-sum-exps and coefficients
+        float g_lse = 0.f, g_coef = 0.f;
+        int g_label = -1;
+        if constexpr (EPI == RGPT_EPI_SOFTMAX_GRAD_BF16) {
+          const int row = row0 + lane;
+          const long long label = row < sh.M ? ep.labels[row] : -1;
+          if (label >= 0 && label < sh.N && label != ep.ignore_index) {
+            g_label = (int)label;
+            g_lse = ep.row_lse[row];
+            g_coef = ep.row_coef[row];
+          }
+        }
         auto chunk_bf16 = [&](int c0, const uint4 (&cc)[8]) {
           const int gn0 = nt * BN + c0;
           const bool live = rows_live && gn0 < sh.N;  // warp-uniform
@@ -513,6 +591,22 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
                 const int col = gn0 + hf * 32 + j;
                 const float bias = (col < sh.N) ? __ldg(ep.colscale + col) : 0.f;
                 v[j] = rcp_approx(1.0f + ex2_approx(-(v[j] + bias) * 1.4426950408889634f));
+              }
+            } else if constexpr (EPI == RGPT_EPI_SOFTMAX_GRAD_BF16) {
+              const int c = gn0 + hf * 32;
+              const float2 nl = make_float2(-g_lse, -g_lse), l2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float2 t = fmul2(fadd2(make_float2(v[j], v[j + 1]), nl), l2e);
+                v[j] = -g_coef * ex2_approx(t.x);
+                v[j + 1] = -g_coef * ex2_approx(t.y);
+              }
+              if (g_label < 0) {  // not scored: zeros, whatever the product holds
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.f;
+              } else if (g_label >= c && g_label < c + 32) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += (g_label == c + j) ? g_coef : 0.f;
               }
             } else if constexpr (EPI == RGPT_EPI_ACT_FWD && !act_two_out) {
               act_fwd32<ACT>(v);  // the post-activation is the only output
@@ -774,6 +868,15 @@ static int dispatch_epi(int epi, const CUtensorMap& ta, const CUtensorMap& tb, c
     RGPT_GEMM_EPI_CASE(RGPT_EPI_POLY_BF16)
     RGPT_GEMM_EPI_CASE(RGPT_EPI_POLY_F32)
     RGPT_GEMM_EPI_CASE(RGPT_EPI_ARGMAX_BF16)
+    case RGPT_EPI_LSE_F32:
+    case RGPT_EPI_SOFTMAX_GRAD_BF16:
+      if constexpr (A_MN == 0 && B_MN == 0) {  // their entry points take K-major operands only
+        return epi == RGPT_EPI_LSE_F32
+                   ? launch_gemm<BN, STAGES, 0, 0, RGPT_EPI_LSE_F32, PAIR>(ta, tb, td, td2, sh, ep, s, dev)
+                   : launch_gemm<BN, STAGES, 0, 0, RGPT_EPI_SOFTMAX_GRAD_BF16, PAIR>(ta, tb, td, td2, sh, ep, s, dev);
+      } else {
+        return rgpt_set_error(RGPT_ERR_INTERNAL, "epilogue %d takes K-major operands", epi);
+      }
     default: return launch_gemm<BN, STAGES, A_MN, B_MN, RGPT_EPI_BIAS_SIGMOID_BF16, PAIR>(ta, tb, td, td2, sh, ep, s, dev);
   }
 #undef RGPT_GEMM_EPI_CASE
@@ -842,6 +945,16 @@ struct DropArgs {
   float p;
 };
 
+struct LogpArgs {  // LSE_F32 / SOFTMAX_GRAD_BF16 (see EpiParams); n_tiles is set to the column tiles used
+  const long long* labels;
+  long long ignore_index;
+  float2* part;
+  float* label_logit;
+  int round_bf16;
+  const float *row_lse, *row_coef;
+  int n_tiles;
+};
+
 struct AmaxArgs {  // ARGMAX_BF16 partial results, [M, ld] each; n_tiles is set to the column tiles used
   float* val;
   int* idx;
@@ -854,7 +967,7 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
                       int act, float alpha, float beta, void* D, long long ldd, long long d_bstride, void* D2,
                       long long ldd2, long long d2_bstride, const void* C, long long ldc, long long c_bstride,
                       const float* colscale, int splitk, const float* alpha_dev, const DropArgs* drop,
-                      void* stream, AmaxArgs* amax = nullptr) {
+                      void* stream, AmaxArgs* amax = nullptr, LogpArgs* logp = nullptr) {
   int dev = 0;
   cudaGetDevice(&dev);
   int st = rgpt_check_device(dev);
@@ -863,10 +976,13 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
   if (batch < 1) batch = 1;
   if (M < 1 || N < 1 || K < 1)
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "gemm needs M, N, K >= 1 (got M=%d N=%d K=%d)", M, N, K);
-  if (epi < RGPT_EPI_STORE_BF16 || epi > RGPT_EPI_ARGMAX_BF16 || (epi == RGPT_EPI_ARGMAX_BF16 && amax == nullptr))
+  const bool lsx = epi == RGPT_EPI_LSE_F32, sgx = epi == RGPT_EPI_SOFTMAX_GRAD_BF16;
+  if (epi < RGPT_EPI_STORE_BF16 || epi > RGPT_EPI_SOFTMAX_GRAD_BF16 ||
+      (epi == RGPT_EPI_ARGMAX_BF16 && amax == nullptr) || ((lsx || sgx) && logp == nullptr))
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "unknown epilogue %d", epi);
-  const bool amx = epi == RGPT_EPI_ARGMAX_BF16;  // no output matrix: per-tile row maxima instead
-  if (amx && (batch != 1 || amax->val == nullptr || amax->idx == nullptr || amax->ld < (N + 127) / 128))
+  // no output matrix: per-tile row maxima (ARGMAX_BF16) or sums (LSE_F32) instead
+  const bool amx = epi == RGPT_EPI_ARGMAX_BF16 || lsx;
+  if (amx && !lsx && (batch != 1 || amax->val == nullptr || amax->idx == nullptr || amax->ld < (N + 127) / 128))
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "argmax GEMM needs batch 1 and [M, >= %d] partial buffers",
                           (N + 127) / 128);
   if (D == nullptr && !amx) return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "gemm output pointer is null");
@@ -908,7 +1024,7 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
   // Short-K GEMMs with few tiles stay on single-CTA tiles, whose shorter signalling chain
   // finishes each tile sooner.
   const long long pair_tiles = (long long)batch * ((M + 255) / 256) * ((N + 255) / 256);
-  const bool plain_store = epi == RGPT_EPI_STORE_BF16 || epi == RGPT_EPI_STORE_F32 || amx;
+  const bool plain_store = epi == RGPT_EPI_STORE_BF16 || epi == RGPT_EPI_STORE_F32 || amx || sgx;
   const bool pair = BN == 256 && M > GEMM_BM &&
                     ((pair_tiles >= nsm / 2 && (sh.num_kb >= 16 || (plain_store && pair_tiles >= 8LL * nsm))) ||
                      (epi == RGPT_EPI_ACCUM_F32 && sh.num_kb >= 32));
@@ -996,10 +1112,18 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
   ep.drop_mask = nullptr;
   ep.drop_ldm = 0;
   ep.drop_scale = 1.0f;
-  if (amx) amax->n_tiles = sh.n_tiles;
-  ep.amax_val = amx ? amax->val : nullptr;
-  ep.amax_idx = amx ? amax->idx : nullptr;
-  ep.amax_ld = amx ? amax->ld : 0;
+  if (amax != nullptr) amax->n_tiles = sh.n_tiles;
+  ep.amax_val = amax ? amax->val : nullptr;
+  ep.amax_idx = amax ? amax->idx : nullptr;
+  ep.amax_ld = amax ? amax->ld : 0;
+  if (logp != nullptr) logp->n_tiles = sh.n_tiles;
+  ep.labels = logp ? logp->labels : nullptr;
+  ep.ignore_index = logp ? logp->ignore_index : 0;
+  ep.lse_part = logp ? logp->part : nullptr;
+  ep.label_logit = logp ? logp->label_logit : nullptr;
+  ep.round_bf16 = logp ? logp->round_bf16 : 0;
+  ep.row_lse = logp ? logp->row_lse : nullptr;
+  ep.row_coef = logp ? logp->row_coef : nullptr;
   if (drop != nullptr && drop->p > 0.0f) {
     if (epi != RGPT_EPI_RESID_F32)
       return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "dropout is only fused into the RESID_F32 epilogue");
@@ -1051,4 +1175,72 @@ extern "C" int rgpt_gemm_argmax(const void* A, long long lda, const void* B, lon
   launch_pdl(argmax_reduce_kernel, dim3((unsigned)((M + 7) / 8)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1,
              (const float*)part_val, (const int*)part_idx, ld_part, a.n_tiles, M, argmax);
   return rgpt_check_launch("argmax_reduce_kernel");
+}
+
+// Joins the LSE_F32 GEMM's column tiles: lane = row (32 rows a CTA, coalesced reads of part[tile][row]), the warps
+// share the tiles, and the CTA combines their (maximum, sum) pairs in a fixed order. On entry logps holds the scored
+// rows' label logits. lse and the log-probability are formed in fp64 and rounded once.
+__global__ void __launch_bounds__(1024) lse_reduce_kernel(const float2* __restrict__ part, int n_tiles, int M, int N,
+                                                          const long long* __restrict__ labels, long long ignore_index,
+                                                          float* logps, float* __restrict__ lse) {
+  griddep_wait();
+  griddep_launch();
+  __shared__ float sm[32][33], ss[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  auto merge = [&](float om, float os) {
+    const float nm = fmaxf(m, om), r = nm == -INFINITY ? 0.f : nm;
+    s = s * ex2_approx((m - r) * 1.4426950408889634f) + os * ex2_approx((om - r) * 1.4426950408889634f);
+    m = nm;
+  };
+  if (row < M)
+    for (int t = warp; t < n_tiles; t += 32) {
+      const float2 p = part[(long long)t * M + row];
+      merge(p.x, p.y);
+    }
+  sm[warp][lane] = m;
+  ss[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || row >= M) return;
+  for (int w = 1; w < 32; ++w) merge(sm[w][lane], ss[w][lane]);
+  const long long label = labels[row];
+  const bool scored = label >= 0 && label < N && label != ignore_index;
+  const double l = (double)m + log((double)s);
+  logps[row] = scored ? (float)((double)logps[row] - l) : 0.f;
+  if (lse) lse[row] = (float)l;
+}
+
+static int logp_gemm_check(const char* what, const long long* labels) {
+  return labels == nullptr ? rgpt_set_error(RGPT_ERR_BAD_SHAPE, "%s: null pointer", what) : RGPT_OK;
+}
+
+extern "C" int rgpt_linear_logprobs(const void* X, long long ldx, const void* W, long long ldw, int M, int V, int K,
+                                    const long long* labels, long long ignore_index, int round_bf16, float* part,
+                                    long long part_floats, float* logps, float* lse, void* stream) {
+  int st = logp_gemm_check("linear_logprobs", labels);
+  if (st) return st;
+  if (logps == nullptr || part == nullptr || (reinterpret_cast<uintptr_t>(part) & 7) != 0)
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "linear_logprobs: null or misaligned output or partial buffer");
+  if (M >= 1 && V >= 1 && part_floats < 2ll * M * ((V + 127) / 128))
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "linear_logprobs: the partial buffer needs 2 * M * ceil(V / 128) floats");
+  LogpArgs a = {labels, ignore_index, reinterpret_cast<float2*>(part), logps, round_bf16, nullptr, nullptr, 0};
+  st = gemm_entry(X, 0, ldx, 0, W, 0, ldw, 0, M, V, K, 1, RGPT_EPI_LSE_F32, 0, 1.0f, 0.0f, nullptr, 0, 0, nullptr, 0, 0,
+                  nullptr, 0, 0, nullptr, 1, nullptr, nullptr, stream, nullptr, &a);
+  if (st) return st;
+  launch_pdl(lse_reduce_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, reinterpret_cast<cudaStream_t>(stream), 1,
+             (const float2*)part, a.n_tiles, M, V, labels, ignore_index, logps, lse);
+  return rgpt_check_launch("lse_reduce_kernel");
+}
+
+extern "C" int rgpt_linear_logprobs_dlogits(const void* X, long long ldx, const void* W, long long ldw, int M, int V,
+                                            int K, const long long* labels, long long ignore_index, const float* lse,
+                                            const float* dlogps, void* dlogits, long long ldd, void* stream) {
+  int st = logp_gemm_check("linear_logprobs_dlogits", labels);
+  if (st) return st;
+  if (lse == nullptr || dlogps == nullptr)
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "linear_logprobs_dlogits: null pointer");
+  LogpArgs a = {labels, ignore_index, nullptr, nullptr, 0, lse, dlogps, 0};
+  return gemm_entry(X, 0, ldx, 0, W, 0, ldw, 0, M, V, K, 1, RGPT_EPI_SOFTMAX_GRAD_BF16, 0, 1.0f, 0.0f, dlogits, ldd, 0,
+                    nullptr, 0, 0, nullptr, 0, 0, nullptr, 1, nullptr, nullptr, stream, nullptr, &a);
 }

@@ -5,6 +5,8 @@
 //   p -= lr * (m / bc1) / (sqrt(v) / sqrt(bc2) + eps)
 // and, when a bf16 shadow pointer is given, shadow = bf16(p) (the GEMM operand copy).
 //
+// AdamW with both moments in 8 bits (blocks of 256 elements): adamw8, adamw8_moments.
+//
 // Muon (optimizer.py:51-74, :199-227), per shape class of matrices [R, C]:
 //   muon_prep   g_b = bf16(grad); m = lerp(m, g_b, 1-beta) (bf16); g = lerp(g_b, m, beta) (Nesterov);
 //               X = g (transposed when R > C) into a zero-padded bf16 stack; ||X||_F^2 per matrix
@@ -16,6 +18,9 @@
 //   ns_sumsq    ||X||_F^2 per matrix, reading the unit-stride dimension fastest
 //   ns_split    X / max(||X||_F, 1e-7) (optional), an fp32 copy, and bf16 hi/lo blocks for the GEMMs
 // Tensors are addressed through small device-resident descriptor tables built once by the host.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
 #include "common.cuh"
 #include "rgpt.h"
 
@@ -82,6 +87,146 @@ __global__ void adamw_kernel(const RgptAdamwTensor* __restrict__ tab, const int*
     t.v[i] = v;
     t.p[i] = p;
     if (t.shadow) t.shadow[i] = __bfloat16_as_ushort(__float2bfloat16(p));
+  }
+}
+
+// ---------------------------------------------------------------------------- AdamW, 8-bit moments
+// One warp per block of 256 elements, 8 consecutive elements a lane: the two block maxima are warp reductions and the
+// block's codes are written from the registers that made them. Bound by HBM: 16 bytes a parameter (p read and
+// written, g read, both codes read and written) and 2 more for the bf16 copy, against 28 and 2 with fp32 moments.
+// Every operation is spelled out with its one rounding (no contraction), so that vector and scalar paths, and any
+// other program of the same formulas, give the same codes.
+constexpr float A8_M_TOP = 448.0f, A8_M_STEP = (float)(1.0 / 448.0);
+constexpr float A8_R_TOP = 1.96875f, A8_R_STEP = (float)(1.0 / 1.96875);
+constexpr float A8_TINY = 7.888609052210118e-31f;  // 2^-100
+
+// unsigned code of y in [0, 1.97): 3 bits of exponent, 5 of mantissa, denormal below 2^-6
+__device__ __forceinline__ uint32_t a8_encode_r(float y) {
+  const uint32_t bits = __float_as_uint(y);
+  const uint32_t fine = ((bits + 0x1FFFFu + ((bits >> 18) & 1u)) >> 18) - (120u << 5);
+  const uint32_t q = y >= 0.015625f ? fine : (uint32_t)__float2int_rn(__fmul_rn(y, 2048.0f));
+  return q < 255u ? q : 255u;
+}
+// The code's bits are those of a half of the same exponent width below its bias: value * 2^-8, denormals included.
+__device__ __forceinline__ float a8_decode_r(uint32_t q) {
+  return __half2float(__ushort_as_half((unsigned short)(q << 5))) * 256.0f;
+}
+__device__ __forceinline__ float2 a8_decode_m2(uint32_t q2) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q2, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+__global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __restrict__ tab,
+                                                     const int* __restrict__ chunk_tensor,
+                                                     const long long* __restrict__ chunk_start, int chunk_elems,
+                                                     float lr, float wd, float beta1, float beta2, float eps,
+                                                     float inv_bc1, float inv_sqrt_bc2, const float* __restrict__ hp) {
+  griddep_wait();
+  griddep_launch();
+  if (hp != nullptr) {
+    lr = hp[0], wd = hp[1], beta1 = hp[2], beta2 = hp[3], eps = hp[4], inv_bc1 = hp[5], inv_sqrt_bc2 = hp[6];
+  }
+  const RgptAdamw8Tensor t = tab[chunk_tensor[blockIdx.x]];
+  const long long start = chunk_start[blockIdx.x];
+  const long long end = min(start + (long long)chunk_elems, t.n);
+  const int lane = threadIdx.x & 31;
+  const float decay = __fsub_rn(1.0f, __fmul_rn(lr, wd));
+  const float w1 = __fsub_rn(1.0f, beta1), w2 = __fsub_rn(1.0f, beta2);
+  const bool vec = aligned16(t.p) && aligned16(t.g) && aligned16(t.shadow) &&
+                   ((reinterpret_cast<uintptr_t>(t.mq) | reinterpret_cast<uintptr_t>(t.vq)) & 7) == 0;
+  for (long long b0 = start + 256ll * (threadIdx.x >> 5); b0 < end; b0 += 256ll * (blockDim.x >> 5)) {
+    const long long i = b0 + 8 * lane;
+    const bool whole = vec && i + 8 <= end;
+    const int n = end - i >= 8 ? 8 : (end > i ? (int)(end - i) : 0);
+    const float ms = t.m_scale[b0 >> 8], rs = t.r_scale[b0 >> 8];
+    float p[8], g[8], m[8], r[8];
+    uint32_t cm[2] = {0u, 0u}, cr[2] = {0u, 0u};
+    if (whole) {
+      const float4 p0 = *reinterpret_cast<const float4*>(t.p + i), p1 = *reinterpret_cast<const float4*>(t.p + i + 4);
+      const float4 g0 = *reinterpret_cast<const float4*>(t.g + i), g1 = *reinterpret_cast<const float4*>(t.g + i + 4);
+      const uint2 a = *reinterpret_cast<const uint2*>(t.mq + i), b = *reinterpret_cast<const uint2*>(t.vq + i);
+      p[0] = p0.x, p[1] = p0.y, p[2] = p0.z, p[3] = p0.w, p[4] = p1.x, p[5] = p1.y, p[6] = p1.z, p[7] = p1.w;
+      g[0] = g0.x, g[1] = g0.y, g[2] = g0.z, g[3] = g0.w, g[4] = g1.x, g[5] = g1.y, g[6] = g1.z, g[7] = g1.w;
+      cm[0] = a.x, cm[1] = a.y, cr[0] = b.x, cr[1] = b.y;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        p[k] = k < n ? t.p[i + k] : 0.f;
+        g[k] = k < n ? t.g[i + k] : 0.f;
+        cm[k >> 2] |= (k < n ? (uint32_t)t.mq[i + k] : 0u) << (8 * (k & 3));
+        cr[k >> 2] |= (k < n ? (uint32_t)t.vq[i + k] : 0u) << (8 * (k & 3));
+      }
+    }
+    float am = 0.f, ar = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      const float2 c = a8_decode_m2((cm[k >> 2] >> (8 * (k & 3))) & 0xFFFFu);
+      m[k] = __fmul_rn(c.x, ms);
+      m[k + 1] = __fmul_rn(c.y, ms);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float q = __fmul_rn(a8_decode_r((cr[k >> 2] >> (8 * (k & 3))) & 0xFFu), rs);
+      m[k] = __fadd_rn(__fmul_rn(m[k], beta1), __fmul_rn(g[k], w1));
+      r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q, q), beta2), __fmul_rn(__fmul_rn(g[k], g[k]), w2)));
+      const float u = __fmul_rn(__fdiv_rn(m[k], __fadd_rn(__fmul_rn(r[k], inv_sqrt_bc2), eps)), inv_bc1);
+      p[k] = __fsub_rn(__fmul_rn(p[k], decay), __fmul_rn(u, lr));
+      am = fmaxf(am, fabsf(m[k]));
+      ar = fmaxf(ar, r[k]);
+    }
+    am = warp_max(am);
+    ar = warp_max(ar);
+    if (!(am > A8_TINY)) am = 0.f;
+    if (!(ar > A8_TINY)) ar = 0.f;
+    const float im = am > 0.f ? __fmul_rn(__frcp_rn(am), A8_M_TOP) : 0.f;
+    const float ir = ar > 0.f ? __fmul_rn(__frcp_rn(ar), A8_R_TOP) : 0.f;
+    cm[0] = cm[1] = cr[0] = cr[1] = 0u;
+#pragma unroll
+    for (int k = 0; k < 8; k += 2)
+      cm[k >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(m[k], im), __fmul_rn(m[k + 1], im)),
+                                                       __NV_SATFINITE, __NV_E4M3)
+                    << (8 * (k & 3));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t q = a8_encode_r(__fmul_rn(r[k], ir));
+      cr[k >> 2] |= ((r[k] > 0.f && q == 0u) ? 1u : q) << (8 * (k & 3));
+    }
+    if (lane == 0) {
+      t.m_scale[b0 >> 8] = __fmul_rn(am, A8_M_STEP);
+      t.r_scale[b0 >> 8] = __fmul_rn(ar, A8_R_STEP);
+    }
+    if (whole) {
+      *reinterpret_cast<float4*>(t.p + i) = make_float4(p[0], p[1], p[2], p[3]);
+      *reinterpret_cast<float4*>(t.p + i + 4) = make_float4(p[4], p[5], p[6], p[7]);
+      *reinterpret_cast<uint2*>(t.mq + i) = make_uint2(cm[0], cm[1]);
+      *reinterpret_cast<uint2*>(t.vq + i) = make_uint2(cr[0], cr[1]);
+      if (t.shadow)
+        *reinterpret_cast<uint4*>(t.shadow + i) = make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
+                                                             pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= n) continue;
+        t.p[i + k] = p[k];
+        t.mq[i + k] = (unsigned char)(cm[k >> 2] >> (8 * (k & 3)));
+        t.vq[i + k] = (unsigned char)(cr[k >> 2] >> (8 * (k & 3)));
+        if (t.shadow) t.shadow[i + k] = __bfloat16_as_ushort(__float2bfloat16(p[k]));
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) adamw8_moments_kernel(const unsigned char* __restrict__ mq,
+                                                             const float* __restrict__ ms,
+                                                             const unsigned char* __restrict__ vq,
+                                                             const float* __restrict__ rs, float* __restrict__ m,
+                                                             float* __restrict__ v, long long n) {
+  griddep_wait();
+  griddep_launch();
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    const float r = __fmul_rn(a8_decode_r(vq[i]), rs[i >> 8]);
+    m[i] = __fmul_rn(a8_decode_m2(mq[i]).x, ms[i >> 8]);
+    v[i] = __fmul_rn(r, r);
   }
 }
 
@@ -459,6 +604,32 @@ extern "C" int rgpt_adamw(const RgptAdamwTensor* table, const int* chunk_tensor,
   launch_pdl(adamw_kernel, dim3(n_chunks), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1, 
       table, chunk_tensor, chunk_start, chunk_elems, lr, wd, beta1, beta2, eps, inv_bc1, inv_sqrt_bc2, hp);
   return rgpt_check_launch("adamw_kernel");
+}
+
+extern "C" int rgpt_adamw8(const RgptAdamw8Tensor* table, const int* chunk_tensor, const long long* chunk_start,
+                           int n_chunks, int chunk_elems, float lr, float wd, float beta1, float beta2, float eps,
+                           int step, const float* hp, void* stream) {
+  if (n_chunks <= 0) return RGPT_OK;
+  if (chunk_elems < RGPT_ADAMW8_BLOCK || chunk_elems % RGPT_ADAMW8_BLOCK != 0)
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "adamw8: chunk_elems must be a multiple of %d", RGPT_ADAMW8_BLOCK);
+  float inv_bc1 = 0.f, inv_sqrt_bc2 = 0.f;
+  if (hp == nullptr) {
+    if (step < 1) return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "adamw8 step must be >= 1");
+    inv_bc1 = (float)(1.0 / (1.0 - pow((double)beta1, (double)step)));
+    inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow((double)beta2, (double)step)));
+  }
+  launch_pdl(adamw8_kernel, dim3(n_chunks), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1, table, chunk_tensor,
+             chunk_start, chunk_elems, lr, wd, beta1, beta2, eps, inv_bc1, inv_sqrt_bc2, hp);
+  return rgpt_check_launch("adamw8_kernel");
+}
+
+extern "C" int rgpt_adamw8_moments(const unsigned char* mq, const float* m_scale, const unsigned char* vq,
+                                   const float* r_scale, float* m, float* v, long long n, void* stream) {
+  if (n <= 0) return RGPT_OK;
+  const long long want = (n + 255) / 256;
+  launch_pdl(adamw8_moments_kernel, dim3((unsigned)(want < 148 * 64 ? want : 148 * 64)), dim3(256), 0,
+             reinterpret_cast<cudaStream_t>(stream), 1, mq, m_scale, vq, r_scale, m, v, n);
+  return rgpt_check_launch("adamw8_moments_kernel");
 }
 
 extern "C" int rgpt_muon_prep(const RgptMuonTensor* table, int n, int R, int C, void* X, long long x_bstride, int ldx,

@@ -333,10 +333,11 @@ class Engine:
 
     # ------------------------------------------------------------------ forward
     @torch.no_grad()
-    def forward(self, input_ids, labels=None, *, training=True, want_loss=False, grad_scale=1.0):
+    def forward(self, input_ids, labels=None, *, training=True, want_loss=False, grad_scale=1.0, head=True):
         """Run the model forward (and, with want_loss, the fused loss + in-place dlogits).
 
-        Returns the _Acts holding logits / losses. grad_scale multiplies the stored dlogits."""
+        Returns the _Acts holding logits / losses. grad_scale multiplies the stored dlogits. head=False
+        stops at the final norm (A.hf): no logits."""
         m = self.model
         self.sync_shadows()
         B, T = input_ids.shape
@@ -373,6 +374,8 @@ class Engine:
                 nv.gemm_argmax(A.hq[r], self.lm_w, A.amax_val, A.amax_idx, A.argmax[r])
         kind, eps, alpha, w, temp = self._resid_norm(m, "ln_f")
         nv.rownorm_fwd(A.x[app], A.hf, kind, eps, w=w, temp=1.0, alpha=alpha)
+        if not head:
+            return A
         nv.gemm(A.hf, self.lm_w, A.logits)
         if want_loss:
             A.losses.zero_()

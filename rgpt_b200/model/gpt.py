@@ -11,12 +11,16 @@ Two execution paths share one native engine (model/engine.py):
   and the in-place bf16 dlogits in one pass, then ``loss.backward()`` runs the
   native backward. Returns (total_loss, token_loss, q_loss) as 0-d tensors.
 
+Post-training: ``token_logprobs`` scores labels without storing logits, and
+``preference_loss`` / ``policy_loss`` are training losses like ``forward_loss``.
+
 Weight gradients are accumulated into a flat fp32 arena whose views are the
 parameters' ``.grad`` (use the optimizer's ``zero_grad`` to clear them).
 """
 import torch
 import torch.nn as nn
 
+from .. import native as nv
 from .config import as_config
 from .engine import Engine
 from .norm import functional_l2_norm, functional_rms_norm, get_norm_fn
@@ -80,6 +84,25 @@ class _GPTForward(torch.autograd.Function):
                 dq[..., 0] += d_halt.float() * (torch.sigmoid(A.q[..., 0]) - ctx.correct) / M
             A.dq.copy_(dq)
         eng.backward(A, dlogits=dl)
+        return None, None, None, None
+
+
+class _GPTPostTraining(torch.autograd.Function):
+    """A post-training loss on the model's logits: `loss_fn(logits, dlogits)` writes its outputs and the gradient,
+    in place over the engine's logits when there is one to take. The first output is differentiable."""
+
+    @staticmethod
+    def forward(ctx, input_ids, eng, loss_fn, anchor):
+        A = eng.forward(input_ids, None, training=True, want_loss=False)
+        logits = A.logits.view(*input_ids.shape, -1)
+        outs = loss_fn(logits, logits)
+        ctx.eng, ctx.acts = eng, A
+        ctx.mark_non_differentiable(*outs[1:])
+        return outs
+
+    @staticmethod
+    def backward(ctx, g, *unused):
+        ctx.eng.backward(ctx.acts, alpha_dev=g.reshape(1).float().contiguous())
         return None, None, None, None
 
 
@@ -174,6 +197,67 @@ class GPT(nn.Module):
         eng = self.engine()
         A = eng.forward(input_ids, labels, training=False, want_loss=True)
         return A.loss_rows.view(input_ids.shape).clone()
+
+    @torch.no_grad()
+    def token_logprobs(self, input_ids, labels):
+        """Log-probability of each label [B, T] (fp32; 0 where labels == pad_token_id or outside the vocabulary) of an
+        eval-mode forward, e.g. of a frozen reference or of the policy that sampled them. The logits are never stored:
+        the lm_head GEMM keeps each row's sum of exponentials. They are rounded to bf16 as the stored logits of
+        forward / preference_loss / policy_loss are, so the same weights give the same log-probabilities."""
+        eng = self.engine()
+        A = eng.forward(input_ids, None, training=False, want_loss=False, head=False)
+        lab = labels.reshape(-1).long().contiguous()
+        out = torch.empty(lab.shape, device=lab.device, dtype=torch.float32)
+        nv.linear_logprobs(A.hf, eng.lm_w, lab, out, ignore_index=eng.ignore_index, round_bf16=True)
+        return out.view(input_ids.shape)
+
+    def _post_training_loss(self, input_ids, loss_fn):
+        eng = self.engine()
+        if torch.is_grad_enabled() and self.training:
+            return _GPTPostTraining.apply(input_ids, eng, loss_fn, self._anchor())
+        with torch.no_grad():
+            A = eng.forward(input_ids, None, training=False, want_loss=False)
+            return loss_fn(A.logits.view(*input_ids.shape, -1), None)
+
+    def preference_loss(self, input_ids, labels, ref_logps=None, *, kind="sigmoid", beta=0.1, label_smoothing=0.0,
+                        margin=0.0, average=False):
+        """Paired preference loss (native.preference_loss) of input_ids, labels [2P, T]: the P chosen sequences, then
+        the P rejected ones; labels == pad_token_id (prompts, padding) are not scored. ref_logps [2P]: the frozen
+        reference's summed (averaged, with `average`) token_logprobs. Returns (loss, sequence log-probabilities [2P],
+        margins [P]); the loss is differentiable in training mode. Halting losses are not part of it."""
+        labels = labels.long().contiguous()
+        new = lambda *s: torch.empty(*s, device=labels.device, dtype=torch.float32)  # noqa: E731
+
+        def loss_fn(logits, dlogits):
+            B, T = labels.shape
+            loss, seq, margins = new(1), new(B), new(B // 2)
+            nv.preference_loss(logits, labels, ref_logps, token_logps=new(B, T), lse=new(B, T), seq_logps=seq,
+                               margins=margins, coef=new(B), loss=loss, dlogits=dlogits, kind=kind, beta=beta,
+                               label_smoothing=label_smoothing, margin=margin, average=average,
+                               ignore_index=self.engine().ignore_index)
+            return loss.view(()), seq, margins
+
+        return self._post_training_loss(input_ids, loss_fn)
+
+    def policy_loss(self, input_ids, labels, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=0.2,
+                    kl_coef=0.0, by_sequence=False):
+        """Clipped policy loss with a KL term (native.policy_loss) of input_ids, labels [B, T] (the sampled tokens;
+        pad_token_id where not scored); old_logps and ref_logps [B, T]: token_logprobs of the sampling policy and of
+        the frozen reference; advantages [B] or [B, T]. Returns (loss, stats [4], token log-probabilities [B, T]); the
+        loss is differentiable in training mode. Halting losses are not part of it."""
+        labels = labels.long().contiguous()
+        new = lambda *s, dt=torch.float32: torch.empty(*s, device=labels.device, dtype=dt)  # noqa: E731
+
+        def loss_fn(logits, dlogits):
+            B, T = labels.shape
+            stats, logps = new(4), new(B, T)
+            nv.policy_loss(logits, labels, old_logps, advantages, ref_logps, token_logps=logps,
+                           counts=new(B, dt=torch.int32), stats=stats, dlogits=dlogits, clip_low=clip_low,
+                           clip_high=clip_high, kl_coef=kl_coef, by_sequence=by_sequence,
+                           ignore_index=self.engine().ignore_index)
+            return stats[0].clone(), stats, logps
+
+        return self._post_training_loss(input_ids, loss_fn)
 
     def forward_loss(self, input_ids, labels):
         """Fused forward + loss; returns (total, token, q) 0-d tensors, total differentiable."""

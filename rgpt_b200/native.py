@@ -20,6 +20,8 @@ EPI_POLY_BF16 = 6
 EPI_BIAS_SIGMOID_BF16 = 7
 EPI_POLY_F32 = 8
 EPI_ARGMAX_BF16 = 9
+EPI_LSE_F32 = 10             # linear_logprobs only
+EPI_SOFTMAX_GRAD_BF16 = 11   # linear_logprobs_bwd only
 
 ACTIVATIONS = {"none": 0, "identity": 0, "squared_relu": 1, "gelu": 2, "silu": 3, "mish": 4}
 ACT_SQRELU = 1
@@ -352,6 +354,270 @@ def halt_losses(q: torch.Tensor, argmax: torch.Tensor, labels: torch.Tensor, dq:
               _lib.stream_ptr(q.device))
 
 
+# ----------------------------------------------------------------------------- post-training losses
+LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
+
+
+def _call_on(device: torch.device, name: str, *args, kernels: int | None = None) -> None:
+    """_lib.call with `device` current (the library launches on the current device's context)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(name, *args, kernels=kernels)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, kernels=kernels)
+
+
+def _flat(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device) -> int:
+    """Address of a contiguous tensor of the given shape, type and device (the caller's ptr() of another argument
+    sees to it that the device is a GPU)."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}"
+                         f" with strides {t.stride()}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return t.data_ptr()
+
+
+def _opt(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype, device: torch.device) -> int | None:
+    return None if t is None else _flat(t, name, shape, dtype, device)
+
+
+def _logit_rows(t: torch.Tensor, name: str):
+    """(dtype id, batch stride, token stride, B, T, V) of logits [B, T, V], or [M, V] as M sequences of one token."""
+    if t.dtype not in LOGIT_DTYPES:
+        raise TypeError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
+    if t.dim() not in (2, 3):
+        raise ValueError(f"{name} must be [M, V] or [B, T, V], got {tuple(t.shape)}")
+    V = t.shape[-1]
+    if V > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride along the vocabulary, got strides {t.stride()}")
+    if t.dim() == 2:
+        B, T, sb, st = t.shape[0], 1, t.stride(0), 0
+    else:
+        (B, T), (sb, st) = t.shape[:2], t.stride()[:2]
+    if t.numel() and (B * T >= 2 ** 31 or V >= 2 ** 31):
+        raise ValueError(f"{name} must have fewer than 2^31 rows and columns, got {tuple(t.shape)}")
+    return LOGIT_DTYPES[t.dtype], sb, st, B, T, V
+
+
+def _span(t: torch.Tensor):
+    """[first, last) address of a tensor's elements."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):
+    """(address, batch stride, token stride) of the gradient's rows: the logits themselves, or memory apart from them."""
+    if dlogits is None:
+        return None, 0, 0
+    if dlogits.dtype != logits.dtype or dlogits.shape != logits.shape or dlogits.device != logits.device:
+        raise ValueError("dlogits must have the logits' type, shape and device")
+    _, sb, st, B, T, V = _logit_rows(dlogits, "dlogits")
+    tokens = T == 1 or st >= V
+    if not (tokens and (B == 1 or sb >= (T - 1) * st + V)) and not (sb >= V and st >= (B - 1) * sb + V):
+        raise ValueError(f"the rows of dlogits overlap (strides {dlogits.stride()})")
+    if dlogits.data_ptr() != logits.data_ptr() or dlogits.stride() != logits.stride():
+        (a, b), (c, d) = _span(logits), _span(dlogits)
+        if a < d and c < b:
+            raise ValueError("dlogits must be the logits themselves or share no memory with them")
+    return dlogits.data_ptr(), sb, st
+
+
+def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, logps: torch.Tensor, *, lse: torch.Tensor | None = None,
+                   ignore_index: int = -100) -> None:
+    """logps = log softmax(logits)[label], 0 for tokens that are not scored (label ignore_index or outside the
+    vocabulary); lse (optional, for token_logprobs_bwd) = logsumexp. logits [M, V] or [B, T, V] in bf16, fp16 or fp32
+    with unit stride along the vocabulary and any other strides; labels int64, logps and lse fp32 of the leading shape."""
+    dt, sb, st, B, T, V = _logit_rows(logits, "logits")
+    dev, shape = logits.device, logits.shape[:-1]
+    args = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
+            _flat(logps, "logps", shape, torch.float32, dev), _opt(lse, "lse", shape, torch.float32, dev))
+    if B * T == 0:
+        return
+    if V == 0:
+        raise ValueError("token_logprobs: the vocabulary is empty")
+    _call_on(dev, "rgpt_token_logprobs", ptr(logits), dt, sb, st, B, T, V, *args, _lib.stream_ptr(dev))
+
+
+def token_logprobs_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, dlogps: torch.Tensor,
+                       dlogits: torch.Tensor, *, ignore_index: int = -100) -> None:
+    """dlogits = dlogps * (onehot(label) - softmax(logits)), zero rows for tokens that are not scored. dlogits: the
+    logits themselves (overwritten) or another tensor of their type and shape."""
+    dt, sb, st, B, T, V = _logit_rows(logits, "logits")
+    dev, shape = logits.device, logits.shape[:-1]
+    args = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
+            _flat(lse, "lse", shape, torch.float32, dev), _flat(dlogps, "dlogps", shape, torch.float32, dev))
+    grad = _grad_rows(dlogits, logits)
+    if B * T == 0 or V == 0:
+        return
+    _call_on(dev, "rgpt_token_logprobs_bwd", ptr(logits), dt, sb, st, B, T, V, *args, *grad, _lib.stream_ptr(dev))
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
+                    token_logps: torch.Tensor, lse: torch.Tensor, seq_logps: torch.Tensor, margins: torch.Tensor,
+                    coef: torch.Tensor, loss: torch.Tensor, dlogits: torch.Tensor | None = None,
+                    scratch: torch.Tensor | None = None, kind: str = "sigmoid", beta: float = 0.1,
+                    label_smoothing: float = 0.0, margin: float = 0.0, average: bool = False,
+                    ignore_index: int = -100, grad_scale: float = 1.0) -> None:
+    """Paired preference loss from logits [2P, T, V]: sequences 0..P-1 are the chosen ones, P..2P-1 the rejected ones.
+
+    h = beta * ((s_chosen - ref_chosen) - (s_rejected - ref_rejected)) - margin with s the sum of a sequence's scored
+    log-probabilities (their mean with `average`) and ref_logps [2P] the same of a frozen reference (None: 0);
+    kind "sigmoid" (with label_smoothing), "hinge" max(0, 1 - h) or "squared" (h - 1/2)^2; loss [1] is the pairs' mean.
+    Written: token_logps, lse [2P, T], seq_logps [2P], margins [P] (h), coef [2P] (grad_scale * d loss / d each scored
+    log-probability), loss [1], and dlogits = grad_scale * d loss / d logits when given (the logits themselves, or
+    another tensor of their type and shape). scratch: fp64 [2P, T] (allocated when None)."""
+    if kind not in PREFERENCE_KINDS:
+        raise ValueError(f"preference_loss: kind must be one of {sorted(PREFERENCE_KINDS)}, got {kind!r}")
+    if not 0.0 <= label_smoothing <= 0.5 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError("preference_loss: label_smoothing must be in [0, 0.5], and 0 unless kind is 'sigmoid'")
+    if not 0.0 < beta < float("inf"):
+        raise ValueError(f"preference_loss: beta must be positive and finite, got {beta}")
+    dt, sb, st, B, T, V = _logit_rows(logits, "logits")
+    if logits.dim() != 3 or B % 2 or B == 0 or T == 0 or V == 0:
+        raise ValueError(f"preference_loss needs logits [2P, T, V] of at least one pair and token, got {tuple(logits.shape)}")
+    dev, P, f32 = logits.device, B // 2, torch.float32
+    lab = _flat(labels, "labels", (B, T), torch.int64, dev)
+    ref = _opt(ref_logps, "ref_logps", (B,), f32, dev)
+    outs = (_flat(token_logps, "token_logps", (B, T), f32, dev), _flat(lse, "lse", (B, T), f32, dev),
+            _flat(seq_logps, "seq_logps", (B,), f32, dev), _flat(margins, "margins", (P,), f32, dev),
+            _flat(coef, "coef", (B,), f32, dev), _flat(loss, "loss", (1,), f32, dev))
+    grad = _grad_rows(dlogits, logits)
+    _opt(scratch, "scratch", (B, T), torch.float64, dev)
+    at = ptr(logits)
+    if scratch is None:
+        scratch = torch.empty(B, T, device=dev, dtype=torch.float64)
+    _call_on(dev, "rgpt_preference_loss", at, dt, sb, st, P, T, V, lab, int(ignore_index), ref,
+             PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
+             float(grad_scale), *outs, scratch.data_ptr(), *grad, _lib.stream_ptr(dev),
+             kernels=3 + (dlogits is not None))
+
+
+def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
+                ref_logps: torch.Tensor | None = None, *, token_logps: torch.Tensor, counts: torch.Tensor,
+                stats: torch.Tensor, lse: torch.Tensor | None = None, coef: torch.Tensor | None = None,
+                dlogits: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0,
+                by_sequence: bool = False, ignore_index: int = -100, grad_scale: float = 1.0) -> None:
+    """Clipped policy loss with a KL term from logits [B, T, V] (or [M, V]: sequences of one token).
+
+    Per scored token with ratio r = exp(logp - old_logps): -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+    + kl_coef * (exp(q) - q - 1), q = ref_logps - logp; averaged over the scored tokens, or with by_sequence over each
+    sequence's tokens first and then over the sequences that have any. advantages A: [B], or one per token [B, T].
+    Written: token_logps [B, T], counts [B] int32 (scored tokens), stats [4] = (loss, policy term, KL, clipped share),
+    lse and coef [B, T] when given (coef = grad_scale * d loss / d logp, for token_logprobs_bwd), and dlogits =
+    grad_scale * d loss / d logits when given (the logits themselves, or another tensor of their type and shape)."""
+    if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float("inf"):
+        raise ValueError(f"policy_loss: clip_low must be in [0, 1] and clip_high >= 0, got {clip_low} and {clip_high}")
+    if kl_coef != 0.0 and ref_logps is None:
+        raise ValueError("policy_loss: kl_coef needs ref_logps")
+    dt, sb, st, B, T, V = _logit_rows(logits, "logits")
+    dev, shape, f32 = logits.device, logits.shape[:-1], torch.float32
+    per_token = tuple(advantages.shape) != (B,)
+    adv = _flat(advantages, "advantages", shape if per_token else (B,), f32, dev)
+    ins = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
+           _flat(old_logps, "old_logps", shape, f32, dev), _opt(ref_logps, "ref_logps", shape, f32, dev))
+    outs = (_flat(token_logps, "token_logps", shape, f32, dev), _flat(counts, "counts", (B,), torch.int32, dev),
+            _flat(stats, "stats", (4,), f32, dev), _opt(lse, "lse", shape, f32, dev), _opt(coef, "coef", shape, f32, dev))
+    grad = _grad_rows(dlogits, logits)
+    if B * T == 0 or V == 0:
+        raise ValueError(f"policy_loss needs at least one token, got logits {tuple(logits.shape)}")
+    _call_on(dev, "rgpt_policy_loss", ptr(logits), dt, sb, st, B, T, V, *ins, adv, int(per_token), float(clip_low),
+             float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *outs, *grad,
+             _lib.stream_ptr(dev), kernels=3)
+
+
+def _linear_operands(x: torch.Tensor, w: torch.Tensor):
+    for t, n in ((x, "x"), (w, "w")):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{n} must be bf16, got {t.dtype}")
+        if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < t.shape[1]:
+            raise ValueError(f"{n} must be [rows, K] with unit stride along K and a row stride that is a multiple of 8,"
+                             f" got {tuple(t.shape)} with strides {t.stride()}")
+    (M, K), (V, K2) = x.shape, w.shape
+    if K != K2 or K == 0 or V == 0 or w.device != x.device:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} must share K >= 1 and the device, with V >= 1")
+    if M >= 2 ** 31 or V >= 2 ** 31:
+        raise ValueError("linear_logprobs needs fewer than 2^31 rows and columns")
+    return M, V, K
+
+
+def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logps: torch.Tensor, *,
+                    lse: torch.Tensor | None = None, part: torch.Tensor | None = None, ignore_index: int = -100,
+                    round_bf16: bool = False) -> None:
+    """logps [M] = log softmax(x @ w^T)[label] (0 where not scored) without storing the logits: x [M, K], w [V, K] bf16.
+
+    lse [M] (optional, for linear_logprobs_bwd) is written for every row. round_bf16: the products are rounded to bf16
+    first, which gives what token_logprobs gives on stored bf16 logits. part: fp32 scratch of at least
+    2 * M * ceil(V/128) elements (allocated when None)."""
+    M, V, K = _linear_operands(x, w)
+    dev = x.device
+    need = 2 * M * ((V + 127) // 128)
+    lab = _flat(labels, "labels", (M,), torch.int64, dev)
+    outs = (_flat(logps, "logps", (M,), torch.float32, dev), _opt(lse, "lse", (M,), torch.float32, dev))
+    if part is not None and (part.numel() < need or part.dtype != torch.float32 or not part.is_contiguous()
+                             or part.device != dev):
+        raise ValueError(f"linear_logprobs: part must be a contiguous fp32 tensor of at least {need} elements")
+    if M == 0:
+        return
+    if part is None:
+        part = torch.empty(need, device=dev, dtype=torch.float32)
+    _call_on(dev, "rgpt_linear_logprobs", ptr(x), x.stride(0), ptr(w), w.stride(0), M, V, K, lab, int(ignore_index),
+             int(bool(round_bf16)), ptr(part), part.numel(), *outs, _lib.stream_ptr(dev))
+
+
+# Gradient rows of linear_logprobs_bwd in flight: at most this many bf16 logit gradients (1 GiB) at a time.
+LINEAR_CHUNK_ELEMS = 1 << 29
+
+
+def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, dlogps: torch.Tensor,
+                        dx: torch.Tensor | None, dw: torch.Tensor | None, *, ignore_index: int = -100,
+                        chunk_rows: int | None = None) -> None:
+    """The gradients of linear_logprobs (round_bf16=False): dx [M, K] written in bf16 or fp32; dw [V, K] written when
+    bf16, ACCUMULATED when fp32. Either may be None. The logits' gradient exists for chunk_rows rows at a time (default:
+    as many as fit 1 GiB): its tiles come from the recomputed product, rounded to bf16 for the two GEMMs that follow."""
+    M, V, K = _linear_operands(x, w)
+    dev = x.device
+    _flat(labels, "labels", (M,), torch.int64, dev)
+    _flat(lse, "lse", (M,), torch.float32, dev)
+    _flat(dlogps, "dlogps", (M,), torch.float32, dev)
+    for t, n, shape in ((dx, "dx", (M, K)), (dw, "dw", (V, K))):
+        if t is not None and (tuple(t.shape) != shape or t.dtype not in (torch.bfloat16, torch.float32)
+                              or t.stride(1) != 1 or t.stride(0) % 8 or t.device != dev):
+            raise ValueError(f"{n} must be a bf16 or fp32 {shape} tensor with unit column stride and a row stride that is"
+                             f" a multiple of 8")
+    if chunk_rows is not None and chunk_rows < 1:
+        raise ValueError("linear_logprobs_bwd: chunk_rows must be at least 1")
+    if M == 0:
+        if dw is not None and dw.dtype == torch.bfloat16:
+            dw.zero_()
+        return
+    ld = (V + 7) // 8 * 8
+    rows = min(M, chunk_rows or max(256, LINEAR_CHUNK_ELEMS // ld // 256 * 256))
+    with torch.cuda.device(dev):
+        dl = torch.empty(rows, ld, device=dev, dtype=torch.bfloat16)[:, :V]
+        acc = dw
+        if dw is not None and dw.dtype == torch.bfloat16 and rows < M:
+            acc = torch.zeros(V, K, device=dev, dtype=torch.float32)
+        for a in range(0, M, rows):
+            n = min(rows, M - a)
+            xa, d = x[a:a + n], dl[:n]
+            _lib.call("rgpt_linear_logprobs_dlogits", ptr(xa), x.stride(0), ptr(w), w.stride(0), n, V, K,
+                      ptr(labels[a:a + n]), int(ignore_index), ptr(lse[a:a + n]), ptr(dlogps[a:a + n]), ptr(d), ld,
+                      _lib.stream_ptr(dev))
+            if dx is not None:
+                gemm(d, w.t(), dx[a:a + n], epi=EPI_STORE_BF16 if dx.dtype == torch.bfloat16 else EPI_STORE_F32)
+            if acc is not None:
+                if acc.dtype == torch.bfloat16:
+                    gemm(d.t(), xa.t(), acc)
+                else:
+                    gemm(d.t(), xa.t(), acc, epi=EPI_ACCUM_F32, splitk=0)
+        if acc is not dw:
+            dw.copy_(acc)
+
+
 # ----------------------------------------------------------------------------- optimizer
 # hp: optional device pointer (int) to a parameter group's block of RGPT_HP_FLOATS scalars; when
 # given, the kernels read this step's lr / betas / bias corrections from it instead of the arguments.
@@ -363,6 +629,29 @@ def adamw(table: torch.Tensor, chunk_tensor: torch.Tensor, chunk_start: torch.Te
     _lib.call("rgpt_adamw", ptr(table), ptr(chunk_tensor), ptr(chunk_start), chunk_tensor.numel(), chunk_elems,
               float(lr), float(wd), float(beta1), float(beta2), float(eps), int(step), hp,
               _lib.stream_ptr(table.device))
+
+
+ADAM8_BLOCK = 256  # elements that share a scale
+
+
+def adamw8(table: torch.Tensor, chunk_tensor: torch.Tensor, chunk_start: torch.Tensor, chunk_elems: int, lr: float,
+           wd: float, beta1: float, beta2: float, eps: float, step: int, hp: int | None = None) -> None:
+    """adamw with both moments in 8 bits; table rows: p, g, m codes, m scales, v codes, v scales, shadow, n."""
+    _lib.call("rgpt_adamw8", ptr(table), ptr(chunk_tensor), ptr(chunk_start), chunk_tensor.numel(), chunk_elems,
+              float(lr), float(wd), float(beta1), float(beta2), float(eps), int(step), hp,
+              _lib.stream_ptr(table.device))
+
+
+def adamw8_moments(mq: torch.Tensor, m_scale: torch.Tensor, vq: torch.Tensor, v_scale: torch.Tensor, m: torch.Tensor,
+                   v: torch.Tensor) -> None:
+    """m, v (fp32) = the moments that 8-bit codes and their scales stand for."""
+    n, dev = m.numel(), m.device
+    blocks = (n + ADAM8_BLOCK - 1) // ADAM8_BLOCK
+    args = (_flat(mq.view(-1), "m codes", (n,), torch.uint8, dev), _flat(m_scale, "m scales", (blocks,), torch.float32, dev),
+            _flat(vq.view(-1), "v codes", (n,), torch.uint8, dev), _flat(v_scale, "v scales", (blocks,), torch.float32, dev),
+            ptr(m), _flat(v, "v", m.shape, torch.float32, dev))
+    _flat(m, "m", m.shape, torch.float32, dev)
+    _call_on(dev, "rgpt_adamw8_moments", *args, n, _lib.stream_ptr(dev))
 
 
 def muon_prep(table, n, R, C, X, beta, nesterov, sumsq, hp: int | None = None) -> None:

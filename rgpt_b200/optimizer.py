@@ -30,6 +30,7 @@ from . import native as nv
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)  # optimizer.py:19
 _ADAM_CHUNK = 16384
+ADAM8_MIN_NUMEL = 4096  # smaller parameters keep fp32 moments under adam_state_bits=8
 _HP_RING = 4  # pinned host slots for the per-step scalars (copies in flight before a slot is reused)
 
 
@@ -261,15 +262,22 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params: List[Dict[str, Any]], lr: float = 3e-4, weight_decay: float = 0.01,
                  momentum: float = 0.95, nesterov: bool = True, adam_betas: Tuple[float, float] = (0.9, 0.95),
                  adam_eps: float = 1e-8, muon_lr_multiplier: float = 100.0, ns_steps: int = 5,
-                 ns_coeffs: Tuple[float, float, float] = NS_COEFFS, ns_precision: str = "bf16"):
-        """ns_precision: "bf16" iterates Newton-Schulz in bf16 as the reference does (optimizer.py:20-44);
+                 ns_coeffs: Tuple[float, float, float] = NS_COEFFS, ns_precision: str = "bf16",
+                 adam_state_bits: int = 32):
+        """adam_state_bits (also per group): 32 keeps the AdamW moments in fp32; 8 keeps both in 8-bit codes with fp32
+        scales for blocks of 256 elements (rgpt_adamw8 has the format) for parameters of at least 4096 elements, with
+        state keys exp_avg_q8, exp_avg_scale, exp_avg_sq_q8, exp_avg_sq_scale: 2 bytes a parameter instead of 8.
+        ns_precision: "bf16" iterates Newton-Schulz in bf16 as the reference does (optimizer.py:20-44);
         "fp32" iterates it at fp32 accuracy (hi/lo bf16 operands, fp32 accumulation) from the same bf16
         input, the update still rounded to bf16 as the reference rounds it (optimizer.py:68)."""
         if ns_precision not in ("bf16", "fp32"):
             raise ValueError(f"ns_precision must be 'bf16' or 'fp32', got {ns_precision!r}")
+        if adam_state_bits not in (8, 32):
+            raise ValueError(f"adam_state_bits must be 8 or 32, got {adam_state_bits!r}")
         defaults = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
                         adam_betas=adam_betas, adam_eps=adam_eps, muon_lr_multiplier=muon_lr_multiplier,
-                        ns_steps=ns_steps, ns_coeffs=tuple(ns_coeffs), ns_precision=ns_precision)
+                        ns_steps=ns_steps, ns_coeffs=tuple(ns_coeffs), ns_precision=ns_precision,
+                        adam_state_bits=adam_state_bits)
         super().__init__(params, defaults)
         self._cache: Dict[Any, Any] = {}
         self._hp_dev: Optional[torch.Tensor] = None
@@ -341,8 +349,8 @@ class Muon(torch.optim.Optimizer):
     # ------------------------------------------------------------------ state
     def load_state_dict(self, state_dict):
         """torch's loader casts every state tensor to its parameter's dtype, which would turn the bf16
-        momentum buffers into fp32. Restore the kernels' dtypes (momentum_buffer bf16, AdamW moments
-        fp32), and copy into the state tensors that already exist: their addresses are baked into the
+        momentum buffers into fp32. Restore the kernels' dtypes (momentum_buffer bf16, 8-bit codes
+        uint8, the rest fp32), and copy into the state tensors that already exist: their addresses are baked into the
         update kernels' descriptor tables and into captured CUDA graphs of the step."""
         before = {p: dict(st) for p, st in self.state.items()}
         super().load_state_dict(state_dict)
@@ -351,7 +359,8 @@ class Muon(torch.optim.Optimizer):
                 for k, v in list(st.items()):
                     if not torch.is_tensor(v) or not v.is_floating_point():
                         continue
-                    want = torch.bfloat16 if k == "momentum_buffer" else torch.float32
+                    want = (torch.bfloat16 if k == "momentum_buffer" else torch.uint8 if k.endswith("_q8")
+                            else torch.float32)
                     old = before.get(p, {}).get(k)
                     if old is not None and old.shape == v.shape and old.dtype == want:
                         old.copy_(v)
@@ -507,11 +516,28 @@ class Muon(torch.optim.Optimizer):
             group["_adam_step"] = step_i
         if not params:
             return []
+        bits = group.get("adam_state_bits", 32)
+        if bits not in (8, 32):
+            raise ValueError(f"adam_state_bits must be 8 or 32, got {bits!r}")
+        jobs = []
+        if bits == 8:
+            if slices is not None:
+                raise ValueError("the sharded step cuts AdamW slices inside the blocks of 8-bit moments: "
+                                 "use adam_state_bits=32 with sharded_state=True")
+            small = [p for p in params if p.numel() < ADAM8_MIN_NUMEL]
+            large = [p for p in params if p.numel() >= ADAM8_MIN_NUMEL]
+            if large:
+                jobs.append(self._adamw8_job(gi, large, lr, wd, float(beta1), float(beta2), eps, step_i))
+            params = small
+            if not params:
+                return jobs
         for p in params:
             st = self.state[p]
             if len(st) == 0:
                 st["exp_avg"] = torch.zeros_like(p)
                 st["exp_avg_sq"] = torch.zeros_like(p)
+            elif "exp_avg" not in st:
+                raise ValueError("this parameter's moments are in 8 bits, but its group asks for adam_state_bits=32")
         ranges = slices if slices is not None else [(p, 0, p.numel()) for p in params]
         rows = []
         for p, lo, hi in ranges:
@@ -533,8 +559,51 @@ class Muon(torch.optim.Optimizer):
                    torch.tensor(cs, dtype=torch.int64).to(dev))
             self._cache[key] = ent
         table, ct, cs = ent
-        return [lambda: nv.adamw(table, ct, cs, _ADAM_CHUNK, lr, wd, float(beta1), float(beta2), eps, step_i,
-                                 hp=self._hp(gi))]
+        return jobs + [lambda: nv.adamw(table, ct, cs, _ADAM_CHUNK, lr, wd, float(beta1), float(beta2), eps, step_i,
+                                        hp=self._hp(gi))]
+
+    def _adamw8_job(self, gi, params, lr, wd, beta1, beta2, eps, step_i):
+        """A closure launching the multi-tensor AdamW kernel with 8-bit moments for whole parameters."""
+        rows = []
+        for p in params:
+            st = self.state[p]
+            if len(st) == 0:
+                n = p.numel()
+                for k in ("exp_avg", "exp_avg_sq"):
+                    st[k + "_q8"] = torch.zeros(n, device=p.device, dtype=torch.uint8)
+                    st[k + "_scale"] = torch.zeros(-(-n // nv.ADAM8_BLOCK), device=p.device, dtype=torch.float32)
+            elif "exp_avg_q8" not in st:
+                raise ValueError("this parameter's moments are in fp32, but its group asks for adam_state_bits=8")
+            if p.dtype != torch.float32 or p.grad.dtype != torch.float32 or not p.is_contiguous() \
+                    or not p.grad.is_contiguous():
+                raise ValueError("8-bit AdamW needs contiguous fp32 parameters and gradients")
+            sh = getattr(p, "_rgpt_shadow", None)
+            rows.append([p.data_ptr(), p.grad.data_ptr(), st["exp_avg_q8"].data_ptr(), st["exp_avg_scale"].data_ptr(),
+                         st["exp_avg_sq_q8"].data_ptr(), st["exp_avg_sq_scale"].data_ptr(),
+                         sh.data_ptr() if sh is not None else 0, p.numel()])
+        key = ("adamw8", gi, tuple(tuple(r) for r in rows))
+        ent = self._cache.get(key)
+        if ent is None:
+            dev = params[0].device
+            pieces = [(ti, s) for ti, p in enumerate(params) for s in range(0, p.numel(), _ADAM_CHUNK)]
+            ent = (_table(rows, dev), torch.tensor([t for t, _ in pieces], dtype=torch.int32).to(dev),
+                   torch.tensor([s for _, s in pieces], dtype=torch.int64).to(dev))
+            self._cache[key] = ent
+        table, ct, cs = ent
+        return lambda: nv.adamw8(table, ct, cs, _ADAM_CHUNK, lr, wd, beta1, beta2, eps, step_i, hp=self._hp(gi))
+
+    @torch.no_grad()
+    def adam_moments(self, p: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The fp32 first and second AdamW moments of parameter p, whichever way its group holds them: the state's
+        own tensors with 32 bits, new ones decoded from their codes with 8."""
+        st = self.state.get(p, {})
+        if "exp_avg_q8" in st:
+            m, v = torch.empty_like(p), torch.empty_like(p)
+            nv.adamw8_moments(st["exp_avg_q8"], st["exp_avg_scale"], st["exp_avg_sq_q8"], st["exp_avg_sq_scale"], m, v)
+            return m, v
+        if "exp_avg" not in st:
+            raise ValueError("this parameter has no AdamW moments (no step yet, or it belongs to a Muon group)")
+        return st["exp_avg"], st["exp_avg_sq"]
 
 
 class DistMuon(Muon):
@@ -566,6 +635,9 @@ class DistMuon(Muon):
         self.sharded_state = sharded_state
         if reduce_dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("reduce_dtype must be torch.bfloat16 or torch.float32")
+        if sharded_state and any(g.get("adam_state_bits", 32) != 32 for g in self.param_groups):
+            raise ValueError("the sharded step cuts AdamW slices inside the blocks of 8-bit moments: "
+                             "use adam_state_bits=32 with sharded_state=True")
         self.reduce_dtype = reduce_dtype
         self._pending: List[Any] = []    # async all-reduces launched during the backward
         self._synced: Dict[int, bool] = {}  # arena id -> every bucket reduced in the latest backward

@@ -99,7 +99,8 @@ class Trainer:
         groups = trainer_param_groups(self.model, tie_word_embeddings=tie, weight_decay=ocfg.weight_decay)
         opt_cls = DistMuon if self.is_ddp else Muon
         self.optimizer = opt_cls(groups, lr=ocfg.lr, weight_decay=ocfg.weight_decay,
-                                 muon_lr_multiplier=self.muon_lr_multiplier)
+                                 muon_lr_multiplier=self.muon_lr_multiplier,
+                                 adam_state_bits=get(ocfg, "adam_state_bits", 32))
 
         scfg = tcfg.scheduler
         name = get(scfg, "name", "linear")
