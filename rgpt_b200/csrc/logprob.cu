@@ -33,11 +33,44 @@ constexpr float LP_WIDE = 1048576.0f;
 struct LpRows {
   long long sb, st;
   int T;
+  __device__ __forceinline__ unsigned batch(long long row) const { return (unsigned)row / (unsigned)T; }  // rows < 2^31
   __device__ __forceinline__ long long offset(long long row) const {
-    const long long b = row / T;
-    return b * sb + (row - b * T) * st;
+    const unsigned b = batch(row);
+    return (long long)b * sb + (long long)((unsigned)row - b * (unsigned)T) * st;
   }
 };
+
+// A pair of floats in one 64-bit register: the packed instructions take and give it as it is.
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 f2_get(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 f2_ex2(F2 t) {
+  const float2 v = f2_get(t);
+  return f2(ex2_approx(v.x), ex2_approx(v.y));
+}
 
 template <typename E>
 struct LpType;
@@ -46,22 +79,25 @@ struct LpType<__nv_bfloat16> {
   static constexpr int VEC = 8;
   static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16(v); }
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
+  static constexpr uint32_t LOWEST = 0xFF80FF80u;  // -inf, twice
+  static __device__ __forceinline__ void unpack(const uint4& u, F2 (&f)[4]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 p = unpack_bf16x2(w[k]);
-      f[2 * k] = p.x, f[2 * k + 1] = p.y;
-    }
+    for (int k = 0; k < 4; ++k) f[k] = f2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u));
   }
   static __device__ __forceinline__ float max8(const uint4& u) {  // packed compares: exact
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
     const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
     return fmaxf(m.x, m.y);
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                      pack_bf16x2(f[6], f[7]));
+  static __device__ __forceinline__ uint4 pack(const F2 (&f)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 p = f2_get(f[k]);
+      w[k] = pack_bf16x2(p.x, p.y);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <>
@@ -69,12 +105,13 @@ struct LpType<__half> {
   static constexpr int VEC = 8;
   static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
+  static constexpr uint32_t LOWEST = 0xFC00FC00u;
+  static __device__ __forceinline__ void unpack(const uint4& u, F2 (&f)[4]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-      f[2 * k] = p.x, f[2 * k + 1] = p.y;
+      f[k] = f2(p.x, p.y);
     }
   }
   static __device__ __forceinline__ float max8(const uint4& u) {
@@ -82,11 +119,12 @@ struct LpType<__half> {
     const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
     return fmaxf(m.x, m.y);
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
+  static __device__ __forceinline__ uint4 pack(const F2 (&f)[4]) {
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+      const float2 p = f2_get(f[k]);
+      const __half2 h = __floats2half2_rn(p.x, p.y);
       w[k] = *reinterpret_cast<const uint32_t*>(&h);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
@@ -97,14 +135,17 @@ struct LpType<float> {
   static constexpr int VEC = 4;
   static __device__ __forceinline__ float get(float v) { return v; }
   static __device__ __forceinline__ float put(float v) { return v; }
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+  static constexpr uint32_t LOWEST = 0xFF800000u;
+  static __device__ __forceinline__ void unpack(const uint4& u, F2 (&f)[2]) {
+    f[0] = f2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = f2(__uint_as_float(u.z), __uint_as_float(u.w));
   }
   static __device__ __forceinline__ float max8(const uint4& u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  static __device__ __forceinline__ uint4 pack(const F2 (&f)[2]) {
+    const float2 p = f2_get(f[0]), q = f2_get(f[1]);
+    return make_uint4(__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(q.x), __float_as_uint(q.y));
   }
 };
 
@@ -136,21 +177,20 @@ struct LpSum {
     const float nm = fmaxf(m, lm > LP_LOW ? lm * LP_LOG2E : -INFINITY), r = lp_ref(nm);
     s *= ex2_approx(m - r);
     m = nm;
-    const float2 nr = make_float2(-r, -r), l2e = make_float2(LP_LOG2E, LP_LOG2E);
-    float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
+    const F2 nr = f2(-r, -r), l2e = f2(LP_LOG2E, LP_LOG2E);
+    F2 a0 = f2(s, 0.f), a1 = f2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      float f[L::VEC];
+      F2 f[L::VEC / 2];
       L::unpack(u[k], f);
 #pragma unroll
-      for (int j = 0; j < L::VEC; j += 4) {
-        const float2 t0 = ffma2(make_float2(f[j], f[j + 1]), l2e, nr);
-        const float2 t1 = ffma2(make_float2(f[j + 2], f[j + 3]), l2e, nr);
-        a0 = fadd2(a0, make_float2(ex2_approx(t0.x), ex2_approx(t0.y)));
-        a1 = fadd2(a1, make_float2(ex2_approx(t1.x), ex2_approx(t1.y)));
+      for (int j = 0; j < L::VEC / 2; j += 2) {
+        a0 = f2_add(a0, f2_ex2(f2_fma(f[j], l2e, nr)));
+        a1 = f2_add(a1, f2_ex2(f2_fma(f[j + 1], l2e, nr)));
       }
     }
-    s += (a0.x + a0.y) + (a1.x + a1.y);
+    const float2 b = f2_get(f2_add(a0, a1));
+    s = b.x + b.y;
   }
   __device__ __forceinline__ void add(float f) {
     const float nm = fmaxf(m, f > LP_LOW ? f * LP_LOG2E : -INFINITY), r = lp_ref(nm);
@@ -206,7 +246,8 @@ __device__ __forceinline__ float2 lp_join(float2 a, LpShare sh, MERGE&& merge) {
   __syncthreads();
   float2 r = sm[0];
 #pragma unroll
-  for (int w = 1; w < LP_THREADS / 32; ++w) r = merge(r, sm[w]);
+  for (int w = 1; w < LP_THREADS / 32; ++w)
+    if (w < (int)(blockDim.x >> 5)) r = merge(r, sm[w]);
   if constexpr (CL) {
     if (threadIdx.x == 0) all = r;
     cluster_sync_all();
@@ -283,28 +324,39 @@ __device__ __forceinline__ LpRow lp_row_sum(const E* x, int V, LpShare sh) {
   return lp_careful(x, V, sh.part * LP_THREADS + (int)threadIdx.x, sh.parts * LP_THREADS, LpCtaJoin<CL>{sh});
 }
 
-// This CTA's share of coef * ([j = label] - p(x_j)) over one row; prob maps two logits to two probabilities. d may be
-// x: each thread reads an element before it writes the same one.
-template <typename E, typename P>
-__device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label, float coef, LpShare sh, P&& prob) {
+// 2^{c (x - a) - b} of two logits, times a factor
+struct LpProb {
+  F2 na, nb, k;
+  __device__ __forceinline__ LpProb(float a, float b, float factor)
+      : na(f2(-a, -a)), nb(f2(-b, -b)), k(f2(factor, factor)) {}
+  __device__ __forceinline__ F2 operator()(F2 f) const {
+    return f2_mul(f2_ex2(f2_fma(f2_add(f, na), f2(LP_LOG2E, LP_LOG2E), nb)), k);
+  }
+  __device__ __forceinline__ float one(float f) const { return f2_get((*this)(f2(f, 0.f))).x; }
+};
+// adds coef to element `at` of a vector
+template <typename L>
+__device__ __forceinline__ void lp_at_label(F2 (&f)[L::VEC / 2], int at, float coef) {
+#pragma unroll
+  for (int k = 0; k < L::VEC / 2; ++k) f[k] = f2_add(f[k], f2(2 * k == at ? coef : 0.f, 2 * k + 1 == at ? coef : 0.f));
+}
+
+// This CTA's share of coef * ([j = label] - p(x_j)) over one row; prob gives -coef * p. d may be x: each thread reads
+// an element before it writes the same one. LAST: nobody reads the row after this, so its lines may leave L2 first.
+template <typename E, bool LAST>
+__device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label, float coef, LpShare sh,
+                                              const LpProb& prob) {
   using L = LpType<E>;
   const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
   const int head = vec ? lp_head(x, V) : V, nvec = (V - head) / L::VEC;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   uint4* dv = reinterpret_cast<uint4*>(d + head);
-  const float2 nc = make_float2(-coef, -coef);
   auto one = [&](const uint4& u, int at) {
-    float f[L::VEC];
+    F2 f[L::VEC / 2];
     L::unpack(u, f);
 #pragma unroll
-    for (int k = 0; k < L::VEC; k += 2) {
-      const float2 g = fmul2(prob(make_float2(f[k], f[k + 1])), nc);
-      f[k] = g.x, f[k + 1] = g.y;
-    }
-    if (at >= 0 && at < L::VEC) {
-#pragma unroll
-      for (int k = 0; k < L::VEC; ++k) f[k] += k == at ? coef : 0.f;
-    }
+    for (int k = 0; k < L::VEC / 2; ++k) f[k] = prob(f[k]);
+    if (at >= 0 && at < L::VEC) lp_at_label<L>(f, at, coef);
     return L::pack(f);
   };
   int v = sh.lo(nvec) + threadIdx.x;
@@ -312,17 +364,17 @@ __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label
   for (; v + (LP_UNROLL - 1) * LP_THREADS < vend; v += LP_UNROLL * LP_THREADS) {
     uint4 u[LP_UNROLL];
 #pragma unroll
-    for (int k = 0; k < LP_UNROLL; ++k) u[k] = xv[v + k * LP_THREADS];
+    for (int k = 0; k < LP_UNROLL; ++k) u[k] = LAST ? __ldcs(&xv[v + k * LP_THREADS]) : xv[v + k * LP_THREADS];
 #pragma unroll
     for (int k = 0; k < LP_UNROLL; ++k)
-      dv[v + k * LP_THREADS] = one(u[k], label - head - (v + k * LP_THREADS) * L::VEC);
+      __stcs(&dv[v + k * LP_THREADS], one(u[k], label - head - (v + k * LP_THREADS) * L::VEC));  // not kept in L2
   }
   for (; v < vend; v += LP_THREADS) dv[v] = one(xv[v], label - head - v * L::VEC);
   const int rest = V - nvec * L::VEC;
   for (int i = sh.lo(rest) + threadIdx.x; i < sh.hi(rest); i += LP_THREADS) {
     const int j = i < head ? i : i + nvec * L::VEC;
-    const float p = prob(make_float2(L::get(x[j]), 0.f)).x;
-    d[j] = L::put(j == label ? coef - coef * p : -coef * p);
+    const float g = prob.one(L::get(x[j]));
+    d[j] = L::put(j == label ? g + coef : g);
   }
 }
 
@@ -331,25 +383,139 @@ __device__ __forceinline__ void lp_write_zero(E* d, int V, LpShare sh) {
   using L = LpType<E>;
   const int head = lp_head(d, V), nvec = (V - head) / L::VEC;
   uint4* dv = reinterpret_cast<uint4*>(d + head);
-  for (int v = sh.lo(nvec) + threadIdx.x; v < sh.hi(nvec); v += LP_THREADS) dv[v] = make_uint4(0u, 0u, 0u, 0u);
+  for (int v = sh.lo(nvec) + threadIdx.x; v < sh.hi(nvec); v += blockDim.x)
+    __stcs(&dv[v], make_uint4(0u, 0u, 0u, 0u));
   const int rest = V - nvec * L::VEC;
-  for (int i = sh.lo(rest) + threadIdx.x; i < sh.hi(rest); i += LP_THREADS)
+  for (int i = sh.lo(rest) + threadIdx.x; i < sh.hi(rest); i += blockDim.x)
     d[i < head ? i : i + nvec * L::VEC] = L::put(0.f);
 }
 
-// 2^{c (x - a) - b} of two logits, times a factor
-struct LpProb {
-  float2 na, nb, k;
-  __device__ __forceinline__ LpProb(float a, float b, float factor)
-      : na(make_float2(-a, -a)), nb(make_float2(-b, -b)), k(make_float2(factor, factor)) {}
-  __device__ __forceinline__ float2 operator()(float2 f) const {
-    const float2 t = ffma2(fadd2(f, na), make_float2(LP_LOG2E, LP_LOG2E), nb);
-    return fmul2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), k);
+// ---------------------------------------------------------------------------- rows through shared memory
+// This CTA's share of a row's vectors, brought in by bulk copies of VECS each, in order, into `slots` places
+// that are used again once every thread is done with them.
+// Waits are bounded; after one has run out (the device error word says so) the rest is not waited for again.
+template <int VECS>
+struct LpStage {
+  const uint4* src;
+  uint4* place;
+  uint64_t* full;
+  int n, pieces, slots;
+  bool ok;
+  __device__ __forceinline__ LpStage(const uint4* src_, int n_, void* smem, uint64_t* full_, int slots_)
+      : src(src_), place(reinterpret_cast<uint4*>(smem)), full(full_), n(n_),
+        pieces((n_ + VECS - 1) / VECS), slots(slots_), ok(true) {}
+  __device__ __forceinline__ int size(int c) const { return min(VECS, n - c * VECS); }
+  __device__ __forceinline__ void issue(int c) {  // one thread
+    const uint32_t bytes = 16u * (uint32_t)size(c);
+    mbar_arrive_expect_tx(&full[c % slots], bytes);
+    bulk_load_1d(place + (c % slots) * VECS, src + (long long)c * VECS, bytes, &full[c % slots]);
+  }
+  // all threads, first
+  __device__ __forceinline__ void start() {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < min(pieces, slots); ++i) mbar_init(&full[i], 1);
+      fence_barrier_init();
+      for (int i = 0; i < min(pieces, slots); ++i) issue(i);
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ const uint4* wait(int c) {
+    if (ok) ok = mbar_wait(&full[c % slots], (uint32_t)(c / slots) & 1u, nullptr);
+    return place + (c % slots) * VECS;
+  }
+  // all threads, after their reads of piece c
+  __device__ __forceinline__ void next(int c) {
+    if (c + slots >= pieces) return;
+    __syncthreads();
+    if (threadIdx.x == 0) issue(c + slots);
   }
 };
 
+// Adds a piece of n vectors to a thread's sum, U vectors at a time; lanes past the end of the last ones add -inf.
+template <typename L, int VECS, int THREADS, int U>
+__device__ __forceinline__ void lp_add_piece(LpSum& sum, const uint4* v, int n) {
+  static_assert(VECS % (U * THREADS) == 0, "a whole piece takes whole steps");
+  const int t = threadIdx.x;
+  if (n == VECS) {
+#pragma unroll 1
+    for (int i = t; i < VECS; i += U * THREADS) {
+      uint4 u[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) u[k] = v[i + k * THREADS];
+      sum.template add<L, U>(u);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = t; i - (t & 31) < n; i += THREADS) {  // warp-uniform
+      const uint4 u[1] = {i < n ? v[i] : make_uint4(L::LOWEST, L::LOWEST, L::LOWEST, L::LOWEST)};
+      sum.template add<L, 1>(u);
+    }
+  }
+}
+
+// The sum of one row through shared memory, the same in every thread of its CTAs, all of which have read it on return.
+template <typename E, bool CL, int THREADS, int VECS, int SLOTS>
+__device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, LpRow* out) {
+  using L = LpType<E>;
+  const int head = lp_head(x, V), nvec = (V - head) / L::VEC, rest = V - nvec * L::VEC;
+  const int lo = sh.lo(nvec);
+  LpStage<VECS> st(reinterpret_cast<const uint4*>(x + head) + lo, sh.hi(nvec) - lo, smem, full, SLOTS);
+  st.start();
+  LpSum a;
+  for (int j = sh.lo(rest) + threadIdx.x; j < sh.hi(rest); j += THREADS)
+    a.add(L::get(x[j < head ? j : j + nvec * L::VEC]));
+  for (int c = 0; c < st.pieces; ++c) {
+    lp_add_piece<L, VECS, THREADS, 4>(a, st.wait(c), st.size(c));
+    st.next(c);
+  }
+  const float2 q = lp_join<CL>(make_float2(a.m, a.s), sh, lp_merge);
+  *out = lp_plain(q) ? lp_finish(q)
+                     : lp_careful(x, V, sh.part * THREADS + (int)threadIdx.x, sh.parts * THREADS, LpCtaJoin<CL>{sh});
+}
+
 // ---------------------------------------------------------------------------- token log-probabilities
-// One pass over a row with a running maximum and sum.
+// Forward for long rows: one CTA a row (or a share of it), 24 KB of it in flight; nine small CTAs an SM, each in its own
+// phase, keep the copies and the exponentials going at the same time (4092 rows of 50304 bf16 logits, 2492 of them
+// scored: 44 us, 5.7 TB/s, as without the exponentials; four CTAs of 256 threads 51 us; loads into registers 55 us).
+constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512, LP_FWD_SLOTS = 3;
+constexpr uint32_t LP_FWD_SMEM = LP_FWD_SLOTS * LP_FWD_VECS * 16u;
+template <typename E, bool CL>
+__global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E* __restrict__ logits, LpRows lr, int V,
+                                                                        const long long* __restrict__ labels,
+                                                                        long long ignore_index,
+                                                                        float* __restrict__ logps,
+                                                                        float* __restrict__ lse,
+                                                                        double* __restrict__ wide) {
+  using L = LpType<E>;
+  extern __shared__ __align__(128) uint8_t lp_smem[];
+  __shared__ uint64_t full[LP_FWD_SLOTS];
+  griddep_wait();
+  griddep_launch();
+  const LpShare sh = lp_share<CL>();
+  const long long row = blockIdx.x / sh.parts;
+  const long long label = labels[row];
+  const bool first = threadIdx.x == 0 && sh.part == 0;
+  if (!lp_scored(label, ignore_index, V)) {
+    if (first) {
+      logps[row] = 0.f;
+      if (lse) lse[row] = 0.f;
+      if (wide) wide[row] = 0.0;
+    }
+    return;
+  }
+  const E* x = logits + lr.offset(row);
+  const float xl = first ? L::get(x[label]) : 0.f;
+  LpRow r;
+  lp_staged_sum<E, CL, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r);
+  if (first) {
+    const double lp = (double)xl - r.lse;
+    logps[row] = (float)lp;
+    if (lse) lse[row] = (float)r.lse;
+    if (wide) wide[row] = lp;
+  }
+}
+
+// Forward for short rows: one pass over a row with a running maximum and sum.
 template <typename E, bool CL>
 __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restrict__ logits, LpRows lr, int V,
                                                               const long long* __restrict__ labels,
@@ -390,7 +556,8 @@ __global__ void __launch_bounds__(LP_THREADS) logp_bwd_kernel(const E* logits, L
   griddep_wait();
   griddep_launch();
   const LpShare sh = lp_share<CL>();
-  const long long row = blockIdx.x / sh.parts;
+  // the last rows first: the forward has left them in L2 (4092 rows of 100 KB: forward and backward 176 -> 166 us)
+  const long long row = (gridDim.x - 1 - blockIdx.x) / sh.parts;
   const long long label = labels[row];
   E* d = dlogits + dr.offset(row);
   if (!lp_scored(label, ignore_index, V)) {
@@ -398,22 +565,23 @@ __global__ void __launch_bounds__(LP_THREADS) logp_bwd_kernel(const E* logits, L
     return;
   }
   const E* x = logits + lr.offset(row);
-  const float l = lse[row], c = coef[per_seq ? row / lr.T : row];
+  const float l = lse[row], c = coef[per_seq ? lr.batch(row) : row];
   LpRow r = {l, 0.f, 1.f, 0.0};
   if (!(fabsf(l) <= LP_LSE_EXACT)) {
     r = lp_careful(x, V, sh.part * LP_THREADS + (int)threadIdx.x, sh.parts * LP_THREADS, LpCtaJoin<CL>{sh});
     __syncthreads();  // every thread has read the row before an in-place gradient
   }
-  lp_write_grad(x, d, V, (int)label, c, sh, LpProb(r.a, r.b, r.inv));
+  lp_write_grad<E, false>(x, d, V, (int)label, c, sh, LpProb(r.a, r.b, -c * r.inv));
 }
 
 // ---------------------------------------------------------------------------- sums over a CTA
-__device__ __forceinline__ double lp_block_sum(double v, double* red) {
+template <typename S>
+__device__ __forceinline__ S lp_block_sum(S v, S* red) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();  // red may still be read from an earlier sum
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  double t = 0.0;
+  S t = 0;
   for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += red[w];
   return t;
 }
@@ -501,29 +669,35 @@ __global__ void __launch_bounds__(256) pref_loss_kernel(const float* __restrict_
 // ---------------------------------------------------------------------------- policy loss
 struct PolicyArgs {
   float low, high, kl, grad_scale;
+  double log_low, log_high;  // log(1 - low), log(1 + high)
   int adv_per_token, by_sequence;
 };
 
 // Terms of one token from its log-probability lp: r = e^{lp - old}; -min(r A, clip(r) A); e^q - q - 1, q = ref - lp.
+// The differences are taken, and compared with the clip's borders, in fp64; the exponentials of them in fp32.
 struct PolicyTerms {
-  double pg, kl, cut, d;  // d = d (pg + kl_coef * kl) / d lp
+  float pg, kl, cut, d;  // d = d (pg + kl_coef * kl) / d lp
 };
-__device__ __forceinline__ PolicyTerms policy_terms(const PolicyArgs& a, double lp, double old, bool has_ref, double ref,
-                                                    double adv) {
+__device__ __forceinline__ PolicyTerms policy_terms(const PolicyArgs& a, double lp, float old, bool has_ref, float ref,
+                                                    float adv) {
   PolicyTerms t;
-  const double r = exp(lp - old);
-  const double hi = 1.0 + (double)a.high, lo = 1.0 - (double)a.low;
-  const bool cut = (adv > 0.0 && r > hi) || (adv < 0.0 && r < lo);
-  t.pg = cut ? -(adv > 0.0 ? hi : lo) * adv : -r * adv;
-  t.d = cut ? 0.0 : -r * adv;
-  t.cut = cut ? 1.0 : 0.0;
-  t.kl = 0.0;
+  const double lr = lp - (double)old;
+  const bool cut = (adv > 0.f && lr > a.log_high) || (adv < 0.f && lr < a.log_low);
+  const float r = expf((float)lr);
+  t.pg = -(cut ? (adv > 0.f ? 1.f + a.high : 1.f - a.low) : r) * adv;
+  t.d = cut ? 0.f : -r * adv;
+  t.cut = cut ? 1.f : 0.f;
+  t.kl = 0.f;
   if (has_ref) {
-    const double q = ref - lp, e = exp(q);
-    t.kl = e - q - 1.0;
-    t.d += (double)a.kl * (1.0 - e);
+    const float q = (float)((double)ref - lp), e = expm1f(q);
+    t.kl = e - q;
+    t.d -= a.kl * e;
   }
   return t;
+}
+// A token's weight in the loss; n: scored tokens of its sequence, total: of the batch, or its nonempty sequences.
+__device__ __forceinline__ float policy_weight(const PolicyArgs& a, int n, int total) {
+  return a.by_sequence ? 1.f / ((float)n * (float)total) : 1.f / (float)total;
 }
 
 // scored tokens of each sequence
@@ -531,67 +705,114 @@ __global__ void __launch_bounds__(256) policy_count_kernel(const long long* __re
                                                            int V, int T, int* __restrict__ counts) {
   griddep_wait();
   griddep_launch();
-  __shared__ double red[8];
+  __shared__ int red[8];
   const long long base = (long long)blockIdx.x * T;
-  double c = 0.0;
-  for (int t = threadIdx.x; t < T; t += blockDim.x) c += lp_scored(labels[base + t], ignore_index, V) ? 1.0 : 0.0;
+  int c = 0;
+  for (int t = threadIdx.x; t < T; t += blockDim.x) c += lp_scored(labels[base + t], ignore_index, V) ? 1 : 0;
   c = lp_block_sum(c, red);
-  if (threadIdx.x == 0) counts[blockIdx.x] = (int)c;
+  if (threadIdx.x == 0) counts[blockIdx.x] = c;
 }
 
 // Sum of counts (token mean) or number of nonempty sequences (sequence mean), over the whole CTA.
-__device__ __forceinline__ double policy_total(const int* __restrict__ counts, int B, int by_sequence, double* red) {
-  double c = 0.0;
-  for (int b = threadIdx.x; b < B; b += blockDim.x) c += by_sequence ? (counts[b] > 0 ? 1.0 : 0.0) : (double)counts[b];
+__device__ __forceinline__ int policy_total(const int* __restrict__ counts, int B, int by_sequence, int* red) {
+  int c = 0;
+  for (int b = threadIdx.x; b < B; b += blockDim.x) c += by_sequence ? (counts[b] > 0 ? 1 : 0) : counts[b];
   return lp_block_sum(c, red);
 }
 
+// The inputs and outputs of one row of the policy loss.
+struct PolicyRows {
+  const long long* labels;
+  long long ignore_index;
+  const float *old, *ref, *adv;
+  const int* counts;
+  int B;
+  PolicyArgs a;
+  float *logps, *lse, *coef;
+};
+
+// What thread 0 does with a row's sum: the token's terms, the outputs, and the row's coefficient for the CTA.
+__device__ __forceinline__ float policy_row(const PolicyRows& p, LpRows lr, long long row, float xl, const LpRow& r,
+                                            int total, bool first) {
+  const double lp = (double)xl - r.lse;
+  const unsigned b = lr.batch(row);
+  const PolicyTerms t = policy_terms(p.a, lp, p.old[row], p.ref != nullptr, p.ref ? p.ref[row] : 0.f,
+                                     p.adv[p.a.adv_per_token ? row : b]);
+  const float coef = t.d * policy_weight(p.a, p.counts[b], total) * p.a.grad_scale;
+  if (first) {
+    p.logps[row] = (float)lp;
+    if (p.lse) p.lse[row] = (float)r.lse;
+    if (p.coef) p.coef[row] = coef;
+  }
+  return coef;
+}
+__device__ __forceinline__ void policy_row_unscored(const PolicyRows& p, long long row) {
+  p.logps[row] = 0.f;
+  if (p.lse) p.lse[row] = 0.f;
+  if (p.coef) p.coef[row] = 0.f;
+}
+
+// One CTA a row (or a share of it): the sum, the coefficient, then the gradient from a second read, which finds the
+// row in L2 as long as few rows are on their way: three CTAs an SM (16368 rows of 50304 bf16 logits: 481 us, 5.5 TB/s;
+// nine smaller CTAs 570 us, their rows fill L2; without the hint that the second read is the last 542 us). Holding the
+// row in shared memory instead allows two rows an SM, too few to cover their phases' latencies: 557 us at best.
 template <typename E, bool CL>
-__global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpRows lr, int B, int V,
-                                                            const long long* __restrict__ labels,
-                                                            long long ignore_index, const float* __restrict__ old,
-                                                            const float* __restrict__ ref, const float* __restrict__ adv,
-                                                            PolicyArgs a, const int* __restrict__ counts,
-                                                            float* __restrict__ logps, float* __restrict__ lse,
-                                                            float* __restrict__ coef, E* dlogits, LpRows dr) {
+__global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpRows lr, int V, const PolicyRows p,
+                                                            E* dlogits, LpRows dr) {
   griddep_wait();
   griddep_launch();
-  __shared__ double red[LP_THREADS / 32];
+  __shared__ int red[LP_THREADS / 32];
   __shared__ float s_coef;
   const LpShare sh = lp_share<CL>();
   const long long row = blockIdx.x / sh.parts;
-  const long long label = labels[row];
-  const bool first = threadIdx.x == 0 && sh.part == 0;
+  const long long label = p.labels[row];
   E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
-  if (!lp_scored(label, ignore_index, V)) {
-    if (first) {
-      logps[row] = 0.f;
-      if (lse) lse[row] = 0.f;
-      if (coef) coef[row] = 0.f;
-    }
+  if (!lp_scored(label, p.ignore_index, V)) {
+    if (threadIdx.x == 0 && sh.part == 0) policy_row_unscored(p, row);
     if (d) lp_write_zero(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float xl = LpType<E>::get(x[label]);  // before an in-place gradient
-  const double total = policy_total(counts, B, a.by_sequence, red);
+  const int total = policy_total(p.counts, p.B, p.a.by_sequence, red);
   const LpRow r = lp_row_sum<E, CL>(x, V, sh);
-  if (threadIdx.x == 0) {
-    const double lp = (double)xl - r.lse;
-    const long long b = row / lr.T;
-    const PolicyTerms t = policy_terms(a, lp, (double)old[row], ref != nullptr, ref ? (double)ref[row] : 0.0,
-                                       (double)adv[a.adv_per_token ? row : b]);
-    const double w = a.by_sequence ? 1.0 / ((double)counts[b] * total) : 1.0 / total;
-    s_coef = (float)(t.d * w * (double)a.grad_scale);
-    if (first) {
-      logps[row] = (float)lp;
-      if (lse) lse[row] = (float)r.lse;
-      if (coef) coef[row] = s_coef;
-    }
-  }
+  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, total, sh.part == 0);
   if (!d) return;
   __syncthreads();
-  lp_write_grad(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, r.inv));
+  lp_write_grad<E, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
+}
+
+// The same for long rows, the first read by bulk copies.
+constexpr int POL_VECS = 1024, POL_SLOTS = 3;
+constexpr uint32_t POL_SMEM = POL_SLOTS * POL_VECS * 16u;
+template <typename E, bool CL>
+__global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logits, LpRows lr, int V,
+                                                                    const PolicyRows p, E* dlogits, LpRows dr) {
+  using L = LpType<E>;
+  extern __shared__ __align__(128) uint8_t lp_smem[];
+  __shared__ uint64_t full[POL_SLOTS];
+  __shared__ int red[LP_THREADS / 32];
+  __shared__ float s_coef;
+  griddep_wait();
+  griddep_launch();
+  const LpShare sh = lp_share<CL>();
+  const long long row = blockIdx.x / sh.parts;
+  const long long label = p.labels[row];
+  E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
+  if (!lp_scored(label, p.ignore_index, V)) {
+    if (threadIdx.x == 0 && sh.part == 0) policy_row_unscored(p, row);
+    if (d) lp_write_zero(d, V, sh);
+    return;
+  }
+  const E* x = logits + lr.offset(row);
+  const float xl = L::get(x[label]);
+  LpRow r;
+  lp_staged_sum<E, CL, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, &r);
+  const int total = policy_total(p.counts, p.B, p.a.by_sequence, red);
+  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, total, sh.part == 0);
+  if (!d) return;
+  __syncthreads();
+  lp_write_grad<E, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
 }
 
 // stats = {loss, policy term, KL, clipped share}: weighted sums over the tokens, from their log-probabilities
@@ -604,17 +825,18 @@ __global__ void __launch_bounds__(1024) policy_stats_kernel(const float* __restr
   griddep_wait();
   griddep_launch();
   __shared__ double red[32];
-  const double total = policy_total(counts, B, a.by_sequence, red);
+  __shared__ int ired[32];
+  const int total = policy_total(counts, B, a.by_sequence, ired);
   double pg = 0.0, kl = 0.0, cut = 0.0;
   for (long long i = threadIdx.x; i < (long long)B * T; i += blockDim.x) {
     if (!lp_scored(labels[i], ignore_index, V)) continue;
-    const long long b = i / T;
-    const PolicyTerms t = policy_terms(a, (double)logps[i], (double)old[i], ref != nullptr, ref ? (double)ref[i] : 0.0,
-                                       (double)adv[a.adv_per_token ? i : b]);
-    const double w = a.by_sequence ? 1.0 / ((double)counts[b] * total) : 1.0 / total;
-    pg += w * t.pg;
-    kl += w * t.kl;
-    cut += w * t.cut;
+    const unsigned b = (unsigned)i / (unsigned)T;
+    const PolicyTerms t = policy_terms(a, (double)logps[i], old[i], ref != nullptr, ref ? ref[i] : 0.f,
+                                       adv[a.adv_per_token ? i : b]);
+    const double w = (double)policy_weight(a, counts[b], total);
+    pg += w * (double)t.pg;
+    kl += w * (double)t.kl;
+    cut += w * (double)t.cut;
   }
   pg = lp_block_sum(pg, red);
   kl = lp_block_sum(kl, red);
@@ -668,17 +890,44 @@ static int lp_parts(long long M, int V, int dtype) {
   return c;
 }
 
-static void launch_logp_fwd(const void* logits, int dtype, LpRows lr, long long M, int V, const long long* labels,
+// Rows worth a trip through shared memory: below 16 KB their fixed cost (barriers, the copy's latency) shows.
+static bool lp_long(int V, int dtype) { return (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2) >= 16384; }
+
+// Allows `kern` its dynamic shared memory on the current device (once).
+template <typename K>
+static int lp_smem(K kern, uint32_t bytes, bool* set) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return rgpt_set_error(RGPT_ERR_INTERNAL, "device index %d", dev);
+  if (!set[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+      return rgpt_check_launch("row kernel shared memory");
+    set[dev] = true;
+  }
+  return RGPT_OK;
+}
+
+static int launch_logp_fwd(const void* logits, int dtype, LpRows lr, long long M, int V, const long long* labels,
                             long long ignore_index, float* logps, float* lse, double* wide, cudaStream_t s) {
+  int rc = RGPT_OK;
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
     const int c = lp_parts(M, V, dtype);
+    if (lp_long(V, dtype)) {
+      auto kern = c > 1 ? logp_fwd_staged_kernel<E, true> : logp_fwd_staged_kernel<E, false>;
+      static bool set[2][64] = {};
+      if ((rc = lp_smem(kern, LP_FWD_SMEM, set[c > 1])) == RGPT_OK)
+        launch_pdl(kern, dim3((unsigned)(M * c)), dim3(LP_FWD_THREADS), LP_FWD_SMEM, s, c, (const E*)logits, lr, V, labels,
+                   ignore_index, logps, lse, wide);
+      return;
+    }
     launch_pdl(c > 1 ? logp_fwd_kernel<E, true> : logp_fwd_kernel<E, false>, dim3((unsigned)(M * c)), dim3(LP_THREADS), 0,
                s, c, (const E*)logits, lr, V, labels, ignore_index, logps, lse, wide);
   });
+  return rc;
 }
 
-static void launch_logp_bwd(const void* logits, int dtype, LpRows lr, long long M, int V, const long long* labels,
+static int launch_logp_bwd(const void* logits, int dtype, LpRows lr, long long M, int V, const long long* labels,
                             long long ignore_index, const float* lse, const float* coef, int per_seq, void* dlogits,
                             LpRows dr, cudaStream_t s) {
   lp_dispatch(dtype, [&](auto* tag) {
@@ -687,29 +936,30 @@ static void launch_logp_bwd(const void* logits, int dtype, LpRows lr, long long 
     launch_pdl(c > 1 ? logp_bwd_kernel<E, true> : logp_bwd_kernel<E, false>, dim3((unsigned)(M * c)), dim3(LP_THREADS), 0,
                s, c, (const E*)logits, lr, V, labels, ignore_index, lse, coef, per_seq, (E*)dlogits, dr);
   });
+  return RGPT_OK;
 }
 
 extern "C" int rgpt_token_logprobs(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,
                                    const long long* labels, long long ignore_index, float* logps, float* lse,
                                    void* stream) {
-  const int rc = lp_check("token_logprobs", logits, dtype, B, T, V, labels);
+  int rc = lp_check("token_logprobs", logits, dtype, B, T, V, labels);
   if (rc) return rc;
   if (logps == nullptr) return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "token_logprobs: null output");
-  launch_logp_fwd(logits, dtype, LpRows{sb, st, T}, (long long)B * T, V, labels, ignore_index, logps, lse,
-                  nullptr, reinterpret_cast<cudaStream_t>(stream));
-  return rgpt_check_launch("logp_fwd_kernel");
+  rc = launch_logp_fwd(logits, dtype, LpRows{sb, st, T}, (long long)B * T, V, labels, ignore_index, logps, lse, nullptr,
+                       reinterpret_cast<cudaStream_t>(stream));
+  return rc ? rc : rgpt_check_launch("token_logprobs kernel");
 }
 
 extern "C" int rgpt_token_logprobs_bwd(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,
                                        const long long* labels, long long ignore_index, const float* lse,
                                        const float* dlogps, void* dlogits, long long db, long long dt, void* stream) {
-  const int rc = lp_check("token_logprobs_bwd", logits, dtype, B, T, V, labels);
+  int rc = lp_check("token_logprobs_bwd", logits, dtype, B, T, V, labels);
   if (rc) return rc;
   if (lse == nullptr || dlogps == nullptr || dlogits == nullptr)
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "token_logprobs_bwd: null pointer");
-  launch_logp_bwd(logits, dtype, LpRows{sb, st, T}, (long long)B * T, V, labels, ignore_index, lse, dlogps, 0, dlogits,
-                  LpRows{db, dt, T}, reinterpret_cast<cudaStream_t>(stream));
-  return rgpt_check_launch("logp_bwd_kernel");
+  rc = launch_logp_bwd(logits, dtype, LpRows{sb, st, T}, (long long)B * T, V, labels, ignore_index, lse, dlogps, 0, dlogits,
+                       LpRows{db, dt, T}, reinterpret_cast<cudaStream_t>(stream));
+  return rc ? rc : rgpt_check_launch("token_logprobs_bwd kernel");
 }
 
 extern "C" int rgpt_preference_loss(const void* logits, int dtype, long long sb, long long st, int P, int T, int V,
@@ -718,7 +968,7 @@ extern "C" int rgpt_preference_loss(const void* logits, int dtype, long long sb,
                                     float* token_logps, float* lse, float* seq_logps, float* margins, float* coef,
                                     float* loss, double* scratch, void* dlogits, long long db, long long dt,
                                     void* stream) {
-  const int rc = lp_check("preference_loss", logits, dtype, 2ll * P, T, V, labels);
+  int rc = lp_check("preference_loss", logits, dtype, 2ll * P, T, V, labels);
   if (rc) return rc;
   if (!token_logps || !lse || !seq_logps || !margins || !coef || !loss || !scratch)
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "preference_loss: null output");
@@ -728,12 +978,13 @@ extern "C" int rgpt_preference_loss(const void* logits, int dtype, long long sb,
   const LpRows lr = {sb, st, T};
   const long long M = 2ll * P * T;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  launch_logp_fwd(logits, dtype, lr, M, V, labels, ignore_index, token_logps, lse, scratch, s);
+  if ((rc = launch_logp_fwd(logits, dtype, lr, M, V, labels, ignore_index, token_logps, lse, scratch, s))) return rc;
   launch_pdl(pref_pair_kernel, dim3(P), dim3(256), 0, s, 1, (const double*)scratch, labels, ignore_index, V, P, T, ref_logps, a,
              seq_logps, margins, coef);
   launch_pdl(pref_loss_kernel, dim3(1), dim3(256), 0, s, 1, margins, P, a, loss);
-  if (dlogits)
-    launch_logp_bwd(logits, dtype, lr, M, V, labels, ignore_index, lse, coef, 1, dlogits, LpRows{db, dt, T}, s);
+  if (dlogits &&
+      (rc = launch_logp_bwd(logits, dtype, lr, M, V, labels, ignore_index, lse, coef, 1, dlogits, LpRows{db, dt, T}, s)))
+    return rc;
   return rgpt_check_launch("preference_loss kernels");
 }
 
@@ -743,20 +994,31 @@ extern "C" int rgpt_policy_loss(const void* logits, int dtype, long long sb, lon
                                 float clip_high, float kl_coef, int by_sequence, float grad_scale, float* token_logps,
                                 int* counts, float* stats, float* lse, float* coef, void* dlogits, long long db,
                                 long long dt, void* stream) {
-  const int rc = lp_check("policy_loss", logits, dtype, B, T, V, labels);
+  int rc = lp_check("policy_loss", logits, dtype, B, T, V, labels);
   if (rc) return rc;
   if (!old_logps || !advantages || !token_logps || !counts || !stats)
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "policy_loss: null pointer");
-  const PolicyArgs a = {clip_low, clip_high, kl_coef, grad_scale, adv_per_token, by_sequence};
+  const PolicyArgs a = {clip_low, clip_high, kl_coef, grad_scale, log1p(-(double)clip_low), log1p((double)clip_high),
+                        adv_per_token, by_sequence};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   launch_pdl(policy_count_kernel, dim3(B), dim3(256), 0, s, 1, labels, ignore_index, V, T, counts);
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
-    const int c = lp_parts((long long)B * T, V, dtype);
-    launch_pdl(c > 1 ? policy_kernel<E, true> : policy_kernel<E, false>, dim3((unsigned)((long long)B * T * c)),
-               dim3(LP_THREADS), 0, s, c, (const E*)logits, LpRows{sb, st, T}, B, V, labels, ignore_index, old_logps,
-               ref_logps, advantages, a, (const int*)counts, token_logps, lse, coef, (E*)dlogits, LpRows{db, dt, T});
+    const LpRows lr = {sb, st, T}, dr = {db, dt, T};
+    const PolicyRows p = {labels, ignore_index, old_logps, ref_logps, advantages, counts, B, a, token_logps, lse, coef};
+    const unsigned M = (unsigned)((long long)B * T);
+    const int c = lp_parts(M, V, dtype);
+    if (lp_long(V, dtype)) {
+      auto kern = c > 1 ? policy_staged_kernel<E, true> : policy_staged_kernel<E, false>;
+      static bool set[2][64] = {};
+      if ((rc = lp_smem(kern, POL_SMEM, set[c > 1])) == RGPT_OK)
+        launch_pdl(kern, dim3(M * c), dim3(LP_THREADS), POL_SMEM, s, c, (const E*)logits, lr, V, p, (E*)dlogits, dr);
+      return;
+    }
+    launch_pdl(c > 1 ? policy_kernel<E, true> : policy_kernel<E, false>, dim3(M * c), dim3(LP_THREADS), 0, s, c,
+               (const E*)logits, lr, V, p, (E*)dlogits, dr);
   });
+  if (rc) return rc;
   launch_pdl(policy_stats_kernel, dim3(1), dim3(1024), 0, s, 1, (const float*)token_logps, labels, ignore_index, V, B, T,
              old_logps, ref_logps, advantages, a, (const int*)counts, stats);
   return rgpt_check_launch("policy_loss kernels");

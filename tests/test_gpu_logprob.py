@@ -94,6 +94,10 @@ CASES = [
     (1, 300, 515, torch.bfloat16, "time first"), (5, 40, 96, torch.float32, "time first"), (1, 2, 131071, torch.float32, "plain"),
     (1, 3, 262144, torch.bfloat16, "plain"), (40, 1, 33000, torch.bfloat16, "plain"), (700, 1, 120, torch.bfloat16, "plain"),
     (1, 5000, 65, torch.float16, "plain"),
+    # many long rows
+    (300, 1, 50304, torch.bfloat16, "plain"), (2, 160, 50257, torch.float16, "plain"), (3, 101, 50257, torch.float32, "plain"),
+    (2, 150, 8192, torch.bfloat16, "shifted"), (2, 170, 8201, torch.float16, "shifted"), (1, 700, 4100, torch.float32, "padded"),
+    (5, 70, 32768, torch.bfloat16, "time first"), (1, 300, 131071, torch.float32, "plain"), (4, 300, 16391, torch.bfloat16, "padded"),
 ]
 
 
@@ -130,8 +134,8 @@ def test_two_dimensional_logits_are_rows(cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("V", [130, 50304])
-def test_rows_of_extreme_values(cuda, dtype, V):
+@pytest.mark.parametrize("V,times", [(130, 1), (50304, 1), (50304, 40), (8200, 100)])
+def test_rows_of_extreme_values(cuda, dtype, V, times):
     low, inf = torch.finfo(dtype).min, float("inf")
     x = torch.randn(9, V, device=cuda).to(dtype)
     x[0] = low                      # every logit the lowest value: uniform
@@ -145,10 +149,26 @@ def test_rows_of_extreme_values(cuda, dtype, V):
     x[8, 3] = -inf                  # the label itself is masked out
     labels = torch.full((9,), V - 1, device=cuda)
     labels[7], labels[8] = IGNORE, 3
-    lp, lse = torch.empty(9, device=cuda), torch.empty(9, device=cuda)
+    x, labels = x.repeat(times, 1), labels.repeat(times)
+    lp, lse = torch.empty(9 * times, device=cuda), torch.empty(9 * times, device=cuda)
     nv.token_logprobs(x, labels, lp, lse=lse)
     d = torch.empty_like(x)
-    nv.token_logprobs_bwd(x, labels, lse, torch.ones(9, device=cuda), d)
+    nv.token_logprobs_bwd(x, labels, lse, torch.ones(9 * times, device=cuda), d)
+    # the same through the policy loss, on-policy with advantage -1: the gradient is softmax - onehot over all scored
+    # tokens, and the same rows give the same bits wherever they stand
+    st, lp2, d2 = torch.empty(4, device=cuda), torch.empty_like(lp), torch.empty_like(x)
+    old = torch.where(torch.isfinite(lp), lp, 0.0)
+    n = 9 * times
+    nv.policy_loss(x, labels, old, torch.full((n,), -float(8 * times), device=cuda), token_logps=lp2, stats=st,
+                   counts=torch.empty(n, device=cuda, dtype=torch.int32), dlogits=d2)
+    for t in (lp, lp2, d, d2):
+        assert torch.equal(t.view(times, -1).nan_to_num(7.5), t.view(times, -1)[:1].nan_to_num(7.5).expand(times, -1))
+    x, labels, lp, lse, d, lp2, d2 = x[:9], labels[:9], lp[:9], lse[:9], d[:9], lp2[:9], d2[:9]
+    assert torch.equal(torch.isnan(lp), torch.isnan(lp2)) and lp2[8] == -inf and lp2[7] == 0 and (d2[7] == 0).all()
+    assert ((lp2 - lp)[[0, 1, 2, 6]].abs() <= 2 * rel(V) + 2 * U * lp[[0, 1, 2, 6]].abs()).all()
+    # a ratio of e^0 to e^{2 rel}, and the label at -inf has ratio 0
+    check_grad(d2[[1, 2]][None], x[[1, 2]][None], labels[[1, 2]][None], torch.full((1, 2), 1.0, device=cuda), 3 * rel(V) + 16 * U)
+    assert (d2[8] == 0).all()
     want, _ = ref_logps(x.double()[None], labels[None])
     want = want[0]
     ok = [0, 1, 2, 6]
@@ -186,6 +206,9 @@ PREF = [
     dict(P=300, T=2, V=64, dtype=torch.bfloat16, kind="sigmoid"),
     dict(P=2, T=700, V=301, dtype=torch.bfloat16, kind="squared", average=True, layout="padded"),
     dict(P=2, T=9, V=500, dtype=torch.float32, kind="sigmoid", empty=True),
+    dict(P=2, T=90, V=50304, dtype=torch.bfloat16, kind="sigmoid", smoothing=0.1, layout="shifted"),
+    dict(P=3, T=60, V=8203, dtype=torch.float16, kind="hinge", average=True, beta=1.0),
+    dict(P=160, T=1, V=20001, dtype=torch.float32, kind="squared", layout="padded"),
     dict(P=2, T=9, V=500, dtype=torch.float32, kind="hinge", average=True, empty=True),
 ]
 
@@ -263,6 +286,11 @@ POLICY = [
     dict(B=700, T=3, V=65, dtype=torch.bfloat16, kl=0.01, by_sequence=True),
     dict(B=2, T=900, V=200, dtype=torch.float32, per_token=True, layout="time first"),
     dict(B=3, T=8, V=120, dtype=torch.float32, kl=0.2, by_sequence=True, empty=True),
+    dict(B=4, T=90, V=50304, dtype=torch.bfloat16, kl=0.1, by_sequence=True, layout="shifted"),
+    dict(B=3, T=100, V=50257, dtype=torch.float32, kl=0.04, per_token=True),
+    dict(B=2, T=160, V=8203, dtype=torch.float16, by_sequence=True, kl=0.1, empty=True),
+    dict(B=400, T=1, V=33000, dtype=torch.float16, layout="padded"),
+    dict(B=1, T=310, V=70001, dtype=torch.float32, per_token=True),
 ]
 
 
@@ -312,7 +340,10 @@ def test_policy_loss(cuda, c, inplace):
     err = w * (tol + 4 * U) * (grow + kl_coef * (torch.exp(q) + 1))
     assert ((b["coef"].double() - 2 * coef).abs() <= 2 * err + 2 * U * coef.abs()).all()
     check_grad(d, before, labels, b["coef"], 4 * U)  # the rows, given the coefficients checked above
-    assert all(torch.equal(b[k], b2[k]) for k in b2)
+    # without a gradient another kernel may serve, whose sums run in another order
+    assert torch.equal(b["counts"], b2["counts"])
+    assert ((b["token_logps"] - b2["token_logps"]).abs() <= 2 * tol).all()
+    assert ((b["stats"] - b2["stats"]).abs()[:3] <= 2 * each.sum() + 4 * U * stats[:3].abs()).all()
 
 
 def test_nothing_scored_gives_zeros(cuda):
