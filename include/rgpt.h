@@ -334,8 +334,8 @@ int rgpt_adamw(const RgptAdamwTensor* table, const int* chunk_tensor, const long
  *       2^(q/32 - 7) * (1 + (q%32)/32); r = sqrt(v), r_scale = max r / 1.96875. A nonzero r never takes code 0.
  * Codes round to nearest, ties to even; a block whose largest moment is not above 2^-100 holds zeros. The update:
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr ((m / (sqrt(v) inv_sqrt_bc2 + eps)) inv_bc1)
- * from the moments before they are rounded to codes, every operation one fp32 rounding. chunk_elems: a multiple of
- * 256, and every chunk_start too. */
+ * from the moments before they are rounded to codes. The moments take one fp32 rounding an operation; the division is
+ * accurate to 2 ulp. chunk_elems: a multiple of 256, and every chunk_start too. */
 #define RGPT_ADAMW8_BLOCK 256
 typedef struct RgptAdamw8Tensor {
   float* p; const float* g; unsigned char* mq; float* m_scale; unsigned char* vq; float* r_scale;

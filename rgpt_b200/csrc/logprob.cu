@@ -454,13 +454,15 @@ __device__ __forceinline__ void lp_add_piece(LpSum& sum, const uint4* v, int n) 
 }
 
 // The sum of one row through shared memory, the same in every thread of its CTAs, all of which have read it on return.
-template <typename E, bool CL, int THREADS, int VECS, int SLOTS>
-__device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, LpRow* out) {
+template <typename E, bool CL, int THREADS, int VECS, int SLOTS, typename F>
+__device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, LpRow* out,
+                                              F&& meanwhile) {
   using L = LpType<E>;
   const int head = lp_head(x, V), nvec = (V - head) / L::VEC, rest = V - nvec * L::VEC;
   const int lo = sh.lo(nvec);
   LpStage<VECS> st(reinterpret_cast<const uint4*>(x + head) + lo, sh.hi(nvec) - lo, smem, full, SLOTS);
   st.start();
+  meanwhile();
   LpSum a;
   for (int j = sh.lo(rest) + threadIdx.x; j < sh.hi(rest); j += THREADS)
     a.add(L::get(x[j < head ? j : j + nvec * L::VEC]));
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
   const E* x = logits + lr.offset(row);
   const float xl = first ? L::get(x[label]) : 0.f;
   LpRow r;
-  lp_staged_sum<E, CL, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r);
+  lp_staged_sum<E, CL, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r, [] {});
   if (first) {
     const double lp = (double)xl - r.lse;
     logps[row] = (float)lp;
@@ -584,6 +586,20 @@ __device__ __forceinline__ S lp_block_sum(S v, S* red) {
   S t = 0;
   for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += red[w];
   return t;
+}
+
+// three sums at once, in thread 0
+__device__ __forceinline__ double3 lp_block_sum3(double3 v, double3* red) {
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v.x += red[w].x, v.y += red[w].y, v.z += red[w].z;
+  return v;
 }
 
 // ---------------------------------------------------------------------------- preference loss
@@ -725,26 +741,56 @@ struct PolicyRows {
   const long long* labels;
   long long ignore_index;
   const float *old, *ref, *adv;
-  const int* counts;
-  int B;
+  int* counts;
+  int B, count_here;  // few tokens: each CTA counts for itself, and a sequence's first CTA writes counts
   PolicyArgs a;
   float *logps, *lse, *coef;
 };
 
 // What thread 0 does with a row's sum: the token's terms, the outputs, and the row's coefficient for the CTA.
 __device__ __forceinline__ float policy_row(const PolicyRows& p, LpRows lr, long long row, float xl, const LpRow& r,
-                                            int total, bool first) {
+                                            int n, int total, bool first) {
   const double lp = (double)xl - r.lse;
   const unsigned b = lr.batch(row);
   const PolicyTerms t = policy_terms(p.a, lp, p.old[row], p.ref != nullptr, p.ref ? p.ref[row] : 0.f,
                                      p.adv[p.a.adv_per_token ? row : b]);
-  const float coef = t.d * policy_weight(p.a, p.counts[b], total) * p.a.grad_scale;
+  const float coef = t.d * policy_weight(p.a, n, total) * p.a.grad_scale;
   if (first) {
     p.logps[row] = (float)lp;
     if (p.lse) p.lse[row] = (float)r.lse;
     if (p.coef) p.coef[row] = coef;
   }
   return coef;
+}
+// (scored tokens of the row's sequence, policy_total) over the whole CTA.
+__device__ __forceinline__ int2 policy_counts(const PolicyRows& p, LpRows lr, int V, long long row, bool writer,
+                                              int* red) {
+  const unsigned b = lr.batch(row);
+  int2 c = make_int2(0, 0);
+  if (!p.count_here) {
+    c.y = policy_total(p.counts, p.B, p.a.by_sequence, red);
+    c.x = p.counts[b];
+    return c;
+  }
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (p.a.by_sequence) {  // a warp a sequence
+    for (unsigned s = threadIdx.x >> 5; s < (unsigned)p.B; s += warps) {
+      int n = 0;
+      for (int t = lane; t < lr.T; t += 32) n += lp_scored(p.labels[(long long)s * lr.T + t], p.ignore_index, V) ? 1 : 0;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) c.y += n > 0 ? 1 : 0, c.x += s == b ? n : 0;
+    }
+  } else {
+    for (unsigned i = threadIdx.x; i < (unsigned)p.B * (unsigned)lr.T; i += blockDim.x) {
+      const int n = lp_scored(p.labels[i], p.ignore_index, V) ? 1 : 0;
+      c.y += n;
+      c.x += i / (unsigned)lr.T == b ? n : 0;
+    }
+  }
+  c.y = lp_block_sum(c.y, red);
+  c.x = lp_block_sum(c.x, red);
+  if (writer && threadIdx.x == 0 && (unsigned)row == b * (unsigned)lr.T) p.counts[b] = c.x;
+  return c;
 }
 __device__ __forceinline__ void policy_row_unscored(const PolicyRows& p, long long row) {
   p.logps[row] = 0.f;
@@ -769,14 +815,15 @@ __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpR
   E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
   if (!lp_scored(label, p.ignore_index, V)) {
     if (threadIdx.x == 0 && sh.part == 0) policy_row_unscored(p, row);
+    if (p.count_here && sh.part == 0 && (unsigned)row % (unsigned)lr.T == 0) policy_counts(p, lr, V, row, true, red);
     if (d) lp_write_zero(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float xl = LpType<E>::get(x[label]);  // before an in-place gradient
-  const int total = policy_total(p.counts, p.B, p.a.by_sequence, red);
+  const int2 n = policy_counts(p, lr, V, row, sh.part == 0, red);
   const LpRow r = lp_row_sum<E, CL>(x, V, sh);
-  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, total, sh.part == 0);
+  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
   if (!d) return;
   __syncthreads();
   lp_write_grad<E, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
@@ -801,15 +848,18 @@ __global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logi
   E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
   if (!lp_scored(label, p.ignore_index, V)) {
     if (threadIdx.x == 0 && sh.part == 0) policy_row_unscored(p, row);
+    if (p.count_here && sh.part == 0 && (unsigned)row % (unsigned)lr.T == 0) policy_counts(p, lr, V, row, true, red);
     if (d) lp_write_zero(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float xl = L::get(x[label]);
   LpRow r;
-  lp_staged_sum<E, CL, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, &r);
-  const int total = policy_total(p.counts, p.B, p.a.by_sequence, red);
-  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, total, sh.part == 0);
+  int2 n;
+  lp_staged_sum<E, CL, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, &r, [&] {
+    n = policy_counts(p, lr, V, row, sh.part == 0, red);  // while the first pieces are on their way
+  });
+  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
   if (!d) return;
   __syncthreads();
   lp_write_grad<E, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
@@ -824,7 +874,7 @@ __global__ void __launch_bounds__(1024) policy_stats_kernel(const float* __restr
                                                             const int* __restrict__ counts, float* __restrict__ stats) {
   griddep_wait();
   griddep_launch();
-  __shared__ double red[32];
+  __shared__ double3 red[32];
   __shared__ int ired[32];
   const int total = policy_total(counts, B, a.by_sequence, ired);
   double pg = 0.0, kl = 0.0, cut = 0.0;
@@ -838,9 +888,8 @@ __global__ void __launch_bounds__(1024) policy_stats_kernel(const float* __restr
     kl += w * (double)t.kl;
     cut += w * (double)t.cut;
   }
-  pg = lp_block_sum(pg, red);
-  kl = lp_block_sum(kl, red);
-  cut = lp_block_sum(cut, red);
+  const double3 t = lp_block_sum3(make_double3(pg, kl, cut), red);
+  pg = t.x, kl = t.y, cut = t.z;
   if (threadIdx.x == 0) {
     stats[0] = (float)(pg + (double)a.kl * kl);
     stats[1] = (float)pg;
@@ -879,12 +928,13 @@ static void lp_dispatch(int dtype, F&& f) {
   else f((float*)nullptr);
 }
 
-// CTAs a row: doubled (up to the portable cluster of 8) while the grid leaves SMs without their share of CTAs and each
-// part keeps at least 8 KB of the row.
+// CTAs a row: doubled (up to the portable cluster of 8) while the grid stays within two CTAs an SM and each part keeps
+// at least 8 KB of the row. Policy loss of rows of 100 KB, us for 1 / 2 / 4 / 8 CTAs a row: 16 rows 20.5 / 20.5 / 18.4 /
+// 16.4, 64 rows 20.5 / 20.5 / 18.4 / 26.7, 148 rows 20.5 / 20.5 / 28.7 / 42.0, 300 rows 28.5 / 34.8 / 41.8 / 69.6.
 static int lp_parts(long long M, int V, int dtype) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const long long bytes = (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2), full = 4ll * rgpt_num_sms(dev);
+  const long long bytes = (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2), full = 2ll * rgpt_num_sms(dev);
   int c = 1;
   while (c < 8 && 2 * c * M <= full && bytes / (2 * c) >= 8192) c *= 2;
   return c;
@@ -1001,11 +1051,13 @@ extern "C" int rgpt_policy_loss(const void* logits, int dtype, long long sb, lon
   const PolicyArgs a = {clip_low, clip_high, kl_coef, grad_scale, log1p(-(double)clip_low), log1p((double)clip_high),
                         adv_per_token, by_sequence};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  launch_pdl(policy_count_kernel, dim3(B), dim3(256), 0, s, 1, labels, ignore_index, V, T, counts);
+  // up to this many tokens each CTA counts them for itself, while its row is on its way, which saves a launch
+  const int count_here = (long long)B * T <= 2048 ? 1 : 0;
+  if (!count_here) launch_pdl(policy_count_kernel, dim3(B), dim3(256), 0, s, 1, labels, ignore_index, V, T, counts);
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
     const LpRows lr = {sb, st, T}, dr = {db, dt, T};
-    const PolicyRows p = {labels, ignore_index, old_logps, ref_logps, advantages, counts, B, a, token_logps, lse, coef};
+    const PolicyRows p = {labels, ignore_index, old_logps, ref_logps, advantages, counts, B, count_here, a, token_logps, lse, coef};
     const unsigned M = (unsigned)((long long)B * T);
     const int c = lp_parts(M, V, dtype);
     if (lp_long(V, dtype)) {
@@ -1019,7 +1071,8 @@ extern "C" int rgpt_policy_loss(const void* logits, int dtype, long long sb, lon
                (const E*)logits, lr, V, p, (E*)dlogits, dr);
   });
   if (rc) return rc;
-  launch_pdl(policy_stats_kernel, dim3(1), dim3(1024), 0, s, 1, (const float*)token_logps, labels, ignore_index, V, B, T,
+  const long long M = (long long)B * T;
+  launch_pdl(policy_stats_kernel, dim3(1), dim3(M < 1024 ? (unsigned)((M + 31) / 32 * 32) : 1024u), 0, s, 1, (const float*)token_logps, labels, ignore_index, V, B, T,
              old_logps, ref_logps, advantages, a, (const int*)counts, stats);
   return rgpt_check_launch("policy_loss kernels");
 }

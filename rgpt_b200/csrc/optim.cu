@@ -94,8 +94,9 @@ __global__ void adamw_kernel(const RgptAdamwTensor* __restrict__ tab, const int*
 // One warp per block of 256 elements, 8 consecutive elements a lane: the two block maxima are warp reductions and the
 // block's codes are written from the registers that made them. Bound by HBM: 16 bytes a parameter (p read and
 // written, g read, both codes read and written) and 2 more for the bf16 copy, against 28 and 2 with fp32 moments.
-// Every operation is spelled out with its one rounding (no contraction), so that vector and scalar paths, and any
-// other program of the same formulas, give the same codes.
+// The moments' operations are spelled out with their one rounding each (no contraction), so that vector and scalar
+// paths, and any other program of the same formulas, give the same codes; the parameter's step divides by
+// multiplication (2 ulp of the step), which no code depends on.
 constexpr float A8_M_TOP = 448.0f, A8_M_STEP = (float)(1.0 / 448.0);
 constexpr float A8_R_TOP = 1.96875f, A8_R_STEP = (float)(1.0 / 1.96875);
 constexpr float A8_TINY = 7.888609052210118e-31f;  // 2^-100
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __r
   const long long end = min(start + (long long)chunk_elems, t.n);
   const int lane = threadIdx.x & 31;
   const float decay = __fsub_rn(1.0f, __fmul_rn(lr, wd));
-  const float w1 = __fsub_rn(1.0f, beta1), w2 = __fsub_rn(1.0f, beta2);
+  const float w1 = __fsub_rn(1.0f, beta1), w2 = __fsub_rn(1.0f, beta2), step = -lr * inv_bc1;
   const bool vec = aligned16(t.p) && aligned16(t.g) && aligned16(t.shadow) &&
                    ((reinterpret_cast<uintptr_t>(t.mq) | reinterpret_cast<uintptr_t>(t.vq)) & 7) == 0;
   for (long long b0 = start + 256ll * (threadIdx.x >> 5); b0 < end; b0 += 256ll * (blockDim.x >> 5)) {
@@ -169,8 +170,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __r
       const float q = __fmul_rn(a8_decode_r((cr[k >> 2] >> (8 * (k & 3))) & 0xFFu), rs);
       m[k] = __fadd_rn(__fmul_rn(m[k], beta1), __fmul_rn(g[k], w1));
       r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q, q), beta2), __fmul_rn(__fmul_rn(g[k], g[k]), w2)));
-      const float u = __fmul_rn(__fdiv_rn(m[k], __fadd_rn(__fmul_rn(r[k], inv_sqrt_bc2), eps)), inv_bc1);
-      p[k] = __fsub_rn(__fmul_rn(p[k], decay), __fmul_rn(u, lr));
+      const float u = __fdividef(m[k], fmaf(r[k], inv_sqrt_bc2, eps));
+      p[k] = fmaf(u, step, __fmul_rn(p[k], decay));
       am = fmaxf(am, fabsf(m[k]));
       ar = fmaxf(ar, r[k]);
     }
@@ -223,10 +224,34 @@ __global__ void __launch_bounds__(256) adamw8_moments_kernel(const unsigned char
                                                              float* __restrict__ v, long long n) {
   griddep_wait();
   griddep_launch();
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    const float r = __fmul_rn(a8_decode_r(vq[i]), rs[i >> 8]);
-    m[i] = __fmul_rn(a8_decode_m2(mq[i]).x, ms[i >> 8]);
-    v[i] = __fmul_rn(r, r);
+  // 4 elements a thread and step: a warp's loads and stores are whole lines (8 B read, 32 B written)
+  const bool vec = aligned16(m) && aligned16(v) && ((reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(vq)) & 3) == 0;
+  for (long long i = 4 * ((long long)blockIdx.x * blockDim.x + threadIdx.x); i < n; i += 4ll * gridDim.x * blockDim.x) {
+    const float a = ms[i >> 8], b = rs[i >> 8];
+    const int k = n - i < 4 ? (int)(n - i) : 4;
+    uint32_t cm = 0u, cr = 0u;
+    if (vec && k == 4) {
+      cm = *reinterpret_cast<const uint32_t*>(mq + i);
+      cr = *reinterpret_cast<const uint32_t*>(vq + i);
+    } else {
+      for (int j = 0; j < k; ++j) cm |= (uint32_t)mq[i + j] << (8 * j), cr |= (uint32_t)vq[i + j] << (8 * j);
+    }
+    const float2 m0 = a8_decode_m2(cm & 0xFFFFu), m1 = a8_decode_m2(cm >> 16);
+    const float om[4] = {__fmul_rn(m0.x, a), __fmul_rn(m0.y, a), __fmul_rn(m1.x, a), __fmul_rn(m1.y, a)};
+    float ov[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float r = __fmul_rn(a8_decode_r((cr >> (8 * j)) & 0xFFu), b);
+      ov[j] = __fmul_rn(r, r);
+    }
+    if (vec && k == 4) {
+      *reinterpret_cast<float4*>(m + i) = make_float4(om[0], om[1], om[2], om[3]);
+      *reinterpret_cast<float4*>(v + i) = make_float4(ov[0], ov[1], ov[2], ov[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < k) m[i + j] = om[j], v[i + j] = ov[j];
+    }
   }
 }
 
@@ -626,7 +651,7 @@ extern "C" int rgpt_adamw8(const RgptAdamw8Tensor* table, const int* chunk_tenso
 extern "C" int rgpt_adamw8_moments(const unsigned char* mq, const float* m_scale, const unsigned char* vq,
                                    const float* r_scale, float* m, float* v, long long n, void* stream) {
   if (n <= 0) return RGPT_OK;
-  const long long want = (n + 255) / 256;
+  const long long want = (n + 1023) / 1024;
   launch_pdl(adamw8_moments_kernel, dim3((unsigned)(want < 148 * 64 ? want : 148 * 64)), dim3(256), 0,
              reinterpret_cast<cudaStream_t>(stream), 1, mq, m_scale, vq, r_scale, m, v, n);
   return rgpt_check_launch("adamw8_moments_kernel");

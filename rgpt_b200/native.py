@@ -359,48 +359,53 @@ LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 
-def _call_on(device: torch.device, name: str, *args, kernels: int | None = None) -> None:
-    """_lib.call with `device` current (the library launches on the current device's context)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        _lib.call(name, *args, kernels=kernels)
+def _call_on(index: int, name: str, *args, kernels: int | None = None) -> None:
+    """_lib.call on the current stream of device `index`, with that device current (the library launches on the current
+    device's context). The stream is the call's last argument."""
+    if index < 0:
+        raise RuntimeError("librgpt_kernels only takes CUDA tensors (no CPU path)")
+    if index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, _lib.raw_stream(index), kernels=kernels)
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, kernels=kernels)
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _lib.raw_stream(index), kernels=kernels)
 
 
-def _flat(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device) -> int:
-    """Address of a contiguous tensor of the given shape, type and device (the caller's ptr() of another argument
-    sees to it that the device is a GPU)."""
-    if t.dtype != dtype:
+def _flat(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int) -> int:
+    """Address of a contiguous tensor of the given shape, type and device (-1: host memory, which _call_on refuses)."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}"
                          f" with strides {t.stride()}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected device {index}")
     return t.data_ptr()
 
 
-def _opt(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype, device: torch.device) -> int | None:
-    return None if t is None else _flat(t, name, shape, dtype, device)
+def _opt(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype, index: int) -> int | None:
+    return None if t is None else _flat(t, name, shape, dtype, index)
 
 
 def _logit_rows(t: torch.Tensor, name: str):
     """(dtype id, batch stride, token stride, B, T, V) of logits [B, T, V], or [M, V] as M sequences of one token."""
-    if t.dtype not in LOGIT_DTYPES:
+    dt = LOGIT_DTYPES.get(t.dtype)
+    if dt is None:
         raise TypeError(f"{name} must be bf16, fp16 or fp32, got {t.dtype}")
-    if t.dim() not in (2, 3):
-        raise ValueError(f"{name} must be [M, V] or [B, T, V], got {tuple(t.shape)}")
-    V = t.shape[-1]
-    if V > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must have unit stride along the vocabulary, got strides {t.stride()}")
-    if t.dim() == 2:
-        B, T, sb, st = t.shape[0], 1, t.stride(0), 0
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
+        B, T, V = shape
+        sb, st, sv = stride
+    elif len(shape) == 2:
+        (B, V), T = shape, 1
+        (sb, sv), st = stride, 0
     else:
-        (B, T), (sb, st) = t.shape[:2], t.stride()[:2]
-    if t.numel() and (B * T >= 2 ** 31 or V >= 2 ** 31):
-        raise ValueError(f"{name} must have fewer than 2^31 rows and columns, got {tuple(t.shape)}")
-    return LOGIT_DTYPES[t.dtype], sb, st, B, T, V
+        raise ValueError(f"{name} must be [M, V] or [B, T, V], got {tuple(shape)}")
+    if V > 1 and sv != 1:
+        raise ValueError(f"{name} must have unit stride along the vocabulary, got strides {stride}")
+    if B * T >= 2 ** 31 or V >= 2 ** 31:
+        raise ValueError(f"{name} must have fewer than 2^31 rows and columns, got {tuple(shape)}")
+    return dt, sb, st, B, T, V
 
 
 def _span(t: torch.Tensor):
@@ -413,17 +418,19 @@ def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):
     """(address, batch stride, token stride) of the gradient's rows: the logits themselves, or memory apart from them."""
     if dlogits is None:
         return None, 0, 0
-    if dlogits.dtype != logits.dtype or dlogits.shape != logits.shape or dlogits.device != logits.device:
+    if dlogits.dtype is not logits.dtype or dlogits.shape != logits.shape or dlogits.get_device() != logits.get_device():
         raise ValueError("dlogits must have the logits' type, shape and device")
     _, sb, st, B, T, V = _logit_rows(dlogits, "dlogits")
-    tokens = T == 1 or st >= V
-    if not (tokens and (B == 1 or sb >= (T - 1) * st + V)) and not (sb >= V and st >= (B - 1) * sb + V):
-        raise ValueError(f"the rows of dlogits overlap (strides {dlogits.stride()})")
-    if dlogits.data_ptr() != logits.data_ptr() or dlogits.stride() != logits.stride():
+    if not dlogits.is_contiguous():
+        tokens = T == 1 or st >= V
+        if not (tokens and (B == 1 or sb >= (T - 1) * st + V)) and not (sb >= V and st >= (B - 1) * sb + V):
+            raise ValueError(f"the rows of dlogits overlap (strides {dlogits.stride()})")
+    at = dlogits.data_ptr()
+    if at != logits.data_ptr() or dlogits.stride() != logits.stride():
         (a, b), (c, d) = _span(logits), _span(dlogits)
         if a < d and c < b:
             raise ValueError("dlogits must be the logits themselves or share no memory with them")
-    return dlogits.data_ptr(), sb, st
+    return at, sb, st
 
 
 def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, logps: torch.Tensor, *, lse: torch.Tensor | None = None,
@@ -432,14 +439,14 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, logps: torch.Tens
     vocabulary); lse (optional, for token_logprobs_bwd) = logsumexp. logits [M, V] or [B, T, V] in bf16, fp16 or fp32
     with unit stride along the vocabulary and any other strides; labels int64, logps and lse fp32 of the leading shape."""
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
-    dev, shape = logits.device, logits.shape[:-1]
+    dev, shape = logits.get_device(), logits.shape[:-1]
     args = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
             _flat(logps, "logps", shape, torch.float32, dev), _opt(lse, "lse", shape, torch.float32, dev))
     if B * T == 0:
         return
     if V == 0:
         raise ValueError("token_logprobs: the vocabulary is empty")
-    _call_on(dev, "rgpt_token_logprobs", ptr(logits), dt, sb, st, B, T, V, *args, _lib.stream_ptr(dev))
+    _call_on(dev, "rgpt_token_logprobs", logits.data_ptr(), dt, sb, st, B, T, V, *args)
 
 
 def token_logprobs_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, dlogps: torch.Tensor,
@@ -447,13 +454,13 @@ def token_logprobs_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Te
     """dlogits = dlogps * (onehot(label) - softmax(logits)), zero rows for tokens that are not scored. dlogits: the
     logits themselves (overwritten) or another tensor of their type and shape."""
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
-    dev, shape = logits.device, logits.shape[:-1]
+    dev, shape = logits.get_device(), logits.shape[:-1]
     args = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
             _flat(lse, "lse", shape, torch.float32, dev), _flat(dlogps, "dlogps", shape, torch.float32, dev))
     grad = _grad_rows(dlogits, logits)
     if B * T == 0 or V == 0:
         return
-    _call_on(dev, "rgpt_token_logprobs_bwd", ptr(logits), dt, sb, st, B, T, V, *args, *grad, _lib.stream_ptr(dev))
+    _call_on(dev, "rgpt_token_logprobs_bwd", logits.data_ptr(), dt, sb, st, B, T, V, *args, *grad)
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
@@ -479,7 +486,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     if logits.dim() != 3 or B % 2 or B == 0 or T == 0 or V == 0:
         raise ValueError(f"preference_loss needs logits [2P, T, V] of at least one pair and token, got {tuple(logits.shape)}")
-    dev, P, f32 = logits.device, B // 2, torch.float32
+    dev, P, f32 = logits.get_device(), B // 2, torch.float32
     lab = _flat(labels, "labels", (B, T), torch.int64, dev)
     ref = _opt(ref_logps, "ref_logps", (B,), f32, dev)
     outs = (_flat(token_logps, "token_logps", (B, T), f32, dev), _flat(lse, "lse", (B, T), f32, dev),
@@ -487,12 +494,11 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
             _flat(coef, "coef", (B,), f32, dev), _flat(loss, "loss", (1,), f32, dev))
     grad = _grad_rows(dlogits, logits)
     _opt(scratch, "scratch", (B, T), torch.float64, dev)
-    at = ptr(logits)
     if scratch is None:
-        scratch = torch.empty(B, T, device=dev, dtype=torch.float64)
-    _call_on(dev, "rgpt_preference_loss", at, dt, sb, st, P, T, V, lab, int(ignore_index), ref,
+        scratch = torch.empty(B, T, device=logits.device, dtype=torch.float64)
+    _call_on(dev, "rgpt_preference_loss", logits.data_ptr(), dt, sb, st, P, T, V, lab, int(ignore_index), ref,
              PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
-             float(grad_scale), *outs, scratch.data_ptr(), *grad, _lib.stream_ptr(dev),
+             float(grad_scale), *outs, scratch.data_ptr(), *grad,
              kernels=3 + (dlogits is not None))
 
 
@@ -514,8 +520,8 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     if kl_coef != 0.0 and ref_logps is None:
         raise ValueError("policy_loss: kl_coef needs ref_logps")
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
-    dev, shape, f32 = logits.device, logits.shape[:-1], torch.float32
-    per_token = tuple(advantages.shape) != (B,)
+    dev, shape, f32 = logits.get_device(), logits.shape[:-1], torch.float32
+    per_token = advantages.shape != (B,)
     adv = _flat(advantages, "advantages", shape if per_token else (B,), f32, dev)
     ins = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
            _flat(old_logps, "old_logps", shape, f32, dev), _opt(ref_logps, "ref_logps", shape, f32, dev))
@@ -524,9 +530,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     grad = _grad_rows(dlogits, logits)
     if B * T == 0 or V == 0:
         raise ValueError(f"policy_loss needs at least one token, got logits {tuple(logits.shape)}")
-    _call_on(dev, "rgpt_policy_loss", ptr(logits), dt, sb, st, B, T, V, *ins, adv, int(per_token), float(clip_low),
+    _call_on(dev, "rgpt_policy_loss", logits.data_ptr(), dt, sb, st, B, T, V, *ins, adv, int(per_token), float(clip_low),
              float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *outs, *grad,
-             _lib.stream_ptr(dev), kernels=3)
+             kernels=2 + (B * T > 2048))
 
 
 def _linear_operands(x: torch.Tensor, w: torch.Tensor):
@@ -553,19 +559,19 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
     first, which gives what token_logprobs gives on stored bf16 logits. part: fp32 scratch of at least
     2 * M * ceil(V/128) elements (allocated when None)."""
     M, V, K = _linear_operands(x, w)
-    dev = x.device
+    dev = x.get_device()
     need = 2 * M * ((V + 127) // 128)
     lab = _flat(labels, "labels", (M,), torch.int64, dev)
     outs = (_flat(logps, "logps", (M,), torch.float32, dev), _opt(lse, "lse", (M,), torch.float32, dev))
     if part is not None and (part.numel() < need or part.dtype != torch.float32 or not part.is_contiguous()
-                             or part.device != dev):
+                             or part.get_device() != dev):
         raise ValueError(f"linear_logprobs: part must be a contiguous fp32 tensor of at least {need} elements")
     if M == 0:
         return
     if part is None:
-        part = torch.empty(need, device=dev, dtype=torch.float32)
-    _call_on(dev, "rgpt_linear_logprobs", ptr(x), x.stride(0), ptr(w), w.stride(0), M, V, K, lab, int(ignore_index),
-             int(bool(round_bf16)), ptr(part), part.numel(), *outs, _lib.stream_ptr(dev))
+        part = torch.empty(need, device=x.device, dtype=torch.float32)
+    _call_on(dev, "rgpt_linear_logprobs", x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), M, V, K, lab, int(ignore_index),
+             int(bool(round_bf16)), part.data_ptr(), part.numel(), *outs)
 
 
 # Gradient rows of linear_logprobs_bwd in flight: at most this many bf16 logit gradients (1 GiB) at a time.
@@ -580,9 +586,8 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
     as many as fit 1 GiB): its tiles come from the recomputed product, rounded to bf16 for the two GEMMs that follow."""
     M, V, K = _linear_operands(x, w)
     dev = x.device
-    _flat(labels, "labels", (M,), torch.int64, dev)
-    _flat(lse, "lse", (M,), torch.float32, dev)
-    _flat(dlogps, "dlogps", (M,), torch.float32, dev)
+    for t, n, dtype in ((labels, "labels", torch.int64), (lse, "lse", torch.float32), (dlogps, "dlogps", torch.float32)):
+        _flat(t, n, (M,), dtype, x.get_device())
     for t, n, shape in ((dx, "dx", (M, K)), (dw, "dw", (V, K))):
         if t is not None and (tuple(t.shape) != shape or t.dtype not in (torch.bfloat16, torch.float32)
                               or t.stride(1) != 1 or t.stride(0) % 8 or t.device != dev):
@@ -645,13 +650,11 @@ def adamw8(table: torch.Tensor, chunk_tensor: torch.Tensor, chunk_start: torch.T
 def adamw8_moments(mq: torch.Tensor, m_scale: torch.Tensor, vq: torch.Tensor, v_scale: torch.Tensor, m: torch.Tensor,
                    v: torch.Tensor) -> None:
     """m, v (fp32) = the moments that 8-bit codes and their scales stand for."""
-    n, dev = m.numel(), m.device
+    n, dev, f32 = m.numel(), m.get_device(), torch.float32
     blocks = (n + ADAM8_BLOCK - 1) // ADAM8_BLOCK
-    args = (_flat(mq.view(-1), "m codes", (n,), torch.uint8, dev), _flat(m_scale, "m scales", (blocks,), torch.float32, dev),
-            _flat(vq.view(-1), "v codes", (n,), torch.uint8, dev), _flat(v_scale, "v scales", (blocks,), torch.float32, dev),
-            ptr(m), _flat(v, "v", m.shape, torch.float32, dev))
-    _flat(m, "m", m.shape, torch.float32, dev)
-    _call_on(dev, "rgpt_adamw8_moments", *args, n, _lib.stream_ptr(dev))
+    _call_on(dev, "rgpt_adamw8_moments", _flat(mq, "m codes", (n,), torch.uint8, dev), _flat(m_scale, "m scales", (blocks,), f32, dev),
+             _flat(vq, "v codes", (n,), torch.uint8, dev), _flat(v_scale, "v scales", (blocks,), f32, dev),
+             _flat(m, "m", m.shape, f32, dev), _flat(v, "v", m.shape, f32, dev), n)
 
 
 def muon_prep(table, n, R, C, X, beta, nesterov, sumsq, hp: int | None = None) -> None:
