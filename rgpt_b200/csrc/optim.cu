@@ -91,12 +91,16 @@ __global__ void adamw_kernel(const RgptAdamwTensor* __restrict__ tab, const int*
 }
 
 // ---------------------------------------------------------------------------- AdamW, 8-bit moments
-// One warp per block of 256 elements, 8 consecutive elements a lane: the two block maxima are warp reductions and the
+// One warp per block of 256 elements, 8 elements a lane: the two block maxima are warp reductions and the
 // block's codes are written from the registers that made them. Bound by HBM: 16 bytes a parameter (p read and
 // written, g read, both codes read and written) and 2 more for the bf16 copy, against 28 and 2 with fp32 moments.
 // The moments' operations are spelled out with their one rounding each (no contraction), so that vector and scalar
-// paths, and any other program of the same formulas, give the same codes; the parameter's step divides by
-// multiplication (2 ulp of the step), which no code depends on.
+// paths, and any other program of the same formulas, give the same codes; the parameter's step multiplies by an
+// approximate reciprocal (2 ulp of the step), which no code depends on.
+// Two warps a CTA, 20 CTAs an SM, and chunks of few blocks (the host cuts 2048 elements): the blocks of a CTA come one
+// after another, stores before the next loads, so it is the many CTAs that keep loads on their way. 51.5 M parameters
+// with the bf16 copy, us by threads and chunk: 256 x 16384 203, 256 x 2048 163, 128 x 2048 154, 64 x 2048 152 (6.1 TB/s).
+constexpr int A8_THREADS = 64;
 constexpr float A8_M_TOP = 448.0f, A8_M_STEP = (float)(1.0 / 448.0);
 constexpr float A8_R_TOP = 1.96875f, A8_R_STEP = (float)(1.0 / 1.96875);
 constexpr float A8_TINY = 7.888609052210118e-31f;  // 2^-100
@@ -105,19 +109,22 @@ constexpr float A8_TINY = 7.888609052210118e-31f;  // 2^-100
 __device__ __forceinline__ uint32_t a8_encode_r(float y) {
   const uint32_t bits = __float_as_uint(y);
   const uint32_t fine = ((bits + 0x1FFFFu + ((bits >> 18) & 1u)) >> 18) - (120u << 5);
-  const uint32_t q = y >= 0.015625f ? fine : (uint32_t)__float2int_rn(__fmul_rn(y, 2048.0f));
+  // 1.5 * 2^23 added: the nearest integer of 2048 y in the low bits
+  const uint32_t q = y >= 0.015625f ? fine : __float_as_uint(fmaf(y, 2048.0f, 12582912.0f)) - 0x4B400000u;
   return q < 255u ? q : 255u;
 }
-// The code's bits are those of a half of the same exponent width below its bias: value * 2^-8, denormals included.
+// The code's bits are those of a half of the same exponent width below its bias: value * 2^-8, denormals included
+// (the 2^8 goes into the scale, where it is exact).
+constexpr float A8_R_UNIT = 256.0f;
 __device__ __forceinline__ float a8_decode_r(uint32_t q) {
-  return __half2float(__ushort_as_half((unsigned short)(q << 5))) * 256.0f;
+  return __half2float(__ushort_as_half((unsigned short)(q << 5)));
 }
 __device__ __forceinline__ float2 a8_decode_m2(uint32_t q2) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q2, __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-__global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __restrict__ tab,
+__global__ void __launch_bounds__(A8_THREADS, 20) adamw8_kernel(const RgptAdamw8Tensor* __restrict__ tab,
                                                      const int* __restrict__ chunk_tensor,
                                                      const long long* __restrict__ chunk_start, int chunk_elems,
                                                      float lr, float wd, float beta1, float beta2, float eps,
@@ -133,29 +140,34 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __r
   const int lane = threadIdx.x & 31;
   const float decay = __fsub_rn(1.0f, __fmul_rn(lr, wd));
   const float w1 = __fsub_rn(1.0f, beta1), w2 = __fsub_rn(1.0f, beta2), step = -lr * inv_bc1;
-  const bool vec = aligned16(t.p) && aligned16(t.g) && aligned16(t.shadow) &&
-                   ((reinterpret_cast<uintptr_t>(t.mq) | reinterpret_cast<uintptr_t>(t.vq)) & 7) == 0;
+  const bool vec = aligned16(t.p) && aligned16(t.g) && (reinterpret_cast<uintptr_t>(t.shadow) & 7) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(t.mq) | reinterpret_cast<uintptr_t>(t.vq)) & 3) == 0;
+  // lane l takes elements 4 l .. 4 l + 3 of both halves of a block: every access of a warp is one contiguous run
   for (long long b0 = start + 256ll * (threadIdx.x >> 5); b0 < end; b0 += 256ll * (blockDim.x >> 5)) {
-    const long long i = b0 + 8 * lane;
-    const bool whole = vec && i + 8 <= end;
-    const int n = end - i >= 8 ? 8 : (end > i ? (int)(end - i) : 0);
-    const float ms = t.m_scale[b0 >> 8], rs = t.r_scale[b0 >> 8];
+    const long long i = b0 + 4 * lane;
+    const bool whole = vec && b0 + 256 <= end;  // warp-uniform
+    auto inside = [&](int k) { return i + k + (k >= 4 ? 124 : 0) < end; };
+    auto at = [&](int k) { return i + k + (k >= 4 ? 124 : 0); };
+    const float ms = t.m_scale[b0 >> 8], rs = A8_R_UNIT * t.r_scale[b0 >> 8];
     float p[8], g[8], m[8], r[8];
     uint32_t cm[2] = {0u, 0u}, cr[2] = {0u, 0u};
     if (whole) {
-      const float4 p0 = *reinterpret_cast<const float4*>(t.p + i), p1 = *reinterpret_cast<const float4*>(t.p + i + 4);
-      const float4 g0 = *reinterpret_cast<const float4*>(t.g + i), g1 = *reinterpret_cast<const float4*>(t.g + i + 4);
-      const uint2 a = *reinterpret_cast<const uint2*>(t.mq + i), b = *reinterpret_cast<const uint2*>(t.vq + i);
-      p[0] = p0.x, p[1] = p0.y, p[2] = p0.z, p[3] = p0.w, p[4] = p1.x, p[5] = p1.y, p[6] = p1.z, p[7] = p1.w;
-      g[0] = g0.x, g[1] = g0.y, g[2] = g0.z, g[3] = g0.w, g[4] = g1.x, g[5] = g1.y, g[6] = g1.z, g[7] = g1.w;
-      cm[0] = a.x, cm[1] = a.y, cr[0] = b.x, cr[1] = b.y;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 pv = *reinterpret_cast<const float4*>(t.p + i + 128 * h);
+        const float4 gv = *reinterpret_cast<const float4*>(t.g + i + 128 * h);
+        cm[h] = *reinterpret_cast<const uint32_t*>(t.mq + i + 128 * h);
+        cr[h] = *reinterpret_cast<const uint32_t*>(t.vq + i + 128 * h);
+        p[4 * h] = pv.x, p[4 * h + 1] = pv.y, p[4 * h + 2] = pv.z, p[4 * h + 3] = pv.w;
+        g[4 * h] = gv.x, g[4 * h + 1] = gv.y, g[4 * h + 2] = gv.z, g[4 * h + 3] = gv.w;
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        p[k] = k < n ? t.p[i + k] : 0.f;
-        g[k] = k < n ? t.g[i + k] : 0.f;
-        cm[k >> 2] |= (k < n ? (uint32_t)t.mq[i + k] : 0u) << (8 * (k & 3));
-        cr[k >> 2] |= (k < n ? (uint32_t)t.vq[i + k] : 0u) << (8 * (k & 3));
+        p[k] = inside(k) ? t.p[at(k)] : 0.f;
+        g[k] = inside(k) ? t.g[at(k)] : 0.f;
+        cm[k >> 2] |= (inside(k) ? (uint32_t)t.mq[at(k)] : 0u) << (8 * (k & 3));
+        cr[k >> 2] |= (inside(k) ? (uint32_t)t.vq[at(k)] : 0u) << (8 * (k & 3));
       }
     }
     float am = 0.f, ar = 0.f;
@@ -170,7 +182,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __r
       const float q = __fmul_rn(a8_decode_r((cr[k >> 2] >> (8 * (k & 3))) & 0xFFu), rs);
       m[k] = __fadd_rn(__fmul_rn(m[k], beta1), __fmul_rn(g[k], w1));
       r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q, q), beta2), __fmul_rn(__fmul_rn(g[k], g[k]), w2)));
-      const float u = __fdividef(m[k], fmaf(r[k], inv_sqrt_bc2, eps));
+      const float u = __fmul_rn(m[k], rcp_approx(fmaf(r[k], inv_sqrt_bc2, eps)));
       p[k] = fmaf(u, step, __fmul_rn(p[k], decay));
       am = fmaxf(am, fabsf(m[k]));
       ar = fmaxf(ar, r[k]);
@@ -197,21 +209,23 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const RgptAdamw8Tensor* __r
       t.r_scale[b0 >> 8] = __fmul_rn(ar, A8_R_STEP);
     }
     if (whole) {
-      *reinterpret_cast<float4*>(t.p + i) = make_float4(p[0], p[1], p[2], p[3]);
-      *reinterpret_cast<float4*>(t.p + i + 4) = make_float4(p[4], p[5], p[6], p[7]);
-      *reinterpret_cast<uint2*>(t.mq + i) = make_uint2(cm[0], cm[1]);
-      *reinterpret_cast<uint2*>(t.vq + i) = make_uint2(cr[0], cr[1]);
-      if (t.shadow)
-        *reinterpret_cast<uint4*>(t.shadow + i) = make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
-                                                             pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7]));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<float4*>(t.p + i + 128 * h) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+        *reinterpret_cast<uint32_t*>(t.mq + i + 128 * h) = cm[h];
+        *reinterpret_cast<uint32_t*>(t.vq + i + 128 * h) = cr[h];
+        if (t.shadow)
+          *reinterpret_cast<uint2*>(t.shadow + i + 128 * h) =
+              make_uint2(pack_bf16x2(p[4 * h], p[4 * h + 1]), pack_bf16x2(p[4 * h + 2], p[4 * h + 3]));
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (k >= n) continue;
-        t.p[i + k] = p[k];
-        t.mq[i + k] = (unsigned char)(cm[k >> 2] >> (8 * (k & 3)));
-        t.vq[i + k] = (unsigned char)(cr[k >> 2] >> (8 * (k & 3)));
-        if (t.shadow) t.shadow[i + k] = __bfloat16_as_ushort(__float2bfloat16(p[k]));
+        if (!inside(k)) continue;
+        t.p[at(k)] = p[k];
+        t.mq[at(k)] = (unsigned char)(cm[k >> 2] >> (8 * (k & 3)));
+        t.vq[at(k)] = (unsigned char)(cr[k >> 2] >> (8 * (k & 3)));
+        if (t.shadow) t.shadow[at(k)] = __bfloat16_as_ushort(__float2bfloat16(p[k]));
       }
     }
   }
@@ -227,7 +241,7 @@ __global__ void __launch_bounds__(256) adamw8_moments_kernel(const unsigned char
   // 4 elements a thread and step: a warp's loads and stores are whole lines (8 B read, 32 B written)
   const bool vec = aligned16(m) && aligned16(v) && ((reinterpret_cast<uintptr_t>(mq) | reinterpret_cast<uintptr_t>(vq)) & 3) == 0;
   for (long long i = 4 * ((long long)blockIdx.x * blockDim.x + threadIdx.x); i < n; i += 4ll * gridDim.x * blockDim.x) {
-    const float a = ms[i >> 8], b = rs[i >> 8];
+    const float a = ms[i >> 8], b = A8_R_UNIT * rs[i >> 8];
     const int k = n - i < 4 ? (int)(n - i) : 4;
     uint32_t cm = 0u, cr = 0u;
     if (vec && k == 4) {
@@ -643,7 +657,7 @@ extern "C" int rgpt_adamw8(const RgptAdamw8Tensor* table, const int* chunk_tenso
     inv_bc1 = (float)(1.0 / (1.0 - pow((double)beta1, (double)step)));
     inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow((double)beta2, (double)step)));
   }
-  launch_pdl(adamw8_kernel, dim3(n_chunks), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1, table, chunk_tensor,
+  launch_pdl(adamw8_kernel, dim3(n_chunks), dim3(A8_THREADS), 0, reinterpret_cast<cudaStream_t>(stream), 1, table, chunk_tensor,
              chunk_start, chunk_elems, lr, wd, beta1, beta2, eps, inv_bc1, inv_sqrt_bc2, hp);
   return rgpt_check_launch("adamw8_kernel");
 }

@@ -410,8 +410,10 @@ def _logit_rows(t: torch.Tensor, name: str):
 
 def _span(t: torch.Tensor):
     """[first, last) address of a tensor's elements."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    at, last = t.data_ptr(), 1
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    return at, at + last * t.element_size()
 
 
 def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):

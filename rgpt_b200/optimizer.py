@@ -30,6 +30,7 @@ from . import native as nv
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)  # optimizer.py:19
 _ADAM_CHUNK = 16384
+_ADAM8_CHUNK = 2048
 ADAM8_MIN_NUMEL = 4096  # smaller parameters keep fp32 moments under adam_state_bits=8
 _HP_RING = 4  # pinned host slots for the per-step scalars (copies in flight before a slot is reused)
 
@@ -585,20 +586,20 @@ class Muon(torch.optim.Optimizer):
         ent = self._cache.get(key)
         if ent is None:
             dev = params[0].device
-            pieces = [(ti, s) for ti, p in enumerate(params) for s in range(0, p.numel(), _ADAM_CHUNK)]
+            pieces = [(ti, s) for ti, p in enumerate(params) for s in range(0, p.numel(), _ADAM8_CHUNK)]
             ent = (_table(rows, dev), torch.tensor([t for t, _ in pieces], dtype=torch.int32).to(dev),
                    torch.tensor([s for _, s in pieces], dtype=torch.int64).to(dev))
             self._cache[key] = ent
         table, ct, cs = ent
-        return lambda: nv.adamw8(table, ct, cs, _ADAM_CHUNK, lr, wd, beta1, beta2, eps, step_i, hp=self._hp(gi))
+        return lambda: nv.adamw8(table, ct, cs, _ADAM8_CHUNK, lr, wd, beta1, beta2, eps, step_i, hp=self._hp(gi))
 
-    @torch.no_grad()
     def adam_moments(self, p: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """The fp32 first and second AdamW moments of parameter p, whichever way its group holds them: the state's
         own tensors with 32 bits, new ones decoded from their codes with 8."""
         st = self.state.get(p, {})
         if "exp_avg_q8" in st:
-            m, v = torch.empty_like(p), torch.empty_like(p)
+            both = torch.empty((2,) + p.shape, device=p.device, dtype=torch.float32)
+            m, v = both[0], both[1]
             nv.adamw8_moments(st["exp_avg_q8"], st["exp_avg_scale"], st["exp_avg_sq_q8"], st["exp_avg_sq_scale"], m, v)
             return m, v
         if "exp_avg" not in st:
