@@ -265,7 +265,7 @@ int rgpt_policy_loss(const void* logits, int dtype, long long sb, long long st, 
 /* Log-probabilities straight from hidden states, logits = X @ W^T never stored: X [M, K], W [V, K] bf16, K-major,
  * 16-byte aligned rows; labels [M]. logps [M], lse [M] (optional, written for every row) as rgpt_token_logprobs over
  * the fp32 product (round_bf16: over the product rounded to bf16, which is what a stored bf16 product gives).
- * part: scratch of part_floats >= 2 * M * ceil(V/128) floats, 8-byte aligned. */
+ * part: scratch of part_floats >= 4 * M * ceil(V/128) floats, 8-byte aligned. */
 int rgpt_linear_logprobs(const void* X, long long ldx, const void* W, long long ldw, int M, int V, int K,
                          const long long* labels, long long ignore_index, int round_bf16, float* part,
                          long long part_floats, float* logps, float* lse, void* stream);

@@ -31,7 +31,7 @@
 //   POLY_F32     the same in fp32 (C and D fp32)     (fp32 Newton-Schulz on split bf16 operands)
 //   ARGMAX_BF16  per row and column tile: the first maximum of bf16(acc) and its column; no output
 //                matrix (the rGPT per-step lm_head argmax, model/gpt.py:119-120)
-//   LSE_F32      per row and column tile: maximum and sum of exponentials, and the label's value; no output
+//   LSE_F32      per row and half column tile: maximum and sum of exponentials, and the label's value; no output
 //                matrix (log-probabilities from hidden states)
 //   SOFTMAX_GRAD coef[row] * ([column = label] - e^{acc - lse[row]}): the gradient tiles of those
 //                log-probabilities, from the recomputed product
@@ -74,7 +74,7 @@ struct EpiParams {
   // LSE_F32 / SOFTMAX_GRAD_BF16: each row's label (scored when in [0, N) and not ignore_index)
   const long long* labels;
   long long ignore_index;
-  float2* lse_part;        // LSE_F32: [column tile][M] (maximum, sum of e^{v - maximum}) of the tile's columns
+  float2* lse_part;        // LSE_F32: [half column tile][M] (maximum, sum of e^{v - maximum}) of its columns
   float* label_logit;      // LSE_F32: [M], the label's value, written for scored rows only
   int round_bf16;          // LSE_F32: the values are rounded to bf16 first (what a stored bf16 product would hold)
   const float* row_lse;    // SOFTMAX_GRAD_BF16: [M]
@@ -86,10 +86,15 @@ constexpr int GEMM_BK = 64;
 // Epilogue warps per CTA (EW): 4 = one per TMEM lane quadrant; 8 = two per quadrant, each taking half
 // of the tile's columns, for the epilogues that read an input C (their per-chunk work is the longest),
 // so that two warps per SM sub-partition hide each other's latency (measured 2-5 % faster there;
-// the two-output activation forward measured slower with 8).
+// the two-output activation forward measured slower with 8). The exponential epilogues take 8 as well.
 __host__ __device__ constexpr int gemm_epi_warps(int epi) {
   return (epi == RGPT_EPI_ACT_BWD || epi == RGPT_EPI_POLY_BF16 || epi == RGPT_EPI_RESID_F32 ||
-          epi == RGPT_EPI_POLY_F32) ? 8 : 4;
+          epi == RGPT_EPI_POLY_F32 || epi == RGPT_EPI_LSE_F32 || epi == RGPT_EPI_SOFTMAX_GRAD_BF16) ? 8 : 4;
+}
+// Warps with staging buffers for a stored output: none where the epilogue keeps only a row's sums, whose shared memory
+// goes to operand stages instead.
+__host__ __device__ constexpr int gemm_staging_warps(int epi) {
+  return epi == RGPT_EPI_LSE_F32 ? 0 : gemm_epi_warps(epi);
 }
 __host__ __device__ constexpr int gemm_threads(int ew) { return 64 + 32 * ew; }
 constexpr int GROUP_M = 8;
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
                         GemmShape sh, EpiParams ep) {
   constexpr bool reads_c = epi_reads_c(EPI);
   constexpr int EW = gemm_epi_warps(EPI);
-  using L = GemmSmem<BN, STAGES, PAIR, EW>;
+  using L = GemmSmem<BN, STAGES, PAIR, gemm_staging_warps(EPI)>;
   constexpr int NUM_ACC = 512 / BN;  // TMEM accumulator buffers (2 for 256-wide tiles, 4 for 128-wide)
   constexpr uint32_t TMEM_COLS = NUM_ACC * BN;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
           }
           s += (a0.x + a0.y) + (a1.x + a1.y);
         }
-        if (row < sh.M) ep.lse_part[(long long)nt * sh.M + row] = make_float2(m, s);
+        if (row < sh.M) ep.lse_part[(long long)(nt * (EW / 4) + col_half) * sh.M + row] = make_float2(m, s);
       } else if constexpr (bf16_out) {
         // SOFTMAX_GRAD: this thread's row of labels, log-sum-exps and coefficients
         float g_lse = 0.f, g_coef = 0.f;
@@ -791,10 +796,11 @@ template <int BN, int STAGES_IN, int A_MN, int B_MN, int EPI, bool PAIR, int ACT
 static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const CUtensorMap& td2,
                        const GemmShape& sh, const EpiParams& ep, cudaStream_t stream, int dev) {
   constexpr int EW = gemm_epi_warps(EPI);
-  constexpr int STAGES = gemm_fit_stages<BN, PAIR, EW>(STAGES_IN);
+  constexpr int SW = gemm_staging_warps(EPI);
+  constexpr int STAGES = gemm_fit_stages<BN, PAIR, SW>(SW == 0 ? STAGES_IN + 2 : STAGES_IN);
   constexpr int THREADS = gemm_threads(EW);
   auto kern = gemm_bf16_tc_kernel<BN, STAGES, A_MN, B_MN, EPI, PAIR, ACT>;
-  constexpr uint32_t smem = GemmSmem<BN, STAGES, PAIR, EW>::TOTAL;
+  constexpr uint32_t smem = GemmSmem<BN, STAGES, PAIR, SW>::TOTAL;
   static_assert(smem <= 232448, "GEMM shared memory exceeds the per-CTA limit");
   static bool attr_set[64] = {false};
   static int max_clusters[64] = {0};
@@ -1177,7 +1183,7 @@ extern "C" int rgpt_gemm_argmax(const void* A, long long lda, const void* B, lon
   return rgpt_check_launch("argmax_reduce_kernel");
 }
 
-// Joins the LSE_F32 GEMM's column tiles: lane = row (32 rows a CTA, coalesced reads of part[tile][row]), the warps
+// Joins the LSE_F32 GEMM's half column tiles: lane = row (32 rows a CTA, coalesced reads of part[tile][row]), the warps
 // share the tiles, and the CTA combines their (maximum, sum) pairs in a fixed order. On entry logps holds the scored
 // rows' label logits. lse and the log-probability are formed in fp64 and rounded once.
 __global__ void __launch_bounds__(1024) lse_reduce_kernel(const float2* __restrict__ part, int n_tiles, int M, int N,
@@ -1222,14 +1228,14 @@ extern "C" int rgpt_linear_logprobs(const void* X, long long ldx, const void* W,
   if (st) return st;
   if (logps == nullptr || part == nullptr || (reinterpret_cast<uintptr_t>(part) & 7) != 0)
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "linear_logprobs: null or misaligned output or partial buffer");
-  if (M >= 1 && V >= 1 && part_floats < 2ll * M * ((V + 127) / 128))
-    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "linear_logprobs: the partial buffer needs 2 * M * ceil(V / 128) floats");
+  if (M >= 1 && V >= 1 && part_floats < 4ll * M * ((V + 127) / 128))
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "linear_logprobs: the partial buffer needs 4 * M * ceil(V / 128) floats");
   LogpArgs a = {labels, ignore_index, reinterpret_cast<float2*>(part), logps, round_bf16, nullptr, nullptr, 0};
   st = gemm_entry(X, 0, ldx, 0, W, 0, ldw, 0, M, V, K, 1, RGPT_EPI_LSE_F32, 0, 1.0f, 0.0f, nullptr, 0, 0, nullptr, 0, 0,
                   nullptr, 0, 0, nullptr, 1, nullptr, nullptr, stream, nullptr, &a);
   if (st) return st;
   launch_pdl(lse_reduce_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, reinterpret_cast<cudaStream_t>(stream), 1,
-             (const float2*)part, a.n_tiles, M, V, labels, ignore_index, logps, lse);
+             (const float2*)part, a.n_tiles * (gemm_epi_warps(RGPT_EPI_LSE_F32) / 4), M, V, labels, ignore_index, logps, lse);
   return rgpt_check_launch("lse_reduce_kernel");
 }
 

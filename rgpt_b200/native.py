@@ -559,10 +559,10 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
 
     lse [M] (optional, for linear_logprobs_bwd) is written for every row. round_bf16: the products are rounded to bf16
     first, which gives what token_logprobs gives on stored bf16 logits. part: fp32 scratch of at least
-    2 * M * ceil(V/128) elements (allocated when None)."""
+    4 * M * ceil(V/128) elements (allocated when None)."""
     M, V, K = _linear_operands(x, w)
     dev = x.get_device()
-    need = 2 * M * ((V + 127) // 128)
+    need = 4 * M * ((V + 127) // 128)
     lab = _flat(labels, "labels", (M,), torch.int64, dev)
     outs = (_flat(logps, "logps", (M,), torch.float32, dev), _opt(lse, "lse", (M,), torch.float32, dev))
     if part is not None and (part.numel() < need or part.dtype != torch.float32 or not part.is_contiguous()
