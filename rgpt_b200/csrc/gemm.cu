@@ -51,6 +51,8 @@ struct GemmShape {
   int m_tiles, n_tiles, splitk, kb_per_split, num_kb;
   int num_units;
   int group_m;  // row tiles per visiting group (see decode_unit)
+  int bn;       // columns of a tile: BN, or for LSE_F32 any multiple of 16 up to it
+  int am;       // rows of A that a tile loads: all 128, or for LSE_F32 those that exist, rounded up to 8
 };
 
 struct EpiParams {
@@ -209,7 +211,10 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
   constexpr uint32_t TMEM_COLS = NUM_ACC * BN;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
   constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // rows of B this CTA loads
-  constexpr uint32_t IDESC = make_idesc_bf16(TILE_M, BN, A_MN, B_MN);
+  // LSE_F32 stores no tiles, so its width may be cut to what spreads a short sweep evenly over the SMs
+  constexpr bool CUT = EPI == RGPT_EPI_LSE_F32 && !PAIR;
+  const int bn = CUT ? sh.bn : BN;
+  const uint32_t IDESC = make_idesc_bf16(TILE_M, CUT ? bn : BN, A_MN, B_MN);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -285,11 +290,11 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
           return B_MN ? max(0, min(B_ROWS / 64, (sh.N - nt * BN - rk * B_ROWS + 63) / 64)) : 1;
         };
         auto stage_bytes = [&](int rk) -> uint32_t {
-          return (A_MN ? a_subs(rk) * (64 * GEMM_BK * 2) : L::A_BYTES) +
-                 (B_MN ? b_subs(rk) * (64 * GEMM_BK * 2) : L::B_BYTES);
+          return (A_MN ? a_subs(rk) * (64 * GEMM_BK * 2) : CUT ? (uint32_t)sh.am * GEMM_BK * 2 : L::A_BYTES) +
+                 (B_MN ? b_subs(rk) * (64 * GEMM_BK * 2) : CUT ? (uint32_t)bn * GEMM_BK * 2 : L::B_BYTES);
         };
         const int a_sub = a_subs(rank), b_sub = b_subs(rank);
-        const int a_row = mt * TILE_M + rank * GEMM_BM, b_row = nt * BN + rank * B_ROWS;
+        const int a_row = mt * TILE_M + rank * GEMM_BM, b_row = nt * bn + rank * B_ROWS;
         const uint32_t expect = PAIR ? stage_bytes(0) + stage_bytes(1) : stage_bytes(0);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
@@ -491,12 +496,12 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
         const bool scored = label >= 0 && label < sh.N && label != ep.ignore_index;
         float m = -INFINITY, s = 0.f;
 #pragma unroll 1
-        for (int c0 = cbeg; c0 < cend; c0 += 32) {
-          const int gn0 = nt * BN + c0;
+        for (int c0 = cbeg; c0 < min(cend, bn); c0 += 32) {
+          const int gn0 = nt * bn + c0, end = min(sh.N, nt * bn + bn);  // this chunk, and where the tile's columns end
+          if (gn0 >= end) break;
           uint32_t rr[32];
           tmem_ld32(t_row + c0, rr);
           tmem_wait_ld();
-          if (gn0 >= sh.N) continue;
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rr[j]);
@@ -504,11 +509,11 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = bf16_round(v[j]);
           }
-          if (gn0 + 32 > sh.N) {
+          if (gn0 + 32 > end) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = gn0 + j < sh.N ? v[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) v[j] = gn0 + j < end ? v[j] : -INFINITY;
           }
-          if (scored && label >= gn0 && label < gn0 + 32) {
+          if (scored && label >= gn0 && label < min(gn0 + 32, end)) {
             const int at = (int)label - gn0;
             float x = v[0];
 #pragma unroll
@@ -1036,7 +1041,17 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
                      (epi == RGPT_EPI_ACCUM_F32 && sh.num_kb >= 32));
   const int units_per_wave = pair ? nsm / 2 : nsm;
   sh.m_tiles = pair ? (M + 255) / 256 : m128;
-  sh.n_tiles = (N + BN - 1) / BN;
+  // One row tile's sums read B once and compute little: cut the tiles so that every SM gets as many rows of B, give or
+  // take 16, in as few rounds as 256-wide tiles take (16 x 50304 x 512: 2 rounds of 176 instead of 2 of 256 for a third
+  // of the SMs and 1 for the rest).
+  // Rows of A past M are not loaded either: what the tensor core makes of stale shared memory stays in their own rows.
+  sh.bn = BN;
+  sh.am = lsx && m128 == 1 ? (M + 7) / 8 * 8 : GEMM_BM;
+  if (lsx && m128 == 1 && BN == 256) {
+    const int rounds = ((N + 255) / 256 + nsm - 1) / nsm;
+    sh.bn = ((N + rounds * nsm - 1) / (rounds * nsm) + 15) / 16 * 16;
+  }
+  sh.n_tiles = (N + sh.bn - 1) / sh.bn;
   const int tiles = batch * sh.m_tiles * sh.n_tiles;
   if (splitk <= 0) {
     // Split K (accumulating epilogue only) to minimise waves x (k-blocks per unit + the
@@ -1074,12 +1089,12 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
   if (a_mn_major)
     st = make_tmap_3d(&ta, A, 2, M, K, batch, lda, a_bstride, 64, GEMM_BK);
   else
-    st = make_tmap_3d(&ta, A, 2, K, M, batch, lda, a_bstride, GEMM_BK, GEMM_BM);
+    st = make_tmap_3d(&ta, A, 2, K, M, batch, lda, a_bstride, GEMM_BK, sh.am);
   if (st) return st;
   if (b_mn_major)
     st = make_tmap_3d(&tb, B, 2, N, K, batch, ldb, b_bstride, 64, GEMM_BK);
   else
-    st = make_tmap_3d(&tb, B, 2, K, N, batch, ldb, b_bstride, GEMM_BK, pair ? BN / 2 : BN);
+    st = make_tmap_3d(&tb, B, 2, K, N, batch, ldb, b_bstride, GEMM_BK, pair ? BN / 2 : sh.bn);
   if (st) return st;
   // Output maps: one 32-row x 128-byte box per epilogue warp and chunk.
   const int ob = out_f32 ? 4 : 2;
@@ -1183,36 +1198,55 @@ extern "C" int rgpt_gemm_argmax(const void* A, long long lda, const void* B, lon
   return rgpt_check_launch("argmax_reduce_kernel");
 }
 
-// Joins the LSE_F32 GEMM's half column tiles: lane = row (32 rows a CTA, coalesced reads of part[tile][row]), the warps
-// share the tiles, and the CTA combines their (maximum, sum) pairs in a fixed order. On entry logps holds the scored
-// rows' label logits. lse and the log-probability are formed in fp64 and rounded once.
-__global__ void __launch_bounds__(1024) lse_reduce_kernel(const float2* __restrict__ part, int n_tiles, int M, int N,
-                                                          const long long* __restrict__ labels, long long ignore_index,
-                                                          float* logps, float* __restrict__ lse) {
+// Joins the LSE_F32 GEMM's half column tiles. ROWS = 32: a CTA takes 32 rows, first lane = row (coalesced reads of
+// part[tile][row]) with the warps sharing the tiles, then a warp joins the 32 (maximum, sum) pairs of a row. ROWS = 1,
+// for few rows: a CTA a row, its threads share the tiles. Always in a fixed order. On entry logps holds the scored rows'
+// label logits. lse and the log-probability are formed in fp64 and rounded once.
+__device__ __forceinline__ float2 lse_merge(float2 a, float2 b) {
+  const float nm = fmaxf(a.x, b.x), r = nm == -INFINITY ? 0.f : nm;
+  return make_float2(nm, a.y * ex2_approx((a.x - r) * 1.4426950408889634f) +
+                             b.y * ex2_approx((b.x - r) * 1.4426950408889634f));
+}
+__device__ __forceinline__ float2 lse_warp_merge(float2 s) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    s = lse_merge(s, make_float2(__shfl_xor_sync(0xffffffffu, s.x, o), __shfl_xor_sync(0xffffffffu, s.y, o)));
+  return s;
+}
+template <int ROWS>
+__global__ void __launch_bounds__(ROWS == 1 ? 256 : 1024) lse_reduce_kernel(
+    const float2* __restrict__ part, int n_tiles, int M, int N, const long long* __restrict__ labels,
+    long long ignore_index, float* logps, float* __restrict__ lse) {
+  constexpr int WARPS = ROWS == 1 ? 8 : 32, STEP = ROWS == 1 ? 256 : 32;
   griddep_wait();
   griddep_launch();
-  __shared__ float sm[32][33], ss[32][33];
+  __shared__ float2 sums[ROWS][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x * 32 + lane;
-  float m = -INFINITY, s = 0.f;
-  auto merge = [&](float om, float os) {
-    const float nm = fmaxf(m, om), r = nm == -INFINITY ? 0.f : nm;
-    s = s * ex2_approx((m - r) * 1.4426950408889634f) + os * ex2_approx((om - r) * 1.4426950408889634f);
-    m = nm;
-  };
-  if (row < M)
-    for (int t = warp; t < n_tiles; t += 32) {
-      const float2 p = part[(long long)t * M + row];
-      merge(p.x, p.y);
-    }
-  sm[warp][lane] = m;
-  ss[warp][lane] = s;
+  int row = ROWS == 1 ? (int)blockIdx.x : (int)blockIdx.x * 32 + lane;
+  const float2 none = make_float2(-INFINITY, 0.f);
+  float2 s = none;
+  for (int t0 = ROWS == 1 ? (int)threadIdx.x : warp; t0 < n_tiles; t0 += 4 * STEP) {  // four loads on their way
+    float2 p[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      p[k] = row < M && t0 + STEP * k < n_tiles ? part[(long long)(t0 + STEP * k) * M + row] : none;
+    s = lse_merge(s, lse_merge(lse_merge(p[0], p[1]), lse_merge(p[2], p[3])));
+  }
+  if constexpr (ROWS == 1) s = lse_warp_merge(s);
+  if (ROWS != 1 || lane == 0) sums[ROWS == 1 ? 0 : lane][warp] = s;
   __syncthreads();
-  if (warp != 0 || row >= M) return;
-  for (int w = 1; w < 32; ++w) merge(sm[w][lane], ss[w][lane]);
+  if constexpr (ROWS == 1) {
+    if (warp != 0) return;
+    s = lse_warp_merge(lane < WARPS ? sums[0][lane] : none);
+  } else {
+    row = blockIdx.x * 32 + warp;  // from here a warp a row
+    if (row >= M) return;
+    s = lse_warp_merge(sums[warp][lane]);
+  }
+  if (lane != 0) return;
   const long long label = labels[row];
   const bool scored = label >= 0 && label < N && label != ignore_index;
-  const double l = (double)m + log((double)s);
+  const double l = (double)s.x + log((double)s.y);
   logps[row] = scored ? (float)((double)logps[row] - l) : 0.f;
   if (lse) lse[row] = (float)l;
 }
@@ -1234,7 +1268,9 @@ extern "C" int rgpt_linear_logprobs(const void* X, long long ldx, const void* W,
   st = gemm_entry(X, 0, ldx, 0, W, 0, ldw, 0, M, V, K, 1, RGPT_EPI_LSE_F32, 0, 1.0f, 0.0f, nullptr, 0, 0, nullptr, 0, 0,
                   nullptr, 0, 0, nullptr, 1, nullptr, nullptr, stream, nullptr, &a);
   if (st) return st;
-  launch_pdl(lse_reduce_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, reinterpret_cast<cudaStream_t>(stream), 1,
+  const bool few = M <= 512;
+  launch_pdl(few ? lse_reduce_kernel<1> : lse_reduce_kernel<32>, dim3((unsigned)(few ? M : (M + 31) / 32)),
+             dim3(few ? 256 : 1024), 0, reinterpret_cast<cudaStream_t>(stream), 1,
              (const float2*)part, a.n_tiles * (gemm_epi_warps(RGPT_EPI_LSE_F32) / 4), M, V, labels, ignore_index, logps, lse);
   return rgpt_check_launch("lse_reduce_kernel");
 }
