@@ -76,13 +76,15 @@ struct EpiParams {
   // LSE_F32 / SOFTMAX_GRAD_BF16: each row's label (scored when in [0, N) and not ignore_index)
   const long long* labels;
   long long ignore_index;
-  float2* lse_part;        // LSE_F32: [half column tile][M] (maximum, sum of e^{v - maximum}) of its columns
+  float2* lse_part;        // LSE_F32: [half column tile][M] (M, sum of 2^{c v - M}), M = ceil(c max), c = log2 e, of its columns
   float* label_logit;      // LSE_F32: [M], the label's value, written for scored rows only
   int round_bf16;          // LSE_F32: the values are rounded to bf16 first (what a stored bf16 product would hold)
   const float* row_lse;    // SOFTMAX_GRAD_BF16: [M]
   const float* row_coef;   // SOFTMAX_GRAD_BF16: [M]
 };
 
+constexpr float LSE_LOG2E = 1.4426950408889634f;
+constexpr float LSE_LOG2E_LO = (float)(1.4426950408889634 - (double)LSE_LOG2E);
 constexpr int GEMM_BM = 128;
 constexpr int GEMM_BK = 64;
 // Epilogue warps per CTA (EW): 4 = one per TMEM lane quadrant; 8 = two per quadrant, each taking half
@@ -525,16 +527,19 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
 #pragma unroll
           for (int j = 1; j + 1 < 32; j += 2) cm = fmax3(cm, v[j], v[j + 1]);
           cm = fmaxf(cm, v[31]);
-          const float nm = fmaxf(m, cm);
-          const float r = nm == -INFINITY ? 0.f : nm;  // only -inf so far: e^{-inf - 0} = 0, not a NaN
-          s *= ex2_approx((m - r) * 1.4426950408889634f);
+          // base 2 and a whole reference, so that rescaling is exact (as in the row kernels)
+          const float nm = fmaxf(m, ceilf(cm * LSE_LOG2E));
+          const float r = nm == -INFINITY ? 0.f : nm;  // only -inf so far: 2^{-inf - 0} = 0, not a NaN
+          s *= ex2_approx(m - r);
           m = nm;
-          const float2 nr = make_float2(-r, -r), l2e = make_float2(1.4426950408889634f, 1.4426950408889634f);
+          const float2 nr = make_float2(-r, -r), l2e = make_float2(LSE_LOG2E, LSE_LOG2E);
+          const float2 lo = make_float2(LSE_LOG2E_LO, LSE_LOG2E_LO);
           float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            const float2 t0 = fmul2(fadd2(make_float2(v[j], v[j + 1]), nr), l2e);
-            const float2 t1 = fmul2(fadd2(make_float2(v[j + 2], v[j + 3]), nr), l2e);
+            const float2 v0 = make_float2(v[j], v[j + 1]), v1 = make_float2(v[j + 2], v[j + 3]);
+            const float2 t0 = ffma2(v0, lo, ffma2(v0, l2e, nr));
+            const float2 t1 = ffma2(v1, lo, ffma2(v1, l2e, nr));
             a0 = fadd2(a0, make_float2(ex2_approx(t0.x), ex2_approx(t0.y)));
             a1 = fadd2(a1, make_float2(ex2_approx(t1.x), ex2_approx(t1.y)));
           }
@@ -1204,8 +1209,7 @@ extern "C" int rgpt_gemm_argmax(const void* A, long long lda, const void* B, lon
 // label logits. lse and the log-probability are formed in fp64 and rounded once.
 __device__ __forceinline__ float2 lse_merge(float2 a, float2 b) {
   const float nm = fmaxf(a.x, b.x), r = nm == -INFINITY ? 0.f : nm;
-  return make_float2(nm, a.y * ex2_approx((a.x - r) * 1.4426950408889634f) +
-                             b.y * ex2_approx((b.x - r) * 1.4426950408889634f));
+  return make_float2(nm, a.y * ex2_approx(a.x - r) + b.y * ex2_approx(b.x - r));
 }
 __device__ __forceinline__ float2 lse_warp_merge(float2 s) {
 #pragma unroll
@@ -1246,7 +1250,8 @@ __global__ void __launch_bounds__(ROWS == 1 ? 256 : 1024) lse_reduce_kernel(
   if (lane != 0) return;
   const long long label = labels[row];
   const bool scored = label >= 0 && label < N && label != ignore_index;
-  const double l = (double)s.x + log((double)s.y);
+  // ln 2 (M + log2 s), less the hardware exponential's mean relative error (-5.25e-8, measured)
+  const double l = 0.69314718055994530942 * (double)s.x + log((double)s.y) + 5.25e-8;
   logps[row] = scored ? (float)((double)logps[row] - l) : 0.f;
   if (lse) lse[row] = (float)l;
 }

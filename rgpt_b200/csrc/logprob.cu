@@ -22,6 +22,8 @@
 namespace rgpt {
 
 constexpr float LP_LOG2E = 1.4426950408889634f;
+constexpr double LP_EX2_MEAN = -5.25e-8;  // of ex2.approx.ftz.f32 over [-16, 0], measured on sm_100a
+constexpr float LP_LOG2E_LO = (float)(1.4426950408889634 - (double)LP_LOG2E);  // what fp32 leaves of it, 1.9e-8
 constexpr int LP_THREADS = 256;
 // A stored lse carries 2^-24 |lse| of rounding into every probability of the backward: 4e-6 at this size, less than a
 // sum of exponentials has of its own. Rows beyond it (a row of the type's lowest values, say) are summed again.
@@ -156,9 +158,11 @@ __device__ __forceinline__ bool lp_scored(long long label, long long ignore_inde
 // The reference point of an exponent: -inf (nothing seen yet) is replaced by 0, so that e^{-inf - 0} = 0.
 __device__ __forceinline__ float lp_ref(float m) { return m == -INFINITY ? 0.f : m; }
 
-// A running (M, sum of 2^{c x - M}) in base 2, c = fp32(log2 e): one fused multiply-add and one exponential an
-// element. M = fp32(c max) is the reference itself, so its rounding leaves no error; c's own (c ln 2 = 1 - 1.3e-8) is
-// corrected to first order at the end. Elements up to LP_LOW, where c x overflows, count as nothing (M = -inf). A row
+// A running (M, sum of 2^{c x - M}) in base 2, c = log2 e in two parts: two fused multiply-adds and one exponential an
+// element. What is the same for every row would add up over a long sequence, so it is kept small: c's first part alone
+// makes log-probabilities some 6e-8 too high; M = ceil(c max) is a whole number, so that rescaling a sum is exact (with
+// any other M the hardware exponential's mean relative error, -5.25e-8 over a binade, comes in at each rescaling: 2e-7
+// in all); and that error of the elements themselves is taken off the row's sum at the end. Elements up to LP_LOW, where c x overflows, count as nothing (M = -inf). A row
 // that holds nothing else, or whose |M| is so large that c max - M may be (beyond LP_WIDE its 2^-24 |M| is no longer
 // small), takes lp_row_sum's careful pass: e^{x - max} after the subtraction.
 struct LpSum {
@@ -174,10 +178,10 @@ struct LpSum {
     float lm = L::max8(u[0]);
 #pragma unroll
     for (int k = 1; k < U; ++k) lm = fmaxf(lm, L::max8(u[k]));
-    const float nm = fmaxf(m, lm > LP_LOW ? lm * LP_LOG2E : -INFINITY), r = lp_ref(nm);
+    const float nm = fmaxf(m, lm > LP_LOW ? ceilf(lm * LP_LOG2E) : -INFINITY), r = lp_ref(nm);
     s *= ex2_approx(m - r);
     m = nm;
-    const F2 nr = f2(-r, -r), l2e = f2(LP_LOG2E, LP_LOG2E);
+    const F2 nr = f2(-r, -r), l2e = f2(LP_LOG2E, LP_LOG2E), lo = f2(LP_LOG2E_LO, LP_LOG2E_LO);
     F2 a0 = f2(s, 0.f), a1 = f2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -185,16 +189,16 @@ struct LpSum {
       L::unpack(u[k], f);
 #pragma unroll
       for (int j = 0; j < L::VEC / 2; j += 2) {
-        a0 = f2_add(a0, f2_ex2(f2_fma(f[j], l2e, nr)));
-        a1 = f2_add(a1, f2_ex2(f2_fma(f[j + 1], l2e, nr)));
+        a0 = f2_add(a0, f2_ex2(f2_fma(f[j], lo, f2_fma(f[j], l2e, nr))));
+        a1 = f2_add(a1, f2_ex2(f2_fma(f[j + 1], lo, f2_fma(f[j + 1], l2e, nr))));
       }
     }
     const float2 b = f2_get(f2_add(a0, a1));
     s = b.x + b.y;
   }
   __device__ __forceinline__ void add(float f) {
-    const float nm = fmaxf(m, f > LP_LOW ? f * LP_LOG2E : -INFINITY), r = lp_ref(nm);
-    s = s * ex2_approx(m - r) + ex2_approx(fmaf(f, LP_LOG2E, -r));
+    const float nm = fmaxf(m, f > LP_LOW ? ceilf(f * LP_LOG2E) : -INFINITY), r = lp_ref(nm);
+    s = s * ex2_approx(m - r) + ex2_approx(fmaf(f, LP_LOG2E_LO, fmaf(f, LP_LOG2E, -r)));
     m = nm;
   }
 };
@@ -260,13 +264,12 @@ __device__ __forceinline__ float2 lp_join(float2 a, LpShare sh, MERGE&& merge) {
 
 // The finished row from its joined (M, s).
 __device__ __forceinline__ LpRow lp_finish(float2 r) {
-  // lse = ln2 (M + log2 s) + (1 - c ln2) M / c; log(s) from the mantissa in [0.75, 1.5) in fp32 (absolute error 2^-25)
-  // and the exponent in fp64
-  constexpr double C = (double)LP_LOG2E, LN2 = 0.69314718055994530942;
+  // lse = ln2 (M + log2 s); log(s) from the mantissa in [0.75, 1.5) in fp32 (absolute error 2^-25) and the exponent in fp64
+  constexpr double LN2 = 0.69314718055994530942;
   const int e = (int)((__float_as_uint(r.y) - 0x3F400000u) & 0xFF800000u) >> 23;
   const float f = __uint_as_float(__float_as_uint(r.y) - ((uint32_t)e << 23));
   const double M = (double)r.x;
-  return LpRow{0.f, r.x, 1.f / r.y, fma(M, LN2 + (1.0 - C * LN2) / C, fma((double)e, LN2, (double)logf(f)))};
+  return LpRow{0.f, r.x, 1.f / r.y, fma(M + (double)e, LN2, (double)logf(f) - LP_EX2_MEAN)};
 }
 __device__ __forceinline__ bool lp_plain(float2 r) {
   return fabsf(r.x) <= LP_WIDE && r.y < INFINITY;  // a NaN in the row makes the sum NaN
@@ -629,41 +632,46 @@ __device__ __forceinline__ void pref_terms(const PrefArgs& a, double h, double* 
 }
 
 // One CTA per pair: the two sequences' log-probabilities in fp64, the margin h and the sequences' coefficients
-// d loss / d (a scored token's log-probability).
+// d loss / d (a scored token's log-probability). A single CTA takes all pairs when they are few and short, and their
+// mean, which saves a launch.
 __global__ void __launch_bounds__(256) pref_pair_kernel(const double* __restrict__ logps,
                                                         const long long* __restrict__ labels, long long ignore_index,
                                                         int V, int P, int T, const float* __restrict__ ref, PrefArgs a,
                                                         float* __restrict__ seq_logps, float* __restrict__ margins,
-                                                        float* __restrict__ coef) {
+                                                        float* __restrict__ coef, float* __restrict__ loss_out) {
   griddep_wait();
   griddep_launch();
   __shared__ double red[8];
-  const int p = blockIdx.x;
-  double s[2], n[2];
+  double mean = 0.0;
+  for (int p = blockIdx.x; p < P; p += gridDim.x) {
+    double s[2], n[2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const long long base = (long long)(p + k * P) * T;
-    double v = 0.0, c = 0.0;
-    for (int t = threadIdx.x; t < T; t += blockDim.x) {
-      v += logps[base + t];
-      if (a.average) c += lp_scored(labels[base + t], ignore_index, V) ? 1.0 : 0.0;
+    for (int k = 0; k < 2; ++k) {
+      const long long base = (long long)(p + k * P) * T;
+      double v = 0.0, c = 0.0;
+      for (int t = threadIdx.x; t < T; t += blockDim.x) {
+        v += logps[base + t];
+        if (a.average) c += lp_scored(labels[base + t], ignore_index, V) ? 1.0 : 0.0;
+      }
+      s[k] = lp_block_sum(v, red);
+      n[k] = a.average ? fmax(lp_block_sum(c, red), 1.0) : 1.0;
+      s[k] /= n[k];
     }
-    s[k] = lp_block_sum(v, red);
-    n[k] = a.average ? fmax(lp_block_sum(c, red), 1.0) : 1.0;
-    s[k] /= n[k];
+    if (threadIdx.x != 0) continue;
+    double d = s[0] - s[1];
+    if (ref) d = (s[0] - (double)ref[p]) - (s[1] - (double)ref[p + P]);
+    const double h = (double)a.beta * d - (double)a.margin;
+    double loss, dh;
+    pref_terms(a, h, &loss, &dh);
+    dh *= (double)a.beta * (double)a.grad_scale / P;
+    seq_logps[p] = (float)s[0];
+    seq_logps[p + P] = (float)s[1];
+    margins[p] = (float)h;
+    coef[p] = (float)(dh / n[0]);
+    coef[p + P] = (float)(-dh / n[1]);
+    mean += loss;
   }
-  if (threadIdx.x != 0) return;
-  double d = s[0] - s[1];
-  if (ref) d = (s[0] - (double)ref[p]) - (s[1] - (double)ref[p + P]);
-  const double h = (double)a.beta * d - (double)a.margin;
-  double loss, dh;
-  pref_terms(a, h, &loss, &dh);
-  dh *= (double)a.beta * (double)a.grad_scale / P;
-  seq_logps[p] = (float)s[0];
-  seq_logps[p + P] = (float)s[1];
-  margins[p] = (float)h;
-  coef[p] = (float)(dh / n[0]);
-  coef[p + P] = (float)(-dh / n[1]);
+  if (gridDim.x == 1 && threadIdx.x == 0) loss_out[0] = (float)(mean / P);
 }
 
 // mean of the pairs' losses, from their margins
@@ -1029,9 +1037,10 @@ extern "C" int rgpt_preference_loss(const void* logits, int dtype, long long sb,
   const long long M = 2ll * P * T;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if ((rc = launch_logp_fwd(logits, dtype, lr, M, V, labels, ignore_index, token_logps, lse, scratch, s))) return rc;
-  launch_pdl(pref_pair_kernel, dim3(P), dim3(256), 0, s, 1, (const double*)scratch, labels, ignore_index, V, P, T, ref_logps, a,
-             seq_logps, margins, coef);
-  launch_pdl(pref_loss_kernel, dim3(1), dim3(256), 0, s, 1, margins, P, a, loss);
+  const unsigned pair_ctas = (long long)P * T <= 512 ? 1u : (unsigned)P;
+  launch_pdl(pref_pair_kernel, dim3(pair_ctas), dim3(256), 0, s, 1, (const double*)scratch, labels, ignore_index, V, P, T,
+             ref_logps, a, seq_logps, margins, coef, loss);
+  if (pair_ctas > 1) launch_pdl(pref_loss_kernel, dim3(1), dim3(256), 0, s, 1, margins, P, a, loss);
   if (dlogits &&
       (rc = launch_logp_bwd(logits, dtype, lr, M, V, labels, ignore_index, lse, coef, 1, dlogits, LpRows{db, dt, T}, s)))
     return rc;

@@ -501,7 +501,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     _call_on(dev, "rgpt_preference_loss", logits.data_ptr(), dt, sb, st, P, T, V, lab, int(ignore_index), ref,
              PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
              float(grad_scale), *outs, scratch.data_ptr(), *grad,
-             kernels=3 + (dlogits is not None))
+             kernels=2 + (B * T > 1024 and B > 2) + (dlogits is not None))
 
 
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
