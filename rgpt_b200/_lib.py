@@ -173,11 +173,6 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def raw_stream(index: int) -> int:
-    """stream_ptr of device `index`, without making a Stream object."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
 def ptr(t: torch.Tensor | None) -> int | None:
     if t is None:
         return None

@@ -1252,7 +1252,8 @@ __global__ void __launch_bounds__(ROWS == 1 ? 256 : 1024) lse_reduce_kernel(
   const bool scored = label >= 0 && label < N && label != ignore_index;
   // ln 2 (M + log2 s), less the hardware exponential's mean relative error (-5.25e-8, measured)
   const double l = 0.69314718055994530942 * (double)s.x + log((double)s.y) + 5.25e-8;
-  logps[row] = scored ? (float)((double)logps[row] - l) : 0.f;
+  const double lp = scored ? (double)logps[row] - l : 0.0;
+  logps[row] = lp > 0.0 ? 0.f : (float)lp;  // rounding may not make a sure label more than sure
   if (lse) lse[row] = (float)l;
 }
 

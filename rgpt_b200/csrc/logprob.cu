@@ -271,6 +271,11 @@ __device__ __forceinline__ LpRow lp_finish(float2 r) {
   const double M = (double)r.x;
   return LpRow{0.f, r.x, 1.f / r.y, fma(M + (double)e, LN2, (double)logf(f) - LP_EX2_MEAN)};
 }
+// The label's log-probability; rounding may not make a sure label more than sure.
+__device__ __forceinline__ double lp_label(float xl, const LpRow& r) {
+  const double lp = (double)xl - r.lse;
+  return lp > 0.0 ? 0.0 : lp;
+}
 __device__ __forceinline__ bool lp_plain(float2 r) {
   return fabsf(r.x) <= LP_WIDE && r.y < INFINITY;  // a NaN in the row makes the sum NaN
 }
@@ -394,24 +399,25 @@ __device__ __forceinline__ void lp_write_zero(E* d, int V, LpShare sh) {
 }
 
 // ---------------------------------------------------------------------------- rows through shared memory
-// This CTA's share of a row's vectors, brought in by bulk copies of VECS each, in order, into `slots` places
-// that are used again once every thread is done with them.
-// Waits are bounded; after one has run out (the device error word says so) the rest is not waited for again.
+// This CTA's share of a row's vectors, brought in by bulk copies of VECS each, in order, into `slots` places that are
+// used again once every thread is done with them. Waits are bounded: after one has run out (the device error word says
+// so) nothing more is issued or waited for, but for what is still on its way at the end.
 template <int VECS>
 struct LpStage {
   const uint4* src;
   uint4* place;
   uint64_t* full;
-  int n, pieces, slots;
+  int n, pieces, slots, issued;
   bool ok;
   __device__ __forceinline__ LpStage(const uint4* src_, int n_, void* smem, uint64_t* full_, int slots_)
-      : src(src_), place(reinterpret_cast<uint4*>(smem)), full(full_), n(n_),
-        pieces((n_ + VECS - 1) / VECS), slots(slots_), ok(true) {}
+      : src(src_), place(reinterpret_cast<uint4*>(smem)), full(full_), n(n_), pieces((n_ + VECS - 1) / VECS),
+        slots(slots_), issued(0), ok(true) {}
   __device__ __forceinline__ int size(int c) const { return min(VECS, n - c * VECS); }
-  __device__ __forceinline__ void issue(int c) {  // one thread
+  __device__ __forceinline__ void issue(int c) {  // thread 0
     const uint32_t bytes = 16u * (uint32_t)size(c);
     mbar_arrive_expect_tx(&full[c % slots], bytes);
     bulk_load_1d(place + (c % slots) * VECS, src + (long long)c * VECS, bytes, &full[c % slots]);
+    issued = c + 1;
   }
   // all threads, first
   __device__ __forceinline__ void start() {
@@ -423,14 +429,18 @@ struct LpStage {
     __syncthreads();
   }
   __device__ __forceinline__ const uint4* wait(int c) {
-    if (ok) ok = mbar_wait(&full[c % slots], (uint32_t)(c / slots) & 1u, nullptr);
+    if (ok && !mbar_wait(&full[c % slots], (uint32_t)(c / slots) & 1u, nullptr)) {
+      ok = false;
+      if (threadIdx.x == 0)  // the copies on their way must land before the CTA's shared memory is given up
+        for (int i = c; i < issued; ++i) mbar_wait(&full[i % slots], (uint32_t)(i / slots) & 1u, nullptr);
+    }
     return place + (c % slots) * VECS;
   }
   // all threads, after their reads of piece c
   __device__ __forceinline__ void next(int c) {
     if (c + slots >= pieces) return;
     __syncthreads();
-    if (threadIdx.x == 0) issue(c + slots);
+    if (threadIdx.x == 0 && ok) issue(c + slots);
   }
 };
 
@@ -513,7 +523,7 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
   LpRow r;
   lp_staged_sum<E, CL, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r, [] {});
   if (first) {
-    const double lp = (double)xl - r.lse;
+    const double lp = lp_label(xl, r);
     logps[row] = (float)lp;
     if (lse) lse[row] = (float)r.lse;
     if (wide) wide[row] = lp;
@@ -543,7 +553,7 @@ __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restric
   const E* x = logits + lr.offset(row);
   const LpRow r = lp_row_sum<E, CL>(x, V, sh);
   if (first) {
-    const double lp = (double)LpType<E>::get(x[label]) - r.lse;
+    const double lp = lp_label(LpType<E>::get(x[label]), r);
     logps[row] = (float)lp;
     if (lse) lse[row] = (float)r.lse;
     if (wide) wide[row] = lp;
@@ -758,7 +768,7 @@ struct PolicyRows {
 // What thread 0 does with a row's sum: the token's terms, the outputs, and the row's coefficient for the CTA.
 __device__ __forceinline__ float policy_row(const PolicyRows& p, LpRows lr, long long row, float xl, const LpRow& r,
                                             int n, int total, bool first) {
-  const double lp = (double)xl - r.lse;
+  const double lp = lp_label(xl, r);
   const unsigned b = lr.batch(row);
   const PolicyTerms t = policy_terms(p.a, lp, p.old[row], p.ref != nullptr, p.ref ? p.ref[row] : 0.f,
                                      p.adv[p.a.adv_per_token ? row : b]);
@@ -920,9 +930,9 @@ static int lp_check(const char* what, const void* logits, int dtype, long long B
   if (st) return st;
   if (dtype < RGPT_DTYPE_BF16 || dtype > RGPT_DTYPE_F32)
     return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "%s: unknown logits type %d", what, dtype);
-  if (B < 1 || T < 1 || V < 1 || B * T > 0x7fffffffll)
-    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "%s needs 1 <= B * T < 2^31 rows and V >= 1 (got B=%lld T=%lld V=%d)", what,
-                          B, T, V);
+  if (B < 1 || T < 1 || V < 1 || V > (1 << 30) || B * T > 0x7fffffffll)
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "%s needs 1 <= B * T < 2^31 rows and 1 <= V <= 2^30 (got B=%lld T=%lld V=%d)",
+                          what, B, T, V);
   if (logits == nullptr || labels == nullptr) return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "%s: null pointer", what);
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == RGPT_DTYPE_F32 ? 4 : 2) != 0)
     return rgpt_set_error(RGPT_ERR_MISALIGNED, "%s: logits are not aligned to their type", what);

@@ -359,28 +359,38 @@ LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 
-def _call_on(index: int, name: str, *args, kernels: int | None = None) -> None:
+_entries: dict = {}  # bound entry points by name
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call_on(index: int, name: str, *args, kernels: int = 1) -> None:
     """_lib.call on the current stream of device `index`, with that device current (the library launches on the current
     device's context). The stream is the call's last argument."""
     if index < 0:
         raise RuntimeError("librgpt_kernels only takes CUDA tensors (no CPU path)")
-    if index == torch._C._cuda_getDevice():
-        _lib.call(name, *args, _lib.raw_stream(index), kernels=kernels)
-    else:
+    if index != _current_device():
         with torch.cuda.device(index):
-            _lib.call(name, *args, _lib.raw_stream(index), kernels=kernels)
+            return _call_on(index, name, *args, kernels=kernels)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    rc = fn(*args, _current_stream(index))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (status {rc}): {_lib.last_error()}")
+    _lib.launch_count += kernels
 
 
 def _flat(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int) -> int:
     """Address of a contiguous tensor of the given shape, type and device (-1: host memory, which _call_on refuses)."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}"
-                         f" with strides {t.stride()}")
     if t.get_device() != index:
         raise ValueError(f"{name} is on {t.device}, expected device {index}")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}"
+                     f" with strides {t.stride()}")
 
 
 def _opt(t: torch.Tensor | None, name: str, shape, dtype: torch.dtype, index: int) -> int | None:
@@ -403,17 +413,17 @@ def _logit_rows(t: torch.Tensor, name: str):
         raise ValueError(f"{name} must be [M, V] or [B, T, V], got {tuple(shape)}")
     if V > 1 and sv != 1:
         raise ValueError(f"{name} must have unit stride along the vocabulary, got strides {stride}")
-    if B * T >= 2 ** 31 or V >= 2 ** 31:
-        raise ValueError(f"{name} must have fewer than 2^31 rows and columns, got {tuple(shape)}")
+    if B * T >= 2 ** 31 or V > 2 ** 30:
+        raise ValueError(f"{name} must have fewer than 2^31 rows and at most 2^30 columns, got {tuple(shape)}")
     return dt, sb, st, B, T, V
 
 
-def _span(t: torch.Tensor):
-    """[first, last) address of a tensor's elements."""
-    at, last = t.data_ptr(), 1
+def _end(t: torch.Tensor) -> int:
+    """The address behind a tensor's last element."""
+    last = 1
     for n, s in zip(t.shape, t.stride()):
         last += (n - 1) * s
-    return at, at + last * t.element_size()
+    return t.data_ptr() + last * t.element_size()
 
 
 def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):
@@ -423,15 +433,15 @@ def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):
     if dlogits.dtype is not logits.dtype or dlogits.shape != logits.shape or dlogits.get_device() != logits.get_device():
         raise ValueError("dlogits must have the logits' type, shape and device")
     _, sb, st, B, T, V = _logit_rows(dlogits, "dlogits")
-    if not dlogits.is_contiguous():
-        tokens = T == 1 or st >= V
-        if not (tokens and (B == 1 or sb >= (T - 1) * st + V)) and not (sb >= V and st >= (B - 1) * sb + V):
+    at, of = dlogits.data_ptr(), logits.data_ptr()
+    if dlogits.is_contiguous():
+        end = at + B * T * V * dlogits.element_size()
+    else:
+        if not ((T == 1 or st >= V) and (B == 1 or sb >= (T - 1) * st + V)) and not (sb >= V and st >= (B - 1) * sb + V):
             raise ValueError(f"the rows of dlogits overlap (strides {dlogits.stride()})")
-    at = dlogits.data_ptr()
-    if at != logits.data_ptr() or dlogits.stride() != logits.stride():
-        (a, b), (c, d) = _span(logits), _span(dlogits)
-        if a < d and c < b:
-            raise ValueError("dlogits must be the logits themselves or share no memory with them")
+        end = _end(dlogits)
+    if (at != of or dlogits.stride() != logits.stride()) and at < _end(logits) and of < end:
+        raise ValueError("dlogits must be the logits themselves or share no memory with them")
     return at, sb, st
 
 
@@ -601,6 +611,8 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
         if dw is not None and dw.dtype == torch.bfloat16:
             dw.zero_()
         return
+    if not x.is_cuda:
+        raise RuntimeError("librgpt_kernels only takes CUDA tensors (no CPU path)")
     ld = (V + 7) // 8 * 8
     rows = min(M, chunk_rows or max(256, LINEAR_CHUNK_ELEMS // ld // 256 * 256))
     with torch.cuda.device(dev):

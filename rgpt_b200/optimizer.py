@@ -598,8 +598,7 @@ class Muon(torch.optim.Optimizer):
         own tensors with 32 bits, new ones decoded from their codes with 8."""
         st = self.state.get(p, {})
         if "exp_avg_q8" in st:
-            both = torch.empty((2,) + p.shape, device=p.device, dtype=torch.float32)
-            m, v = both[0], both[1]
+            m, v = torch.empty((2,) + p.shape, device=p.device, dtype=torch.float32).unbind()
             nv.adamw8_moments(st["exp_avg_q8"], st["exp_avg_scale"], st["exp_avg_sq_q8"], st["exp_avg_sq_scale"], m, v)
             return m, v
         if "exp_avg" not in st:
