@@ -381,6 +381,16 @@ def _call_on(index: int, name: str, *args, kernels: int = 1) -> None:
     _lib.launch_count += kernels
 
 
+# The operators below check their arguments twice over: _fastargs.pack (csrc/fastargs.cpp) in one step, giving the
+# entry point's arguments when all is well, and otherwise here, where a refusal says what was wrong. (Where only the
+# kernel library has been built, the checks here serve alone.)
+try:
+    from ._fastargs import pack as _pack
+except ImportError:
+    def _pack(kinds: str, tensors: tuple):
+        return None
+
+
 def _flat(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int) -> int:
     """Address of a contiguous tensor of the given shape, type and device (-1: host memory, which _call_on refuses)."""
     if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
@@ -450,6 +460,9 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, logps: torch.Tens
     """logps = log softmax(logits)[label], 0 for tokens that are not scored (label ignore_index or outside the
     vocabulary); lse (optional, for token_logprobs_bwd) = logsumexp. logits [M, V] or [B, T, V] in bf16, fp16 or fp32
     with unit stride along the vocabulary and any other strides; labels int64, logps and lse fp32 of the leading shape."""
+    p = _pack("LyfF", (logits, labels, logps, lse))
+    if p is not None:
+        return _call_on(p[10], "rgpt_token_logprobs", *p[:8], int(ignore_index), p[8], p[9])
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     dev, shape = logits.get_device(), logits.shape[:-1]
     args = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
@@ -465,6 +478,9 @@ def token_logprobs_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Te
                        dlogits: torch.Tensor, *, ignore_index: int = -100) -> None:
     """dlogits = dlogps * (onehot(label) - softmax(logits)), zero rows for tokens that are not scored. dlogits: the
     logits themselves (overwritten) or another tensor of their type and shape."""
+    p = _pack("LyffG", (logits, labels, lse, dlogps, dlogits))
+    if p is not None and dlogits is not None:
+        return _call_on(p[13], "rgpt_token_logprobs_bwd", *p[:8], int(ignore_index), *p[8:13])
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     dev, shape = logits.get_device(), logits.shape[:-1]
     args = (_flat(labels, "labels", shape, torch.int64, dev), int(ignore_index),
@@ -495,6 +511,13 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError("preference_loss: label_smoothing must be in [0, 0.5], and 0 unless kind is 'sigmoid'")
     if not 0.0 < beta < float("inf"):
         raise ValueError(f"preference_loss: beta must be positive and finite, got {beta}")
+    p = _pack("LyRffbhb1WG", (logits, labels, ref_logps, token_logps, lse, seq_logps, margins, coef, loss, scratch,
+                              dlogits))
+    if p is not None and logits.dim() == 3:
+        pairs, T = p[4] // 2, p[5]
+        return _call_on(p[19], "rgpt_preference_loss", *p[:4], pairs, *p[5:8], int(ignore_index), p[8],
+                        PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
+                        float(grad_scale), *p[9:19], kernels=2 + (pairs * T > 512) + (dlogits is not None))
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     if logits.dim() != 3 or B % 2 or B == 0 or T == 0 or V == 0:
         raise ValueError(f"preference_loss needs logits [2P, T, V] of at least one pair and token, got {tuple(logits.shape)}")
@@ -505,13 +528,13 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
             _flat(seq_logps, "seq_logps", (B,), f32, dev), _flat(margins, "margins", (P,), f32, dev),
             _flat(coef, "coef", (B,), f32, dev), _flat(loss, "loss", (1,), f32, dev))
     grad = _grad_rows(dlogits, logits)
-    _opt(scratch, "scratch", (B, T), torch.float64, dev)
     if scratch is None:
         scratch = torch.empty(B, T, device=logits.device, dtype=torch.float64)
+    _flat(scratch, "scratch", (B, T), torch.float64, dev)
     _call_on(dev, "rgpt_preference_loss", logits.data_ptr(), dt, sb, st, P, T, V, lab, int(ignore_index), ref,
              PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
              float(grad_scale), *outs, scratch.data_ptr(), *grad,
-             kernels=2 + (B * T > 1024 and B > 2) + (dlogits is not None))
+             kernels=2 + (P * T > 512) + (dlogits is not None))
 
 
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
@@ -531,6 +554,12 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
         raise ValueError(f"policy_loss: clip_low must be in [0, 1] and clip_high >= 0, got {clip_low} and {clip_high}")
     if kl_coef != 0.0 and ref_logps is None:
         raise ValueError("policy_loss: kl_coef needs ref_logps")
+    p = _pack("LyfFafc4FFG", (logits, labels, old_logps, ref_logps, advantages, token_logps, counts, stats, lse, coef,
+                              dlogits))
+    if p is not None:
+        return _call_on(p[20], "rgpt_policy_loss", *p[:8], int(ignore_index), *p[8:12], float(clip_low),
+                        float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *p[12:20],
+                        kernels=2 + (p[4] * p[5] > 2048))
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     dev, shape, f32 = logits.get_device(), logits.shape[:-1], torch.float32
     per_token = advantages.shape != (B,)
@@ -570,6 +599,10 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
     lse [M] (optional, for linear_logprobs_bwd) is written for every row. round_bf16: the products are rounded to bf16
     first, which gives what token_logprobs gives on stored bf16 logits. part: fp32 scratch of at least
     4 * M * ceil(V/128) elements (allocated when None)."""
+    p = _pack("XXyPfF", (x, w, labels, part, logps, lse))
+    if p is not None:
+        return _call_on(p[9], "rgpt_linear_logprobs", *p[:4], *x.shape[:1], *w.shape, p[4], int(ignore_index),
+                        int(bool(round_bf16)), *p[5:9], kernels=2)
     M, V, K = _linear_operands(x, w)
     dev = x.get_device()
     need = 4 * M * ((V + 127) // 128)
@@ -664,6 +697,9 @@ def adamw8(table: torch.Tensor, chunk_tensor: torch.Tensor, chunk_start: torch.T
 def adamw8_moments(mq: torch.Tensor, m_scale: torch.Tensor, vq: torch.Tensor, v_scale: torch.Tensor, m: torch.Tensor,
                    v: torch.Tensor) -> None:
     """m, v (fp32) = the moments that 8-bit codes and their scales stand for."""
+    p = _pack("ususmm", (mq, m_scale, vq, v_scale, m, v))
+    if p is not None:
+        return _call_on(p[6], "rgpt_adamw8_moments", *p[:6], mq.shape[0])
     n, dev, f32 = m.numel(), m.get_device(), torch.float32
     blocks = (n + ADAM8_BLOCK - 1) // ADAM8_BLOCK
     _call_on(dev, "rgpt_adamw8_moments", _flat(mq, "m codes", (n,), torch.uint8, dev), _flat(m_scale, "m scales", (blocks,), f32, dev),
