@@ -217,21 +217,34 @@ __device__ __forceinline__ int lp_head(const E* x, int V) {
   return h < V ? h : V;
 }
 
-// A row is shared by the C CTAs of a cluster (C = 1: no cluster): CTA `part` takes its share of the row's 16-byte
-// vectors and of the elements that lie outside them. Several CTAs a row only when there are too few rows for the SMs.
+// Who works on a row: one CTA; the CTAs of a cluster, when there are too few rows for the SMs; or one warp, when rows
+// are short. CTA `part` of a cluster takes its share of the row's 16-byte vectors and of the elements outside them.
+enum LpTeam { LP_CTA = 0, LP_CLUSTER = 1, LP_WARP = 2 };
 struct LpShare {
   int part, parts;
   __device__ __forceinline__ int lo(int n) const { return (int)((long long)n * part / parts); }
   __device__ __forceinline__ int hi(int n) const { return (int)((long long)n * (part + 1) / parts); }
 };
-template <bool CL>
+template <int W>
 __device__ __forceinline__ LpShare lp_share() {
   LpShare s = {0, 1};
-  if constexpr (CL) {
+  if constexpr (W == LP_CLUSTER) {
     s.part = (int)cluster_ctarank();
     s.parts = (int)cluster_nctarank();
   }
   return s;
+}
+template <int W>
+__device__ __forceinline__ int lp_rank() {  // of this thread among those of its CTA that share its row
+  return W == LP_WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
+}
+template <int W>
+constexpr int lp_size(int cta_threads) {
+  return W == LP_WARP ? 32 : cta_threads;
+}
+template <int W>
+__device__ __forceinline__ long long lp_row(LpShare sh) {
+  return W == LP_WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (long long)(blockIdx.x / sh.parts);
 }
 
 // LP_UNROLL vectors in flight a thread: 4 x 16 bytes x 1280 threads on an SM cover HBM's latency at its full rate.
@@ -239,12 +252,14 @@ constexpr int LP_UNROLL = 4;
 
 // One (m, s) for the row from each thread's, by MERGE: the same in every thread of every CTA of the row, and on return
 // all of them have read it.
-template <bool CL, typename MERGE>
+template <int W, typename MERGE>
 __device__ __forceinline__ float2 lp_join(float2 a, LpShare sh, MERGE&& merge) {
   __shared__ float2 sm[LP_THREADS / 32];
   __shared__ float2 all;
   for (int o = 16; o > 0; o >>= 1)
     a = merge(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
+  if constexpr (W == LP_WARP)  // which of two sums is scaled first rounds differently: lane 0's, for every lane
+    return make_float2(__shfl_sync(0xffffffffu, a.x, 0), __shfl_sync(0xffffffffu, a.y, 0));
   __syncthreads();  // an earlier join may still be read
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = a;
   __syncthreads();
@@ -252,7 +267,7 @@ __device__ __forceinline__ float2 lp_join(float2 a, LpShare sh, MERGE&& merge) {
 #pragma unroll
   for (int w = 1; w < LP_THREADS / 32; ++w)
     if (w < (int)(blockDim.x >> 5)) r = merge(r, sm[w]);
-  if constexpr (CL) {
+  if constexpr (W == LP_CLUSTER) {
     if (threadIdx.x == 0) all = r;
     cluster_sync_all();
     r = ld_shared_cluster_f2(mapa_shared(smem_u32(&all), 0));
@@ -296,40 +311,50 @@ __device__ __forceinline__ float2 lp_merge(float2 p, float2 q) {
   t.merge(q.x, q.y);
   return make_float2(t.m, t.s);
 }
-template <bool CL>
-struct LpCtaJoin {
+template <int W>
+struct LpTeamJoin {
   LpShare sh;
   __device__ float2 operator()(float2 v, bool max) const {
-    return max ? lp_join<CL>(v, sh, [](float2 p, float2 q) { return make_float2(fmaxf(p.x, q.x), 0.f); })
-               : lp_join<CL>(v, sh, [](float2 p, float2 q) { return make_float2(p.x + q.x, 0.f); });
+    return max ? lp_join<W>(v, sh, [](float2 p, float2 q) { return make_float2(fmaxf(p.x, q.x), 0.f); })
+               : lp_join<W>(v, sh, [](float2 p, float2 q) { return make_float2(p.x + q.x, 0.f); });
   }
 };
+// The careful pass by a row's whole team.
+template <typename E, int W, int THREADS>
+__device__ __forceinline__ LpRow lp_team_careful(const E* x, int V, LpShare sh) {
+  constexpr int N = lp_size<W>(THREADS);
+  return lp_careful(x, V, sh.part * N + lp_rank<W>(), sh.parts * N, LpTeamJoin<W>{sh});
+}
 
 // The sum of one row, the same in every thread of its CTAs, all of which have read it on return.
-template <typename E, bool CL>
+template <typename E, int W>
 __device__ __forceinline__ LpRow lp_row_sum(const E* x, int V, LpShare sh) {
   using L = LpType<E>;
+  constexpr int N = lp_size<W>(LP_THREADS);
   const int head = lp_head(x, V), nvec = (V - head) / L::VEC;
   LpSum a;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-  int v = sh.lo(nvec) + threadIdx.x;
-  const int vend = sh.hi(nvec);
-  for (; v + (LP_UNROLL - 1) * LP_THREADS < vend; v += LP_UNROLL * LP_THREADS) {
-    uint4 u[LP_UNROLL];
+  const int vend = sh.hi(nvec), wend = vend + (int)(threadIdx.x & 31);  // the loops are uniform over a warp
+  auto add = [&](auto unroll, int v) {
+    constexpr int U = decltype(unroll)::value;
+    uint4 u[U];
 #pragma unroll
-    for (int k = 0; k < LP_UNROLL; ++k) u[k] = xv[v + k * LP_THREADS];
-    a.template add<L, LP_UNROLL>(u);
+    for (int k = 0; k < U; ++k)
+      u[k] = v + k * N < vend ? xv[v + k * N] : make_uint4(L::LOWEST, L::LOWEST, L::LOWEST, L::LOWEST);
+    a.template add<L, U>(u);
+  };
+  int v = sh.lo(nvec) + lp_rank<W>();
+  for (; v + N < wend; v += LP_UNROLL * N) {
+    if (v + 2 * N < wend) add(std::integral_constant<int, LP_UNROLL>{}, v);
+    else add(std::integral_constant<int, 2>{}, v);
   }
-  for (; v < vend; v += LP_THREADS) {
-    const uint4 u[1] = {xv[v]};
-    a.template add<L, 1>(u);
-  }
+  if (v < wend) add(std::integral_constant<int, 1>{}, v);
   const int rest = V - nvec * L::VEC;  // the head, then the tail behind the vectors
-  for (int j = sh.lo(rest) + threadIdx.x; j < sh.hi(rest); j += LP_THREADS)
+  for (int j = sh.lo(rest) + lp_rank<W>(); j < sh.hi(rest); j += N)
     a.add(L::get(x[j < head ? j : j + nvec * L::VEC]));
-  const float2 r = lp_join<CL>(make_float2(a.m, a.s), sh, lp_merge);
+  const float2 r = lp_join<W>(make_float2(a.m, a.s), sh, lp_merge);
   if (lp_plain(r)) return lp_finish(r);
-  return lp_careful(x, V, sh.part * LP_THREADS + (int)threadIdx.x, sh.parts * LP_THREADS, LpCtaJoin<CL>{sh});
+  return lp_team_careful<E, W, LP_THREADS>(x, V, sh);
 }
 
 // 2^{c (x - a) - b} of two logits, times a factor
@@ -351,10 +376,11 @@ __device__ __forceinline__ void lp_at_label(F2 (&f)[L::VEC / 2], int at, float c
 
 // This CTA's share of coef * ([j = label] - p(x_j)) over one row; prob gives -coef * p. d may be x: each thread reads
 // an element before it writes the same one. LAST: nobody reads the row after this, so its lines may leave L2 first.
-template <typename E, bool LAST>
+template <typename E, int W, bool LAST>
 __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label, float coef, LpShare sh,
                                               const LpProb& prob) {
   using L = LpType<E>;
+  constexpr int N = lp_size<W>(LP_THREADS);
   const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
   const int head = vec ? lp_head(x, V) : V, nvec = (V - head) / L::VEC;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
@@ -367,34 +393,45 @@ __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label
     if (at >= 0 && at < L::VEC) lp_at_label<L>(f, at, coef);
     return L::pack(f);
   };
-  int v = sh.lo(nvec) + threadIdx.x;
+  int v = sh.lo(nvec) + lp_rank<W>();
   const int vend = sh.hi(nvec);
-  for (; v + (LP_UNROLL - 1) * LP_THREADS < vend; v += LP_UNROLL * LP_THREADS) {
+  if constexpr (W == LP_WARP) {  // short rows: one step takes most of them, its last vectors from some lanes only
+    for (; v - lp_rank<W>() < vend; v += LP_UNROLL * N) {
+      uint4 u[LP_UNROLL];
+#pragma unroll
+      for (int k = 0; k < LP_UNROLL; ++k)
+        if (v + k * N < vend) u[k] = xv[v + k * N];
+#pragma unroll
+      for (int k = 0; k < LP_UNROLL; ++k)
+        if (v + k * N < vend) __stcs(&dv[v + k * N], one(u[k], label - head - (v + k * N) * L::VEC));
+    }
+  }
+  for (; v + (LP_UNROLL - 1) * N < vend; v += LP_UNROLL * N) {
     uint4 u[LP_UNROLL];
 #pragma unroll
-    for (int k = 0; k < LP_UNROLL; ++k) u[k] = LAST ? __ldcs(&xv[v + k * LP_THREADS]) : xv[v + k * LP_THREADS];
+    for (int k = 0; k < LP_UNROLL; ++k) u[k] = LAST ? __ldcs(&xv[v + k * N]) : xv[v + k * N];
 #pragma unroll
     for (int k = 0; k < LP_UNROLL; ++k)
-      __stcs(&dv[v + k * LP_THREADS], one(u[k], label - head - (v + k * LP_THREADS) * L::VEC));  // not kept in L2
+      __stcs(&dv[v + k * N], one(u[k], label - head - (v + k * N) * L::VEC));  // not kept in L2
   }
-  for (; v < vend; v += LP_THREADS) dv[v] = one(xv[v], label - head - v * L::VEC);
+  for (; v < vend; v += N) dv[v] = one(xv[v], label - head - v * L::VEC);
   const int rest = V - nvec * L::VEC;
-  for (int i = sh.lo(rest) + threadIdx.x; i < sh.hi(rest); i += LP_THREADS) {
+  for (int i = sh.lo(rest) + lp_rank<W>(); i < sh.hi(rest); i += N) {
     const int j = i < head ? i : i + nvec * L::VEC;
     const float g = prob.one(L::get(x[j]));
     d[j] = L::put(j == label ? g + coef : g);
   }
 }
 
-template <typename E>
+template <typename E, int W>
 __device__ __forceinline__ void lp_write_zero(E* d, int V, LpShare sh) {
   using L = LpType<E>;
   const int head = lp_head(d, V), nvec = (V - head) / L::VEC;
   uint4* dv = reinterpret_cast<uint4*>(d + head);
-  for (int v = sh.lo(nvec) + threadIdx.x; v < sh.hi(nvec); v += blockDim.x)
+  for (int v = sh.lo(nvec) + lp_rank<W>(); v < sh.hi(nvec); v += lp_size<W>(blockDim.x))
     __stcs(&dv[v], make_uint4(0u, 0u, 0u, 0u));
   const int rest = V - nvec * L::VEC;
-  for (int i = sh.lo(rest) + threadIdx.x; i < sh.hi(rest); i += blockDim.x)
+  for (int i = sh.lo(rest) + lp_rank<W>(); i < sh.hi(rest); i += lp_size<W>(blockDim.x))
     d[i < head ? i : i + nvec * L::VEC] = L::put(0.f);
 }
 
@@ -467,7 +504,7 @@ __device__ __forceinline__ void lp_add_piece(LpSum& sum, const uint4* v, int n) 
 }
 
 // The sum of one row through shared memory, the same in every thread of its CTAs, all of which have read it on return.
-template <typename E, bool CL, int THREADS, int VECS, int SLOTS, typename F>
+template <typename E, int W, int THREADS, int VECS, int SLOTS, typename F>
 __device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, LpRow* out,
                                               F&& meanwhile) {
   using L = LpType<E>;
@@ -483,9 +520,8 @@ __device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, voi
     lp_add_piece<L, VECS, THREADS, 4>(a, st.wait(c), st.size(c));
     st.next(c);
   }
-  const float2 q = lp_join<CL>(make_float2(a.m, a.s), sh, lp_merge);
-  *out = lp_plain(q) ? lp_finish(q)
-                     : lp_careful(x, V, sh.part * THREADS + (int)threadIdx.x, sh.parts * THREADS, LpCtaJoin<CL>{sh});
+  const float2 q = lp_join<W>(make_float2(a.m, a.s), sh, lp_merge);
+  *out = lp_plain(q) ? lp_finish(q) : lp_team_careful<E, W, THREADS>(x, V, sh);
 }
 
 // ---------------------------------------------------------------------------- token log-probabilities
@@ -494,7 +530,7 @@ __device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, voi
 // scored: 44 us, 5.7 TB/s, as without the exponentials; four CTAs of 256 threads 51 us; loads into registers 55 us).
 constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512, LP_FWD_SLOTS = 3;
 constexpr uint32_t LP_FWD_SMEM = LP_FWD_SLOTS * LP_FWD_VECS * 16u;
-template <typename E, bool CL>
+template <typename E, int W>
 __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E* __restrict__ logits, LpRows lr, int V,
                                                                         const long long* __restrict__ labels,
                                                                         long long ignore_index,
@@ -506,7 +542,7 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
   __shared__ uint64_t full[LP_FWD_SLOTS];
   griddep_wait();
   griddep_launch();
-  const LpShare sh = lp_share<CL>();
+  const LpShare sh = lp_share<W>();
   const long long row = blockIdx.x / sh.parts;
   const long long label = labels[row];
   const bool first = threadIdx.x == 0 && sh.part == 0;
@@ -521,7 +557,7 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
   const E* x = logits + lr.offset(row);
   const float xl = first ? L::get(x[label]) : 0.f;
   LpRow r;
-  lp_staged_sum<E, CL, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r, [] {});
+  lp_staged_sum<E, W, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r, [] {});
   if (first) {
     const double lp = lp_label(xl, r);
     logps[row] = (float)lp;
@@ -531,17 +567,18 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
 }
 
 // Forward for short rows: one pass over a row with a running maximum and sum.
-template <typename E, bool CL>
+template <typename E, int W>
 __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restrict__ logits, LpRows lr, int V,
                                                               const long long* __restrict__ labels,
                                                               long long ignore_index, float* __restrict__ logps,
-                                                              float* __restrict__ lse, double* __restrict__ wide) {
+                                                              float* __restrict__ lse, double* __restrict__ wide, long long M) {
   griddep_wait();
   griddep_launch();
-  const LpShare sh = lp_share<CL>();
-  const long long row = blockIdx.x / sh.parts;
+  const LpShare sh = lp_share<W>();
+  const long long row = lp_row<W>(sh);
+  if (row >= M) return;  // whole warps
   const long long label = labels[row];
-  const bool first = threadIdx.x == 0 && sh.part == 0;
+  const bool first = lp_rank<W>() == 0 && sh.part == 0;
   if (!lp_scored(label, ignore_index, V)) {
     if (first) {
       logps[row] = 0.f;
@@ -551,7 +588,7 @@ __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restric
     return;
   }
   const E* x = logits + lr.offset(row);
-  const LpRow r = lp_row_sum<E, CL>(x, V, sh);
+  const LpRow r = lp_row_sum<E, W>(x, V, sh);
   if (first) {
     const double lp = lp_label(LpType<E>::get(x[label]), r);
     logps[row] = (float)lp;
@@ -562,31 +599,33 @@ __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restric
 
 // dlogits = coef * (onehot - e^{x - lse}); coef per token, or per sequence (per_seq). Elementwise, so dlogits may be
 // the logits themselves.
-template <typename E, bool CL>
+template <typename E, int W>
 __global__ void __launch_bounds__(LP_THREADS) logp_bwd_kernel(const E* logits, LpRows lr, int V,
                                                               const long long* __restrict__ labels,
                                                               long long ignore_index, const float* __restrict__ lse,
                                                               const float* __restrict__ coef, int per_seq, E* dlogits,
-                                                              LpRows dr) {
+                                                              LpRows dr, long long M) {
   griddep_wait();
   griddep_launch();
-  const LpShare sh = lp_share<CL>();
+  const LpShare sh = lp_share<W>();
   // the last rows first: the forward has left them in L2 (4092 rows of 100 KB: forward and backward 176 -> 166 us)
-  const long long row = (gridDim.x - 1 - blockIdx.x) / sh.parts;
+  const long long row = M - 1 - lp_row<W>(sh);
+  if (row < 0) return;  // whole warps
   const long long label = labels[row];
   E* d = dlogits + dr.offset(row);
   if (!lp_scored(label, ignore_index, V)) {
-    lp_write_zero(d, V, sh);
+    lp_write_zero<E, W>(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float l = lse[row], c = coef[per_seq ? lr.batch(row) : row];
   LpRow r = {l, 0.f, 1.f, 0.0};
   if (!(fabsf(l) <= LP_LSE_EXACT)) {
-    r = lp_careful(x, V, sh.part * LP_THREADS + (int)threadIdx.x, sh.parts * LP_THREADS, LpCtaJoin<CL>{sh});
-    __syncthreads();  // every thread has read the row before an in-place gradient
+    r = lp_team_careful<E, W, LP_THREADS>(x, V, sh);
+    if (W == LP_WARP) __syncwarp();  // every thread has read the row before an in-place gradient
+    else __syncthreads();
   }
-  lp_write_grad<E, false>(x, d, V, (int)label, c, sh, LpProb(r.a, r.b, -c * r.inv));
+  lp_write_grad<E, W, false>(x, d, V, (int)label, c, sh, LpProb(r.a, r.b, -c * r.inv));
 }
 
 // ---------------------------------------------------------------------------- sums over a CTA
@@ -734,17 +773,19 @@ __device__ __forceinline__ float policy_weight(const PolicyArgs& a, int n, int t
   return a.by_sequence ? 1.f / ((float)n * (float)total) : 1.f / (float)total;
 }
 
-// scored tokens of each sequence
+// scored tokens of each sequence: a warp a sequence, or for long ones a CTA
 __global__ void __launch_bounds__(256) policy_count_kernel(const long long* __restrict__ labels, long long ignore_index,
-                                                           int V, int T, int* __restrict__ counts) {
+                                                           int V, int B, int T, int by_warp, int* __restrict__ counts) {
   griddep_wait();
   griddep_launch();
   __shared__ int red[8];
-  const long long base = (long long)blockIdx.x * T;
+  const long long b = by_warp ? (long long)blockIdx.x * 8 + (threadIdx.x >> 5) : (long long)blockIdx.x;
+  const int step = by_warp ? 32 : 256;
   int c = 0;
-  for (int t = threadIdx.x; t < T; t += blockDim.x) c += lp_scored(labels[base + t], ignore_index, V) ? 1 : 0;
-  c = lp_block_sum(c, red);
-  if (threadIdx.x == 0) counts[blockIdx.x] = c;
+  if (b < B)
+    for (int t = threadIdx.x % step; t < T; t += step) c += lp_scored(labels[b * T + t], ignore_index, V) ? 1 : 0;
+  c = by_warp ? __reduce_add_sync(0xffffffffu, c) : lp_block_sum(c, red);
+  if (b < B && threadIdx.x % step == 0) counts[b] = c;
 }
 
 // Sum of counts (token mean) or number of nonempty sequences (sequence mean), over the whole CTA.
@@ -754,12 +795,22 @@ __device__ __forceinline__ int policy_total(const int* __restrict__ counts, int 
   return lp_block_sum(c, red);
 }
 
+__global__ void __launch_bounds__(1024) policy_total_kernel(const int* __restrict__ counts, int B, int by_sequence,
+                                                            int* __restrict__ total) {
+  griddep_wait();
+  griddep_launch();
+  __shared__ int red[32];
+  const int t = policy_total(counts, B, by_sequence, red);
+  if (threadIdx.x == 0) *total = t;
+}
+
 // The inputs and outputs of one row of the policy loss.
 struct PolicyRows {
   const long long* labels;
   long long ignore_index;
   const float *old, *ref, *adv;
   int* counts;
+  const int* total;   // policy_total, or with
   int B, count_here;  // few tokens: each CTA counts for itself, and a sequence's first CTA writes counts
   PolicyArgs a;
   float *logps, *lse, *coef;
@@ -785,11 +836,7 @@ __device__ __forceinline__ int2 policy_counts(const PolicyRows& p, LpRows lr, in
                                               int* red) {
   const unsigned b = lr.batch(row);
   int2 c = make_int2(0, 0);
-  if (!p.count_here) {
-    c.y = policy_total(p.counts, p.B, p.a.by_sequence, red);
-    c.x = p.counts[b];
-    return c;
-  }
+  if (!p.count_here) return make_int2(p.counts[b], *p.total);
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (p.a.by_sequence) {  // a warp a sequence
     for (unsigned s = threadIdx.x >> 5; s < (unsigned)p.B; s += warps) {
@@ -820,37 +867,47 @@ __device__ __forceinline__ void policy_row_unscored(const PolicyRows& p, long lo
 // row in L2 as long as few rows are on their way: three CTAs an SM (16368 rows of 50304 bf16 logits: 481 us, 5.5 TB/s;
 // nine smaller CTAs 570 us, their rows fill L2; without the hint that the second read is the last 542 us). Holding the
 // row in shared memory instead allows two rows an SM, too few to cover their phases' latencies: 557 us at best.
-template <typename E, bool CL>
+template <typename E, int W>
 __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpRows lr, int V, const PolicyRows p,
-                                                            E* dlogits, LpRows dr) {
+                                                            E* dlogits, LpRows dr, long long M) {
   griddep_wait();
   griddep_launch();
   __shared__ int red[LP_THREADS / 32];
   __shared__ float s_coef;
-  const LpShare sh = lp_share<CL>();
-  const long long row = blockIdx.x / sh.parts;
+  const LpShare sh = lp_share<W>();
+  const long long row = lp_row<W>(sh);
+  if (row >= M) return;  // whole warps
   const long long label = p.labels[row];
+  const bool first = lp_rank<W>() == 0 && sh.part == 0;
   E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
   if (!lp_scored(label, p.ignore_index, V)) {
-    if (threadIdx.x == 0 && sh.part == 0) policy_row_unscored(p, row);
-    if (p.count_here && sh.part == 0 && (unsigned)row % (unsigned)lr.T == 0) policy_counts(p, lr, V, row, true, red);
-    if (d) lp_write_zero(d, V, sh);
+    if (first) policy_row_unscored(p, row);
+    if (W != LP_WARP && p.count_here && sh.part == 0 && (unsigned)row % (unsigned)lr.T == 0)
+      policy_counts(p, lr, V, row, true, red);
+    if (d) lp_write_zero<E, W>(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float xl = LpType<E>::get(x[label]);  // before an in-place gradient
-  const int2 n = policy_counts(p, lr, V, row, sh.part == 0, red);
-  const LpRow r = lp_row_sum<E, CL>(x, V, sh);
-  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
+  const int2 n = W == LP_WARP ? make_int2(p.counts[lr.batch(row)], *p.total) : policy_counts(p, lr, V, row, sh.part == 0, red);
+  const LpRow r = lp_row_sum<E, W>(x, V, sh);
+  float coef = 0.f;
+  if (lp_rank<W>() == 0) coef = policy_row(p, lr, row, xl, r, n.x, n.y, first);
   if (!d) return;
-  __syncthreads();
-  lp_write_grad<E, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
+  if constexpr (W == LP_WARP) {
+    coef = __shfl_sync(0xffffffffu, coef, 0);
+  } else {
+    if (threadIdx.x == 0) s_coef = coef;
+    __syncthreads();
+    coef = s_coef;
+  }
+  lp_write_grad<E, W, true>(x, d, V, (int)label, coef, sh, LpProb(r.a, r.b, -coef * r.inv));
 }
 
 // The same for long rows, the first read by bulk copies.
 constexpr int POL_VECS = 1024, POL_SLOTS = 3;
 constexpr uint32_t POL_SMEM = POL_SLOTS * POL_VECS * 16u;
-template <typename E, bool CL>
+template <typename E, int W>
 __global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logits, LpRows lr, int V,
                                                                     const PolicyRows p, E* dlogits, LpRows dr) {
   using L = LpType<E>;
@@ -860,43 +917,47 @@ __global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logi
   __shared__ float s_coef;
   griddep_wait();
   griddep_launch();
-  const LpShare sh = lp_share<CL>();
+  const LpShare sh = lp_share<W>();
   const long long row = blockIdx.x / sh.parts;
   const long long label = p.labels[row];
   E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
   if (!lp_scored(label, p.ignore_index, V)) {
     if (threadIdx.x == 0 && sh.part == 0) policy_row_unscored(p, row);
     if (p.count_here && sh.part == 0 && (unsigned)row % (unsigned)lr.T == 0) policy_counts(p, lr, V, row, true, red);
-    if (d) lp_write_zero(d, V, sh);
+    if (d) lp_write_zero<E, W>(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float xl = L::get(x[label]);
   LpRow r;
   int2 n;
-  lp_staged_sum<E, CL, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, &r, [&] {
+  lp_staged_sum<E, W, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, &r, [&] {
     n = policy_counts(p, lr, V, row, sh.part == 0, red);  // while the first pieces are on their way
   });
   if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
   if (!d) return;
   __syncthreads();
-  lp_write_grad<E, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
+  lp_write_grad<E, W, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
 }
 
-// stats = {loss, policy term, KL, clipped share}: weighted sums over the tokens, from their log-probabilities
+// stats = {loss, policy term, KL, clipped share}: weighted sums over the tokens, from their log-probabilities, by one CTA
+// or, for many tokens, the CTAs of one cluster. total may lie in stats, which is written last.
 __global__ void __launch_bounds__(1024) policy_stats_kernel(const float* __restrict__ logps,
                                                             const long long* __restrict__ labels,
                                                             long long ignore_index, int V, int B, int T,
                                                             const float* __restrict__ old, const float* __restrict__ ref,
                                                             const float* __restrict__ adv, PolicyArgs a,
-                                                            const int* __restrict__ counts, float* __restrict__ stats) {
+                                                            const int* __restrict__ counts, const int* total_at,
+                                                            float* stats) {
   griddep_wait();
   griddep_launch();
   __shared__ double3 red[32];
+  __shared__ __align__(8) double mine[4];
   __shared__ int ired[32];
-  const int total = policy_total(counts, B, a.by_sequence, ired);
+  const int total = total_at ? *total_at : policy_total(counts, B, a.by_sequence, ired);
   double pg = 0.0, kl = 0.0, cut = 0.0;
-  for (long long i = threadIdx.x; i < (long long)B * T; i += blockDim.x) {
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < (long long)B * T;
+       i += (long long)gridDim.x * blockDim.x) {
     if (!lp_scored(labels[i], ignore_index, V)) continue;
     const unsigned b = (unsigned)i / (unsigned)T;
     const PolicyTerms t = policy_terms(a, (double)logps[i], old[i], ref != nullptr, ref ? ref[i] : 0.f,
@@ -906,13 +967,28 @@ __global__ void __launch_bounds__(1024) policy_stats_kernel(const float* __restr
     kl += w * (double)t.kl;
     cut += w * (double)t.cut;
   }
-  const double3 t = lp_block_sum3(make_double3(pg, kl, cut), red);
-  pg = t.x, kl = t.y, cut = t.z;
-  if (threadIdx.x == 0) {
-    stats[0] = (float)(pg + (double)a.kl * kl);
-    stats[1] = (float)pg;
-    stats[2] = (float)kl;
-    stats[3] = (float)cut;
+  double3 t = lp_block_sum3(make_double3(pg, kl, cut), red);
+  if (gridDim.x > 1) {
+    if (threadIdx.x == 0) mine[0] = t.x, mine[1] = t.y, mine[2] = t.z;
+    cluster_sync_all();
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      t = make_double3(0.0, 0.0, 0.0);
+      for (unsigned c = 0; c < gridDim.x; ++c) {
+        double v[3];
+        for (int k = 0; k < 3; ++k) {
+          const float2 h = ld_shared_cluster_f2(mapa_shared(smem_u32(&mine[k]), c));
+          v[k] = __hiloint2double(__float_as_int(h.y), __float_as_int(h.x));
+        }
+        t.x += v[0], t.y += v[1], t.z += v[2];
+      }
+    }
+    cluster_sync_all();  // no CTA leaves while its sums are read
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    stats[0] = (float)(t.x + (double)a.kl * t.y);
+    stats[1] = (float)t.x;
+    stats[2] = (float)t.y;
+    stats[3] = (float)t.z;
   }
 }
 
@@ -954,12 +1030,24 @@ static int lp_parts(long long M, int V, int dtype) {
   cudaGetDevice(&dev);
   const long long bytes = (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2), full = 2ll * rgpt_num_sms(dev);
   int c = 1;
-  while (c < 8 && 2 * c * M <= full && bytes / (2 * c) >= 8192) c *= 2;
+  while (c < 8 && 2 * c * M <= full && bytes / (2 * c) >= 8192) c *= 2;  // 1 for rows that a warp takes
   return c;
 }
 
 // Rows worth a trip through shared memory: below 16 KB their fixed cost (barriers, the copy's latency) shows.
 static bool lp_long(int V, int dtype) { return (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2) >= 16384; }
+
+// A warp a row: rows of up to 4 KB, or of up to 16 KB when there are enough of them for 8 warps an SM. bf16, forward us,
+// warp / CTA a row: 700 x 2000 3.0 / 4.3, 700 x 7000 6.1 / 5.6, 2000 x 4000 5.5 / 10.1, 2000 x 7000 8.1 / 12.2.
+static bool lp_warps(long long M, int V, int dtype) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const long long bytes = (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2);
+  return !lp_long(V, dtype) && (bytes <= 4096 || M >= 8ll * rgpt_num_sms(dev));
+}
+static dim3 lp_grid(long long M, int V, int dtype, int parts) {
+  return dim3((unsigned)(lp_warps(M, V, dtype) ? (M + LP_THREADS / 32 - 1) / (LP_THREADS / 32) : M * parts));
+}
 
 // Allows `kern` its dynamic shared memory on the current device (once).
 template <typename K>
@@ -982,15 +1070,16 @@ static int launch_logp_fwd(const void* logits, int dtype, LpRows lr, long long M
     using E = std::remove_pointer_t<decltype(tag)>;
     const int c = lp_parts(M, V, dtype);
     if (lp_long(V, dtype)) {
-      auto kern = c > 1 ? logp_fwd_staged_kernel<E, true> : logp_fwd_staged_kernel<E, false>;
+      auto kern = c > 1 ? logp_fwd_staged_kernel<E, LP_CLUSTER> : logp_fwd_staged_kernel<E, LP_CTA>;
       static bool set[2][64] = {};
       if ((rc = lp_smem(kern, LP_FWD_SMEM, set[c > 1])) == RGPT_OK)
         launch_pdl(kern, dim3((unsigned)(M * c)), dim3(LP_FWD_THREADS), LP_FWD_SMEM, s, c, (const E*)logits, lr, V, labels,
                    ignore_index, logps, lse, wide);
       return;
     }
-    launch_pdl(c > 1 ? logp_fwd_kernel<E, true> : logp_fwd_kernel<E, false>, dim3((unsigned)(M * c)), dim3(LP_THREADS), 0,
-               s, c, (const E*)logits, lr, V, labels, ignore_index, logps, lse, wide);
+    launch_pdl(lp_warps(M, V, dtype) ? logp_fwd_kernel<E, LP_WARP> : c > 1 ? logp_fwd_kernel<E, LP_CLUSTER> : logp_fwd_kernel<E, LP_CTA>,
+               lp_grid(M, V, dtype, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, labels, ignore_index, logps, lse,
+               wide, M);
   });
   return rc;
 }
@@ -1001,8 +1090,9 @@ static int launch_logp_bwd(const void* logits, int dtype, LpRows lr, long long M
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
     const int c = lp_parts(M, V, dtype);
-    launch_pdl(c > 1 ? logp_bwd_kernel<E, true> : logp_bwd_kernel<E, false>, dim3((unsigned)(M * c)), dim3(LP_THREADS), 0,
-               s, c, (const E*)logits, lr, V, labels, ignore_index, lse, coef, per_seq, (E*)dlogits, dr);
+    launch_pdl(lp_warps(M, V, dtype) ? logp_bwd_kernel<E, LP_WARP> : c > 1 ? logp_bwd_kernel<E, LP_CLUSTER> : logp_bwd_kernel<E, LP_CTA>,
+               lp_grid(M, V, dtype, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, labels, ignore_index, lse, coef,
+               per_seq, (E*)dlogits, dr, M);
   });
   return RGPT_OK;
 }
@@ -1071,27 +1161,35 @@ extern "C" int rgpt_policy_loss(const void* logits, int dtype, long long sb, lon
                         adv_per_token, by_sequence};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // up to this many tokens each CTA counts them for itself, while its row is on its way, which saves a launch
-  const int count_here = (long long)B * T <= 2048 ? 1 : 0;
-  if (!count_here) launch_pdl(policy_count_kernel, dim3(B), dim3(256), 0, s, 1, labels, ignore_index, V, T, counts);
+  const long long rows = (long long)B * T;
+  const bool warps = lp_warps(rows, V, dtype);
+  const int count_here = rows <= 2048 && !warps ? 1 : 0;
+  int* total = count_here ? nullptr : reinterpret_cast<int*>(stats);  // kept there until the statistics replace it
+  if (!count_here) {
+    const int by_warp = T <= 128 ? 1 : 0;
+    launch_pdl(policy_count_kernel, dim3(by_warp ? (B + 7) / 8 : B), dim3(256), 0, s, 1, labels, ignore_index, V, B, T,
+               by_warp, counts);
+    launch_pdl(policy_total_kernel, dim3(1), dim3(1024), 0, s, 1, (const int*)counts, B, by_sequence, total);
+  }
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
     const LpRows lr = {sb, st, T}, dr = {db, dt, T};
-    const PolicyRows p = {labels, ignore_index, old_logps, ref_logps, advantages, counts, B, count_here, a, token_logps, lse, coef};
+    const PolicyRows p = {labels, ignore_index, old_logps, ref_logps, advantages, counts, total, B, count_here, a, token_logps, lse, coef};
     const unsigned M = (unsigned)((long long)B * T);
     const int c = lp_parts(M, V, dtype);
     if (lp_long(V, dtype)) {
-      auto kern = c > 1 ? policy_staged_kernel<E, true> : policy_staged_kernel<E, false>;
+      auto kern = c > 1 ? policy_staged_kernel<E, LP_CLUSTER> : policy_staged_kernel<E, LP_CTA>;
       static bool set[2][64] = {};
       if ((rc = lp_smem(kern, POL_SMEM, set[c > 1])) == RGPT_OK)
         launch_pdl(kern, dim3(M * c), dim3(LP_THREADS), POL_SMEM, s, c, (const E*)logits, lr, V, p, (E*)dlogits, dr);
       return;
     }
-    launch_pdl(c > 1 ? policy_kernel<E, true> : policy_kernel<E, false>, dim3(M * c), dim3(LP_THREADS), 0, s, c,
-               (const E*)logits, lr, V, p, (E*)dlogits, dr);
+    launch_pdl(warps ? policy_kernel<E, LP_WARP> : c > 1 ? policy_kernel<E, LP_CLUSTER> : policy_kernel<E, LP_CTA>,
+               lp_grid(M, V, dtype, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, p, (E*)dlogits, dr, (long long)M);
   });
   if (rc) return rc;
-  const long long M = (long long)B * T;
-  launch_pdl(policy_stats_kernel, dim3(1), dim3(M < 1024 ? (unsigned)((M + 31) / 32 * 32) : 1024u), 0, s, 1, (const float*)token_logps, labels, ignore_index, V, B, T,
-             old_logps, ref_logps, advantages, a, (const int*)counts, stats);
+  const int ctas = rows > 8192 ? 8 : 1;
+  launch_pdl(policy_stats_kernel, dim3(ctas), dim3(rows < 1024 ? (unsigned)((rows + 31) / 32 * 32) : 1024u), 0, s, ctas, (const float*)token_logps, labels, ignore_index, V, B, T,
+             old_logps, ref_logps, advantages, a, (const int*)counts, (const int*)total, stats);
   return rgpt_check_launch("policy_loss kernels");
 }

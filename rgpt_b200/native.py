@@ -559,7 +559,7 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     if p is not None:
         return _call_on(p[20], "rgpt_policy_loss", *p[:8], int(ignore_index), *p[8:12], float(clip_low),
                         float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *p[12:20],
-                        kernels=2 + (p[4] * p[5] > 2048))
+                        kernels=2 + 2 * (p[4] * p[5] > 2048))
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     dev, shape, f32 = logits.get_device(), logits.shape[:-1], torch.float32
     per_token = advantages.shape != (B,)
@@ -573,7 +573,7 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
         raise ValueError(f"policy_loss needs at least one token, got logits {tuple(logits.shape)}")
     _call_on(dev, "rgpt_policy_loss", logits.data_ptr(), dt, sb, st, B, T, V, *ins, adv, int(per_token), float(clip_low),
              float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *outs, *grad,
-             kernels=2 + (B * T > 2048))
+             kernels=2 + 2 * (B * T > 2048))
 
 
 def _linear_operands(x: torch.Tensor, w: torch.Tensor):
