@@ -14,6 +14,8 @@
 //   F R   as f, b, or None                                    address or None
 //   W     as d, or None: allocated                            address
 //   P     None: 4 M ceil(V / 128) fp32 are allocated           address, their number
+//   z     fp32, contiguous: the shape of N, and n              nothing
+//   N     None: fp32 of z's shape is allocated                 address
 // All tensors are on one GPU, whose index follows the arguments; behind it stand the tensors allocated here, which live
 // as long as the list.
 #define PY_SSIZE_T_CLEAN
@@ -32,7 +34,9 @@ struct Pack {
   int64_t device = -1;
   const at::Tensor* logits = nullptr;
   const at::Tensor* like = nullptr;  // the first tensor: what is allocated goes where it is
-  at::Tensor made;
+  const at::Tensor* shape = nullptr;  // z
+  at::Tensor made[2];
+  int n_made = 0;
   bool ok = true;
 
   void put(int64_t v) {
@@ -88,11 +92,14 @@ struct Pack {
         put_none();
         return ok;
       }
-      if ((kind == 'W' || kind == 'P') && like != nullptr) {
+      if ((kind == 'W' || kind == 'P' || kind == 'N') && like != nullptr && n_made < 2) {
         const int64_t floats = 4 * M * ((V + 127) / 128);
-        made = kind == 'P' ? at::empty({floats}, like->options().dtype(at::kFloat))
-                           : at::empty({B * T}, like->options().dtype(at::kDouble));
-        put_address(made);
+        if (kind == 'N' && shape == nullptr) return false;
+        at::Tensor& t = made[n_made++];
+        t = kind == 'P'   ? at::empty({floats}, like->options().dtype(at::kFloat))
+            : kind == 'N' ? at::empty(shape->sizes(), like->options().dtype(at::kFloat))
+                          : at::empty({B * T}, like->options().dtype(at::kDouble));
+        put_address(t);
         if (kind == 'P') put(floats);
         return ok;
       }
@@ -152,6 +159,10 @@ struct Pack {
         put_address(t), put(per_sequence ? 0 : 1);
         return ok;
       }
+      case 'z':
+        if (!is(t, at::kFloat)) return false;
+        shape = tp, n = t.numel();
+        return true;
       case 'u':
         if (n < 0) n = t.numel();
         if (!is(t, at::kByte) || !vec(t, n) || n < 1) return false;
@@ -193,8 +204,8 @@ PyObject* pack(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   if (good) {
     p.put(p.device);
-    if (p.made.defined()) {
-      PyObject* o = THPVariable_Wrap(p.made);
+    for (int i = 0; i < p.n_made; ++i) {
+      PyObject* o = THPVariable_Wrap(p.made[i]);
       if (o != nullptr) PyList_Append(p.out, o);
       Py_XDECREF(o);
     }

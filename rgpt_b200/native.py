@@ -694,17 +694,21 @@ def adamw8(table: torch.Tensor, chunk_tensor: torch.Tensor, chunk_start: torch.T
               _lib.stream_ptr(table.device))
 
 
-def adamw8_moments(mq: torch.Tensor, m_scale: torch.Tensor, vq: torch.Tensor, v_scale: torch.Tensor, m: torch.Tensor,
-                   v: torch.Tensor) -> None:
-    """m, v (fp32) = the moments that 8-bit codes and their scales stand for."""
-    p = _pack("ususmm", (mq, m_scale, vq, v_scale, m, v))
-    if p is not None:
-        return _call_on(p[6], "rgpt_adamw8_moments", *p[:6], mq.shape[0])
-    n, dev, f32 = m.numel(), m.get_device(), torch.float32
+def adamw8_moments(p: torch.Tensor, mq: torch.Tensor, m_scale: torch.Tensor, vq: torch.Tensor, v_scale: torch.Tensor):
+    """(m, v), fp32 of p's shape: the moments of parameter p that 8-bit codes and their scales stand for."""
+    a = _pack("zususNN", (p, mq, m_scale, vq, v_scale, None, None))
+    if a is not None:
+        _call_on(a[6], "rgpt_adamw8_moments", *a[:6], mq.shape[0])
+        return a[7], a[8]
+    n, dev, f32 = p.numel(), p.get_device(), torch.float32
     blocks = (n + ADAM8_BLOCK - 1) // ADAM8_BLOCK
-    _call_on(dev, "rgpt_adamw8_moments", _flat(mq, "m codes", (n,), torch.uint8, dev), _flat(m_scale, "m scales", (blocks,), f32, dev),
-             _flat(vq, "v codes", (n,), torch.uint8, dev), _flat(v_scale, "v scales", (blocks,), f32, dev),
-             _flat(m, "m", m.shape, f32, dev), _flat(v, "v", m.shape, f32, dev), n)
+    args = (_flat(mq, "m codes", (n,), torch.uint8, dev), _flat(m_scale, "m scales", (blocks,), f32, dev),
+            _flat(vq, "v codes", (n,), torch.uint8, dev), _flat(v_scale, "v scales", (blocks,), f32, dev))
+    if dev < 0:
+        raise RuntimeError("librgpt_kernels only takes CUDA tensors (no CPU path)")
+    m, v = (torch.empty(p.shape, device=p.device, dtype=f32) for _ in range(2))
+    _call_on(dev, "rgpt_adamw8_moments", *args, m.data_ptr(), v.data_ptr(), n)
+    return m, v
 
 
 def muon_prep(table, n, R, C, X, beta, nesterov, sumsq, hp: int | None = None) -> None:

@@ -598,9 +598,8 @@ class Muon(torch.optim.Optimizer):
         own tensors with 32 bits, new ones decoded from their codes with 8."""
         st = self.state.get(p, {})
         if "exp_avg_q8" in st:
-            m, v = torch.empty((2,) + p.shape, device=p.device, dtype=torch.float32).unbind()
-            nv.adamw8_moments(st["exp_avg_q8"], st["exp_avg_scale"], st["exp_avg_sq_q8"], st["exp_avg_sq_scale"], m, v)
-            return m, v
+            return nv.adamw8_moments(p, st["exp_avg_q8"], st["exp_avg_scale"], st["exp_avg_sq_q8"],
+                                     st["exp_avg_sq_scale"])
         if "exp_avg" not in st:
             raise ValueError("this parameter has no AdamW moments (no step yet, or it belongs to a Muon group)")
         return st["exp_avg"], st["exp_avg_sq"]

@@ -126,8 +126,7 @@ def test_all_codes_round_trip(cuda):
     n = 256
     q = torch.arange(256, dtype=torch.uint8, device=cuda)
     one = torch.ones(1, device=cuda)
-    m, v = torch.empty(n, device=cuda), torch.empty(n, device=cuda)
-    nv.adamw8_moments(q, one, q, one, m, v)
+    m, v = nv.adamw8_moments(torch.empty(n, device=cuda), q, one, q, one)
     want = q.cpu().view(torch.float8_e4m3fn).float()
     assert torch.equal(torch.isnan(m.cpu()), torch.isnan(want))
     assert torch.equal(m.cpu()[~torch.isnan(want)], want[~torch.isnan(want)])

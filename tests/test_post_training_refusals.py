@@ -119,6 +119,17 @@ def test_linear_logprobs_refuses_types_scratch_and_outputs():
         nv.linear_logprobs_bwd(x, w, y, o, o, None, None, chunk_rows=0)
 
 
+def test_adamw8_moments_refuses():
+    p, q, s = z(300), z(300, dt=torch.uint8), z(2)
+    for bad in ((p, q[:299], s, q, s), (p, q, z(1), q, s), (p, q, s, q, z(3))):
+        with pytest.raises(ValueError, match="codes|scales"):
+            nv.adamw8_moments(*bad)
+    with pytest.raises(TypeError):
+        nv.adamw8_moments(p, q.int(), s, q, s)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        nv.adamw8_moments(p, q, s, q, s)
+
+
 def test_adam_state_bits():
     p = torch.nn.Parameter(z(8))
     with pytest.raises(ValueError, match="adam_state_bits"):
