@@ -54,7 +54,7 @@ enum RgptEpilogue {
   RGPT_EPI_POLY_F32 = 8,   /* D f32  = beta*C + alpha*acc, C f32 (fp32 Newton-Schulz)  */
   RGPT_EPI_ARGMAX_BF16 = 9, /* no D: per row and column tile, the first maximum of bf16(alpha*acc) and its
                               column (rgpt_gemm_argmax only)                          */
-  RGPT_EPI_LSE_F32 = 10,   /* no D: per row and column tile, the maximum and the sum of e^{acc - maximum}
+  RGPT_EPI_LSE_F32 = 10,   /* no D: per row and half column tile, the sum of exponentials and its reference
                               (rgpt_linear_logprobs only)                             */
   RGPT_EPI_SOFTMAX_GRAD_BF16 = 11 /* D bf16 = coef[m]*([n = label[m]] - e^{acc - lse[m]})
                               (rgpt_linear_logprobs_dlogits only)                     */
@@ -224,8 +224,8 @@ int rgpt_cross_entropy_noalloc(void* logits, long long ld, int M, int V, const l
  * vocabulary, any alignment of the type; labels [B, T] int64, contiguous. A token is scored when its label lies in
  * [0, V) and is not ignore_index; an unscored row is not read, has log-probability 0 and a zero gradient row.
  * dlogits has the logits' type and its own strides db, dt; it may be the logits themselves (same pointer and
- * strides), which are then overwritten. B*T < 2^31. Sums are fp32 or wider, and in a fixed order: equal calls give
- * equal bits. */
+ * strides), which are then overwritten; all other outputs share no memory with the inputs. B*T < 2^31. Sums are fp32 or
+ * wider, and in a fixed order: equal calls give equal bits. */
 enum RgptDtype { RGPT_DTYPE_BF16 = 0, RGPT_DTYPE_F16 = 1, RGPT_DTYPE_F32 = 2 };
 /* logps [B, T] = logits[label] - lse, lse [B, T] (optional) = log sum_j e^{logits_j}; 0 where not scored. */
 int rgpt_token_logprobs(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,
@@ -335,7 +335,7 @@ int rgpt_adamw(const RgptAdamwTensor* table, const int* chunk_tensor, const long
  * Codes round to nearest, ties to even; a block whose largest moment is not above 2^-100 holds zeros. The update:
  *   m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2;  p = p (1 - lr wd) - lr ((m / (sqrt(v) inv_sqrt_bc2 + eps)) inv_bc1)
  * from the moments before they are rounded to codes. The moments take one fp32 rounding an operation; the division is
- * accurate to 2 ulp. chunk_elems: a multiple of 256, and every chunk_start too. */
+ * accurate to 2 ulp. A moment that is not finite makes its whole block's so. chunk_elems: a multiple of 256, and every chunk_start too. */
 #define RGPT_ADAMW8_BLOCK 256
 typedef struct RgptAdamw8Tensor {
   float* p; const float* g; unsigned char* mq; float* m_scale; unsigned char* vq; float* r_scale;

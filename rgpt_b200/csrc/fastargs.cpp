@@ -10,12 +10,12 @@
 //   b h c fp32 [B] / fp32 [B / 2] / int32 [B]                 address
 //   a     fp32 [B], or of the leading shape                   address, 1 for the leading shape
 //   1 4   fp32 [1] / [4]                                      address
-//   u s m uint8 [n] / fp32 [ceil(n / 256)] / fp32, n in all   address (n: the first u's length)
+//   u s   uint8 [n] / fp32 [ceil(n / 256)]                    address
 //   F R   as f, b, or None                                    address or None
-//   W     as d, or None: allocated                            address
-//   P     None: 4 M ceil(V / 128) fp32 are allocated           address, their number
-//   z     fp32, contiguous: the shape of N, and n              nothing
-//   N     None: fp32 of z's shape is allocated                 address
+//   W     fp64 of the leading shape; None: allocated          address
+//   P     fp32, 4 M ceil(V / 128) at least; None: allocated   address, their number
+//   z     fp32, contiguous: gives N its shape, and n          nothing
+//   N     None: fp32 of z's shape is allocated                address
 // All tensors are on one GPU, whose index follows the arguments; behind it stand the tensors allocated here, which live
 // as long as the list.
 #define PY_SSIZE_T_CLEAN
@@ -159,16 +159,18 @@ struct Pack {
         put_address(t), put(per_sequence ? 0 : 1);
         return ok;
       }
+      case 'P':
+        if (!is(t, at::kFloat) || t.numel() < 4 * M * ((V + 127) / 128)) return false;
+        put_address(t), put(t.numel());
+        return ok;
       case 'z':
         if (!is(t, at::kFloat)) return false;
         shape = tp, n = t.numel();
         return true;
       case 'u':
-        if (n < 0) n = t.numel();
         if (!is(t, at::kByte) || !vec(t, n) || n < 1) return false;
         break;
       case 's': if (!is(t, at::kFloat) || !vec(t, (n + 255) / 256)) return false; break;
-      case 'm': if (!is(t, at::kFloat) || t.numel() != n) return false; break;
       default: return false;
     }
     put_address(t);

@@ -76,7 +76,8 @@ struct EpiParams {
   // LSE_F32 / SOFTMAX_GRAD_BF16: each row's label (scored when in [0, N) and not ignore_index)
   const long long* labels;
   long long ignore_index;
-  float2* lse_part;        // LSE_F32: [half column tile][M] (M, sum of 2^{c v - M}), M = ceil(c max), c = log2 e, of its columns
+  float2* lse_part;        // LSE_F32: [half column tile][M], of its columns (m, sum of 2^{c v - m}), m = ceil(c max),
+                           // c = log2 e
   float* label_logit;      // LSE_F32: [M], the label's value, written for scored rows only
   int round_bf16;          // LSE_F32: the values are rounded to bf16 first (what a stored bf16 product would hold)
   const float* row_lse;    // SOFTMAX_GRAD_BF16: [M]
@@ -1054,7 +1055,7 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
   sh.am = lsx && m128 == 1 ? (M + 7) / 8 * 8 : GEMM_BM;
   if (lsx && m128 == 1 && BN == 256) {
     const int rounds = ((N + 255) / 256 + nsm - 1) / nsm;
-    sh.bn = ((N + rounds * nsm - 1) / (rounds * nsm) + 15) / 16 * 16;
+    sh.bn = std::max(128, ((N + rounds * nsm - 1) / (rounds * nsm) + 15) / 16 * 16);  // the partial buffer's size counts on 128
   }
   sh.n_tiles = (N + sh.bn - 1) / sh.bn;
   const int tiles = batch * sh.m_tiles * sh.n_tiles;

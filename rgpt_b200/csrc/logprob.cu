@@ -162,9 +162,9 @@ __device__ __forceinline__ float lp_ref(float m) { return m == -INFINITY ? 0.f :
 // element. What is the same for every row would add up over a long sequence, so it is kept small: c's first part alone
 // makes log-probabilities some 6e-8 too high; M = ceil(c max) is a whole number, so that rescaling a sum is exact (with
 // any other M the hardware exponential's mean relative error, -5.25e-8 over a binade, comes in at each rescaling: 2e-7
-// in all); and that error of the elements themselves is taken off the row's sum at the end. Elements up to LP_LOW, where c x overflows, count as nothing (M = -inf). A row
-// that holds nothing else, or whose |M| is so large that c max - M may be (beyond LP_WIDE its 2^-24 |M| is no longer
-// small), takes lp_row_sum's careful pass: e^{x - max} after the subtraction.
+// in all); and that error of the elements themselves is taken off the row's sum at the end. Elements up to LP_LOW, where c x
+// overflows, count as nothing (M = -inf). A row that holds nothing else, or whose |M| is so large that c max - M may be
+// (beyond LP_WIDE its 2^-24 |M| is no longer small), takes the careful pass: e^{x - max} after the subtraction.
 struct LpSum {
   float m = -INFINITY, s = 0.f;
   __device__ __forceinline__ void merge(float om, float os) {
@@ -244,7 +244,8 @@ constexpr int lp_size(int cta_threads) {
 }
 template <int W>
 __device__ __forceinline__ long long lp_row(LpShare sh) {
-  return W == LP_WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : (long long)(blockIdx.x / sh.parts);
+  if (W == LP_WARP) return (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  return (long long)(blockIdx.x / sh.parts);
 }
 
 // LP_UNROLL vectors in flight a thread: 4 x 16 bytes x 1280 threads on an SM cover HBM's latency at its full rate.
@@ -326,32 +327,32 @@ __device__ __forceinline__ LpRow lp_team_careful(const E* x, int V, LpShare sh) 
   return lp_careful(x, V, sh.part * N + lp_rank<W>(), sh.parts * N, LpTeamJoin<W>{sh});
 }
 
-// The sum of one row, the same in every thread of its CTAs, all of which have read it on return.
+// The sum of one short row, the same in every thread of its CTA or warp, all of which have read it on return.
 template <typename E, int W>
-__device__ __forceinline__ LpRow lp_row_sum(const E* x, int V, LpShare sh) {
+__device__ __forceinline__ LpRow lp_row_sum(const E* x, int V) {
   using L = LpType<E>;
   constexpr int N = lp_size<W>(LP_THREADS);
+  const LpShare sh = {0, 1};
   const int head = lp_head(x, V), nvec = (V - head) / L::VEC;
   LpSum a;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-  const int vend = sh.hi(nvec), wend = vend + (int)(threadIdx.x & 31);  // the loops are uniform over a warp
+  const int wend = nvec + (int)(threadIdx.x & 31);  // the loops are uniform over a warp
   auto add = [&](auto unroll, int v) {
     constexpr int U = decltype(unroll)::value;
     uint4 u[U];
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      u[k] = v + k * N < vend ? xv[v + k * N] : make_uint4(L::LOWEST, L::LOWEST, L::LOWEST, L::LOWEST);
+      u[k] = v + k * N < nvec ? xv[v + k * N] : make_uint4(L::LOWEST, L::LOWEST, L::LOWEST, L::LOWEST);
     a.template add<L, U>(u);
   };
-  int v = sh.lo(nvec) + lp_rank<W>();
+  int v = lp_rank<W>();
   for (; v + N < wend; v += LP_UNROLL * N) {
     if (v + 2 * N < wend) add(std::integral_constant<int, LP_UNROLL>{}, v);
     else add(std::integral_constant<int, 2>{}, v);
   }
   if (v < wend) add(std::integral_constant<int, 1>{}, v);
   const int rest = V - nvec * L::VEC;  // the head, then the tail behind the vectors
-  for (int j = sh.lo(rest) + lp_rank<W>(); j < sh.hi(rest); j += N)
-    a.add(L::get(x[j < head ? j : j + nvec * L::VEC]));
+  for (int j = lp_rank<W>(); j < rest; j += N) a.add(L::get(x[j < head ? j : j + nvec * L::VEC]));
   const float2 r = lp_join<W>(make_float2(a.m, a.s), sh, lp_merge);
   if (lp_plain(r)) return lp_finish(r);
   return lp_team_careful<E, W, LP_THREADS>(x, V, sh);
@@ -571,14 +572,14 @@ template <typename E, int W>
 __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restrict__ logits, LpRows lr, int V,
                                                               const long long* __restrict__ labels,
                                                               long long ignore_index, float* __restrict__ logps,
-                                                              float* __restrict__ lse, double* __restrict__ wide, long long M) {
+                                                              float* __restrict__ lse,
+                                                              double* __restrict__ wide, long long M) {
   griddep_wait();
   griddep_launch();
-  const LpShare sh = lp_share<W>();
-  const long long row = lp_row<W>(sh);
+  const long long row = lp_row<W>(LpShare{0, 1});
   if (row >= M) return;  // whole warps
   const long long label = labels[row];
-  const bool first = lp_rank<W>() == 0 && sh.part == 0;
+  const bool first = lp_rank<W>() == 0;
   if (!lp_scored(label, ignore_index, V)) {
     if (first) {
       logps[row] = 0.f;
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(LP_THREADS) logp_fwd_kernel(const E* __restric
     return;
   }
   const E* x = logits + lr.offset(row);
-  const LpRow r = lp_row_sum<E, W>(x, V, sh);
+  const LpRow r = lp_row_sum<E, W>(x, V);
   if (first) {
     const double lp = lp_label(LpType<E>::get(x[label]), r);
     logps[row] = (float)lp;
@@ -863,10 +864,7 @@ __device__ __forceinline__ void policy_row_unscored(const PolicyRows& p, long lo
   if (p.coef) p.coef[row] = 0.f;
 }
 
-// One CTA a row (or a share of it): the sum, the coefficient, then the gradient from a second read, which finds the
-// row in L2 as long as few rows are on their way: three CTAs an SM (16368 rows of 50304 bf16 logits: 481 us, 5.5 TB/s;
-// nine smaller CTAs 570 us, their rows fill L2; without the hint that the second read is the last 542 us). Holding the
-// row in shared memory instead allows two rows an SM, too few to cover their phases' latencies: 557 us at best.
+// A row's sum, its coefficient, then its gradient from a second read. Here for short rows, by one CTA or one warp each.
 template <typename E, int W>
 __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpRows lr, int V, const PolicyRows p,
                                                             E* dlogits, LpRows dr, long long M) {
@@ -874,25 +872,25 @@ __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpR
   griddep_launch();
   __shared__ int red[LP_THREADS / 32];
   __shared__ float s_coef;
-  const LpShare sh = lp_share<W>();
+  const LpShare sh = {0, 1};
   const long long row = lp_row<W>(sh);
   if (row >= M) return;  // whole warps
   const long long label = p.labels[row];
-  const bool first = lp_rank<W>() == 0 && sh.part == 0;
+  const bool first = lp_rank<W>() == 0;
   E* d = dlogits ? dlogits + dr.offset(row) : nullptr;
   if (!lp_scored(label, p.ignore_index, V)) {
     if (first) policy_row_unscored(p, row);
-    if (W != LP_WARP && p.count_here && sh.part == 0 && (unsigned)row % (unsigned)lr.T == 0)
+    if (W != LP_WARP && p.count_here && (unsigned)row % (unsigned)lr.T == 0)
       policy_counts(p, lr, V, row, true, red);
     if (d) lp_write_zero<E, W>(d, V, sh);
     return;
   }
   const E* x = logits + lr.offset(row);
   const float xl = LpType<E>::get(x[label]);  // before an in-place gradient
-  const int2 n = W == LP_WARP ? make_int2(p.counts[lr.batch(row)], *p.total) : policy_counts(p, lr, V, row, sh.part == 0, red);
-  const LpRow r = lp_row_sum<E, W>(x, V, sh);
+  const int2 n = W == LP_WARP ? make_int2(p.counts[lr.batch(row)], *p.total) : policy_counts(p, lr, V, row, true, red);
+  const LpRow r = lp_row_sum<E, W>(x, V);
   float coef = 0.f;
-  if (lp_rank<W>() == 0) coef = policy_row(p, lr, row, xl, r, n.x, n.y, first);
+  if (first) coef = policy_row(p, lr, row, xl, r, n.x, n.y, true);
   if (!d) return;
   if constexpr (W == LP_WARP) {
     coef = __shfl_sync(0xffffffffu, coef, 0);
@@ -904,7 +902,11 @@ __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpR
   lp_write_grad<E, W, true>(x, d, V, (int)label, coef, sh, LpProb(r.a, r.b, -coef * r.inv));
 }
 
-// The same for long rows, the first read by bulk copies.
+// The same for long rows, by one CTA each (or a share of it), the first read by bulk copies. The second read finds the
+// row in L2 as long as few rows are on their way: three CTAs an SM (16368 rows of 50304 bf16 logits, of which 15 in 16
+// are scored: 463 us, 5.6 TB/s; nine smaller CTAs some 90 us more, their rows fill L2; without the hint that the second
+// read is the last 60 us more). Holding the row in shared memory instead allows two rows an SM, too few to cover their
+// phases' latencies: 80 us more at best.
 constexpr int POL_VECS = 1024, POL_SLOTS = 3;
 constexpr uint32_t POL_SMEM = POL_SLOTS * POL_VECS * 16u;
 template <typename E, int W>
@@ -1045,8 +1047,8 @@ static bool lp_warps(long long M, int V, int dtype) {
   const long long bytes = (long long)V * (dtype == RGPT_DTYPE_F32 ? 4 : 2);
   return !lp_long(V, dtype) && (bytes <= 4096 || M >= 8ll * rgpt_num_sms(dev));
 }
-static dim3 lp_grid(long long M, int V, int dtype, int parts) {
-  return dim3((unsigned)(lp_warps(M, V, dtype) ? (M + LP_THREADS / 32 - 1) / (LP_THREADS / 32) : M * parts));
+static dim3 lp_grid(long long M, bool warps, int parts) {
+  return dim3((unsigned)(warps ? (M + LP_THREADS / 32 - 1) / (LP_THREADS / 32) : M * parts));
 }
 
 // Allows `kern` its dynamic shared memory on the current device (once).
@@ -1077,9 +1079,9 @@ static int launch_logp_fwd(const void* logits, int dtype, LpRows lr, long long M
                    ignore_index, logps, lse, wide);
       return;
     }
-    launch_pdl(lp_warps(M, V, dtype) ? logp_fwd_kernel<E, LP_WARP> : c > 1 ? logp_fwd_kernel<E, LP_CLUSTER> : logp_fwd_kernel<E, LP_CTA>,
-               lp_grid(M, V, dtype, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, labels, ignore_index, logps, lse,
-               wide, M);
+    const bool warps = lp_warps(M, V, dtype);
+    launch_pdl(warps ? logp_fwd_kernel<E, LP_WARP> : logp_fwd_kernel<E, LP_CTA>, lp_grid(M, warps, 1), dim3(LP_THREADS), 0, s,
+               1, (const E*)logits, lr, V, labels, ignore_index, logps, lse, wide, M);
   });
   return rc;
 }
@@ -1090,9 +1092,10 @@ static int launch_logp_bwd(const void* logits, int dtype, LpRows lr, long long M
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
     const int c = lp_parts(M, V, dtype);
-    launch_pdl(lp_warps(M, V, dtype) ? logp_bwd_kernel<E, LP_WARP> : c > 1 ? logp_bwd_kernel<E, LP_CLUSTER> : logp_bwd_kernel<E, LP_CTA>,
-               lp_grid(M, V, dtype, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, labels, ignore_index, lse, coef,
-               per_seq, (E*)dlogits, dr, M);
+    const bool warps = lp_warps(M, V, dtype);
+    auto kern = warps ? logp_bwd_kernel<E, LP_WARP> : c > 1 ? logp_bwd_kernel<E, LP_CLUSTER> : logp_bwd_kernel<E, LP_CTA>;
+    launch_pdl(kern, lp_grid(M, warps, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, labels, ignore_index, lse,
+               coef, per_seq, (E*)dlogits, dr, M);
   });
   return RGPT_OK;
 }
@@ -1160,10 +1163,12 @@ extern "C" int rgpt_policy_loss(const void* logits, int dtype, long long sb, lon
   const PolicyArgs a = {clip_low, clip_high, kl_coef, grad_scale, log1p(-(double)clip_low), log1p((double)clip_high),
                         adv_per_token, by_sequence};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // up to this many tokens each CTA counts them for itself, while its row is on its way, which saves a launch
+  // Few tokens: each CTA counts them for itself while its row is on its way, which saves two launches (2 x 512 rows of
+  // 100 KB 51.6 / 55.1 us with and without, 2 x 600 of 14 KB 23.6 / 21.2; for 256 sequences of one token, a warp a
+  // sequence, 30.1 / 21.7).
   const long long rows = (long long)B * T;
-  const bool warps = lp_warps(rows, V, dtype);
-  const int count_here = rows <= 2048 && !warps ? 1 : 0;
+  const int count_here = rows <= 1024 && (!by_sequence || B <= 32) ? 1 : 0;
+  const bool warps = !count_here && lp_warps(rows, V, dtype);
   int* total = count_here ? nullptr : reinterpret_cast<int*>(stats);  // kept there until the statistics replace it
   if (!count_here) {
     const int by_warp = T <= 128 ? 1 : 0;
@@ -1174,22 +1179,23 @@ extern "C" int rgpt_policy_loss(const void* logits, int dtype, long long sb, lon
   lp_dispatch(dtype, [&](auto* tag) {
     using E = std::remove_pointer_t<decltype(tag)>;
     const LpRows lr = {sb, st, T}, dr = {db, dt, T};
-    const PolicyRows p = {labels, ignore_index, old_logps, ref_logps, advantages, counts, total, B, count_here, a, token_logps, lse, coef};
-    const unsigned M = (unsigned)((long long)B * T);
-    const int c = lp_parts(M, V, dtype);
+    const PolicyRows p = {labels, ignore_index, old_logps,  ref_logps, advantages,  counts, total,
+                          B,      count_here,   a,          token_logps, lse,       coef};
+    const int c = lp_parts(rows, V, dtype);
     if (lp_long(V, dtype)) {
       auto kern = c > 1 ? policy_staged_kernel<E, LP_CLUSTER> : policy_staged_kernel<E, LP_CTA>;
       static bool set[2][64] = {};
       if ((rc = lp_smem(kern, POL_SMEM, set[c > 1])) == RGPT_OK)
-        launch_pdl(kern, dim3(M * c), dim3(LP_THREADS), POL_SMEM, s, c, (const E*)logits, lr, V, p, (E*)dlogits, dr);
+        launch_pdl(kern, dim3((unsigned)(rows * c)), dim3(LP_THREADS), POL_SMEM, s, c, (const E*)logits, lr, V, p, (E*)dlogits, dr);
       return;
     }
-    launch_pdl(warps ? policy_kernel<E, LP_WARP> : c > 1 ? policy_kernel<E, LP_CLUSTER> : policy_kernel<E, LP_CTA>,
-               lp_grid(M, V, dtype, c), dim3(LP_THREADS), 0, s, c, (const E*)logits, lr, V, p, (E*)dlogits, dr, (long long)M);
+    launch_pdl(warps ? policy_kernel<E, LP_WARP> : policy_kernel<E, LP_CTA>, lp_grid(rows, warps, 1), dim3(LP_THREADS), 0, s,
+               1, (const E*)logits, lr, V, p, (E*)dlogits, dr, rows);
   });
   if (rc) return rc;
   const int ctas = rows > 8192 ? 8 : 1;
-  launch_pdl(policy_stats_kernel, dim3(ctas), dim3(rows < 1024 ? (unsigned)((rows + 31) / 32 * 32) : 1024u), 0, s, ctas, (const float*)token_logps, labels, ignore_index, V, B, T,
-             old_logps, ref_logps, advantages, a, (const int*)counts, (const int*)total, stats);
+  const unsigned threads = rows < 1024 ? (unsigned)((rows + 31) / 32 * 32) : 1024u;
+  launch_pdl(policy_stats_kernel, dim3(ctas), dim3(threads), 0, s, ctas, (const float*)token_logps, labels, ignore_index, V,
+             B, T, old_logps, ref_logps, advantages, a, (const int*)counts, (const int*)total, stats);
   return rgpt_check_launch("policy_loss kernels");
 }

@@ -201,9 +201,9 @@ class GPT(nn.Module):
     @torch.no_grad()
     def token_logprobs(self, input_ids, labels):
         """Log-probability of each label [B, T] (fp32; 0 where labels == pad_token_id or outside the vocabulary), e.g. of
-        a frozen reference or of the policy that sampled them (dropout, if any, follows the module's mode). The logits are never stored:
-        the lm_head GEMM keeps each row's sum of exponentials. They are rounded to bf16 as the stored logits of
-        forward / preference_loss / policy_loss are, so the same weights give the same log-probabilities."""
+        a frozen reference or of the policy that sampled them (dropout, if any, follows the module's mode). The logits
+        are never stored: the lm_head GEMM keeps each row's sum of exponentials. They are rounded to bf16 as the stored
+        logits of forward / preference_loss / policy_loss are, so the same weights give the same log-probabilities."""
         eng = self.engine()
         A = eng.forward(input_ids, None, training=False, want_loss=False, head=False)
         lab = labels.reshape(-1).long().contiguous()

@@ -537,6 +537,11 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
              kernels=2 + (P * T > 512) + (dlogits is not None))
 
 
+def _policy_kernels(B: int, T: int, by_sequence: bool) -> int:
+    """Launches of policy_loss: few tokens are counted by the row kernel, others by two kernels of their own."""
+    return 2 if B * T <= 1024 and (not by_sequence or B <= 32) else 4
+
+
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Tensor, advantages: torch.Tensor,
                 ref_logps: torch.Tensor | None = None, *, token_logps: torch.Tensor, counts: torch.Tensor,
                 stats: torch.Tensor, lse: torch.Tensor | None = None, coef: torch.Tensor | None = None,
@@ -559,7 +564,7 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
     if p is not None:
         return _call_on(p[20], "rgpt_policy_loss", *p[:8], int(ignore_index), *p[8:12], float(clip_low),
                         float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *p[12:20],
-                        kernels=2 + 2 * (p[4] * p[5] > 2048))
+                        kernels=_policy_kernels(p[4], p[5], by_sequence))
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     dev, shape, f32 = logits.get_device(), logits.shape[:-1], torch.float32
     per_token = advantages.shape != (B,)
@@ -573,7 +578,7 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
         raise ValueError(f"policy_loss needs at least one token, got logits {tuple(logits.shape)}")
     _call_on(dev, "rgpt_policy_loss", logits.data_ptr(), dt, sb, st, B, T, V, *ins, adv, int(per_token), float(clip_low),
              float(clip_high), float(kl_coef), int(bool(by_sequence)), float(grad_scale), *outs, *grad,
-             kernels=2 + 2 * (B * T > 2048))
+             kernels=_policy_kernels(B, T, by_sequence))
 
 
 def _linear_operands(x: torch.Tensor, w: torch.Tensor):
@@ -616,7 +621,7 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
     if part is None:
         part = torch.empty(need, device=x.device, dtype=torch.float32)
     _call_on(dev, "rgpt_linear_logprobs", x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), M, V, K, lab, int(ignore_index),
-             int(bool(round_bf16)), part.data_ptr(), part.numel(), *outs)
+             int(bool(round_bf16)), part.data_ptr(), part.numel(), *outs, kernels=2)
 
 
 # Gradient rows of linear_logprobs_bwd in flight: at most this many bf16 logit gradients (1 GiB) at a time.
@@ -634,10 +639,15 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
     for t, n, dtype in ((labels, "labels", torch.int64), (lse, "lse", torch.float32), (dlogps, "dlogps", torch.float32)):
         _flat(t, n, (M,), dtype, x.get_device())
     for t, n, shape in ((dx, "dx", (M, K)), (dw, "dw", (V, K))):
-        if t is not None and (tuple(t.shape) != shape or t.dtype not in (torch.bfloat16, torch.float32)
-                              or t.stride(1) != 1 or t.stride(0) % 8 or t.device != dev):
+        if t is None:
+            continue
+        if (tuple(t.shape) != shape or t.dtype not in (torch.bfloat16, torch.float32) or t.stride(1) != 1
+                or t.stride(0) % 8 or t.stride(0) < K or t.device != dev):
             raise ValueError(f"{n} must be a bf16 or fp32 {shape} tensor with unit column stride and a row stride that is"
                              f" a multiple of 8")
+        for o in (x, w):  # both are read until the end
+            if t.numel() and o.numel() and t.data_ptr() < _end(o) and o.data_ptr() < _end(t):
+                raise ValueError(f"{n} must share no memory with x and w")
     if chunk_rows is not None and chunk_rows < 1:
         raise ValueError("linear_logprobs_bwd: chunk_rows must be at least 1")
     if M == 0:

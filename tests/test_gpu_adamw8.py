@@ -135,6 +135,24 @@ def test_all_codes_round_trip(cuda):
     assert torch.equal(back[2], q.cpu()) and back[3].item() == 1.0
 
 
+def test_a_gradient_that_is_not_finite_stays_in_its_block(cuda):
+    n = 5000
+    runs = []
+    for bad in (None, float("inf"), float("nan")):
+        p = torch.nn.Parameter(0.02 * torch.randn(n, generator=torch.Generator().manual_seed(1)).cuda())
+        opt = Muon([{"params": [p], "use_muon": False}], lr=1e-3, adam_state_bits=8)
+        for step in range(3):
+            p.grad = gradients(n, step).cuda()
+            if step == 1 and bad is not None:
+                p.grad[700] = bad
+            opt.step()
+        runs.append((p.detach().clone(), *opt.adam_moments(p)))
+    for run in runs[1:]:
+        assert run[0][700].isnan()
+        for a, b in zip(run, runs[0]):
+            assert torch.equal(a[:512], b[:512]) and torch.equal(a[768:], b[768:])
+
+
 def test_near_adamw_with_fp32_moments(cuda):
     """Twenty steps on gradients of one scale. A code is within 2^-4 (first moment) of a value that is not far below its
     block's largest; the update divides by sqrt(v), whose code is within 2^-6. So an update is off by about 8% at most

@@ -291,6 +291,8 @@ POLICY = [
     dict(B=2, T=160, V=8203, dtype=torch.float16, by_sequence=True, kl=0.1, empty=True),
     dict(B=400, T=1, V=33000, dtype=torch.float16, layout="padded"),
     dict(B=1, T=310, V=70001, dtype=torch.float32, per_token=True),
+    dict(B=300, T=2, V=130, dtype=torch.bfloat16, kl=0.1, by_sequence=True),
+    dict(B=33, T=9, V=20000, dtype=torch.bfloat16, by_sequence=True, empty=True),
     dict(B=9000, T=1, V=64, dtype=torch.bfloat16, kl=0.1, by_sequence=True),
     dict(B=40, T=300, V=1201, dtype=torch.float16, kl=0.05, by_sequence=True, empty=True),
 ]

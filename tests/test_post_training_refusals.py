@@ -115,6 +115,11 @@ def test_linear_logprobs_refuses_types_scratch_and_outputs():
         nv.linear_logprobs_bwd(x, w, y, o, o, z(4, 9), None)
     with pytest.raises(ValueError, match="dw"):
         nv.linear_logprobs_bwd(x, w, y, o, o, None, z(9, 8, dt=torch.float16))
+    for dx, dw in ((x, None), (None, w)):
+        with pytest.raises(ValueError, match="share no memory"):
+            nv.linear_logprobs_bwd(x, w, y, o, o, dx, dw)
+    with pytest.raises(ValueError, match="row stride"):
+        nv.linear_logprobs_bwd(x, w, y, o, o, z(1, 8).expand(4, 8), None)
     with pytest.raises(ValueError, match="chunk_rows"):
         nv.linear_logprobs_bwd(x, w, y, o, o, None, None, chunk_rows=0)
 
