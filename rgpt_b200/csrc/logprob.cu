@@ -526,9 +526,10 @@ __device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, voi
 }
 
 // ---------------------------------------------------------------------------- token log-probabilities
-// Forward for long rows: one CTA a row (or a share of it), 24 KB of it in flight; nine small CTAs an SM, each in its own
-// phase, keep the copies and the exponentials going at the same time (4092 rows of 50304 bf16 logits, 2492 of them
-// scored: 44 us, 5.7 TB/s, as without the exponentials; four CTAs of 256 threads 51 us; loads into registers 55 us).
+// Forward for long rows: one CTA a row (or a share of it), 24 KB of it in flight; eight small CTAs an SM, each in its
+// own phase, keep the copies and the exponentials going at the same time (4092 rows of 50304 bf16 logits, 2492 of them
+// scored: 46 us, 5.4 TB/s; 43 without the exponentials; twice the piece 52, half of it 52; four CTAs of 256 threads an
+// SM 7 us more, loads into registers 11 more).
 constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512, LP_FWD_SLOTS = 3;
 constexpr uint32_t LP_FWD_SMEM = LP_FWD_SLOTS * LP_FWD_VECS * 16u;
 template <typename E, int W>
