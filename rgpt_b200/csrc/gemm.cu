@@ -53,6 +53,7 @@ struct GemmShape {
   int group_m;  // row tiles per visiting group (see decode_unit)
   int bn;       // columns of a tile: BN, or for LSE_F32 any multiple of 16 up to it
   int am;       // rows of A that a tile loads: all 128, or for LSE_F32 those that exist, rounded up to 8
+  int hold_a;   // LSE_F32: A stays in shared memory (see HOLD_KB)
 };
 
 struct EpiParams {
@@ -114,14 +115,19 @@ __host__ __device__ constexpr int epi_c_bytes(int epi) {
   return (epi == RGPT_EPI_RESID_F32 || epi == RGPT_EPI_POLY_F32) ? 4 : 2;
 }
 
-template <int BN, int STAGES, bool PAIR, int EW>
+// A held in shared memory (HOLD): with HOLD_MIN_KB to HOLD_KB k-blocks, a CTA's rows of A stay for all column tiles of a
+// row tile, and the ring carries B alone.
+constexpr int HOLD_KB = 8, HOLD_MIN_KB = 6;
+
+template <int BN, int STAGES, bool PAIR, int EW, bool HOLD = false>
 struct GemmSmem {
   static constexpr uint32_t A_BYTES = GEMM_BM * GEMM_BK * 2;              // this CTA's 128 rows of A
   static constexpr uint32_t B_BYTES = (PAIR ? BN / 2 : BN) * GEMM_BK * 2;  // a CTA pair splits B's rows
-  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr uint32_t STAGE_BYTES = HOLD ? B_BYTES : A_BYTES + B_BYTES;
+  static constexpr uint32_t HELD_BYTES = HOLD ? HOLD_KB * A_BYTES : 0;
   static constexpr uint32_t EPI_BYTES = EW * 2 * EPI_STAGE_BYTES;  // 2 staging buffers per epilogue warp
   static constexpr uint32_t BAR_BYTES = 512;
-  static constexpr uint32_t TOTAL = STAGES * STAGE_BYTES + EPI_BYTES + BAR_BYTES + 1024;  // +1024 alignment slack
+  static constexpr uint32_t TOTAL = HELD_BYTES + STAGES * STAGE_BYTES + EPI_BYTES + BAR_BYTES + 1024;  // +1024 alignment slack
 };
 
 // 16 bytes of global memory through L1 (the epilogue's C rows: a row's 128-byte chunk is read
@@ -202,14 +208,15 @@ __device__ __forceinline__ void act_bwd32(float* v, const uint4* c) {
     }
   }
 }
-template <int BN, int STAGES, int A_MN, int B_MN, int EPI, bool PAIR, int ACT>
+template <int BN, int STAGES, int A_MN, int B_MN, int EPI, bool PAIR, int ACT, bool HOLD>
 __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
     gemm_bf16_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmD2,
                         GemmShape sh, EpiParams ep) {
   constexpr bool reads_c = epi_reads_c(EPI);
   constexpr int EW = gemm_epi_warps(EPI);
-  using L = GemmSmem<BN, STAGES, PAIR, gemm_staging_warps(EPI)>;
+  static_assert(!HOLD || !A_MN, "A is held K-major");
+  using L = GemmSmem<BN, STAGES, PAIR, gemm_staging_warps(EPI), HOLD>;
   constexpr int NUM_ACC = 512 / BN;  // TMEM accumulator buffers (2 for 256-wide tiles, 4 for 128-wide)
   constexpr uint32_t TMEM_COLS = NUM_ACC * BN;
   constexpr int TILE_M = PAIR ? 2 * GEMM_BM : GEMM_BM;
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * L::A_BYTES;
+  uint8_t* sB = smem + (HOLD ? HOLD_KB : STAGES) * L::A_BYTES;
   uint8_t* sEpi = sB + STAGES * L::B_BYTES;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sEpi + L::EPI_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
@@ -234,8 +241,11 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_ctarank() : 0;  // 0 = the CTA that issues the pair's MMAs
-  const int first_unit = PAIR ? (int)cluster_id_x() : (int)blockIdx.x;
-  const int unit_step = PAIR ? (int)cluster_count_x() : (int)gridDim.x;
+  const int team = PAIR ? (int)cluster_id_x() : (int)blockIdx.x, teams = PAIR ? (int)cluster_count_x() : (int)gridDim.x;
+  // units are dealt out in turn, or with A held as one run each: the column tiles of one row tile after another
+  const int first_unit = HOLD ? (int)((long long)sh.num_units * team / teams) : team;
+  const int end_unit = HOLD ? (int)((long long)sh.num_units * (team + 1) / teams) : sh.num_units;
+  const int unit_step = HOLD ? 1 : teams;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int u = first_unit; u < sh.num_units && ok; u += unit_step) {
+      for (int u = first_unit; u < end_unit && ok; u += unit_step) {
         int b, mt, nt, ks;
         decode_unit(u, sh, b, mt, nt, ks);
         const int kb0 = ks * sh.kb_per_split;
@@ -298,7 +308,11 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
         };
         const int a_sub = a_subs(rank), b_sub = b_subs(rank);
         const int a_row = mt * TILE_M + rank * GEMM_BM, b_row = nt * bn + rank * B_ROWS;
-        const uint32_t expect = PAIR ? stage_bytes(0) + stage_bytes(1) : stage_bytes(0);
+        // A is loaded again for a new row tile only. The slot that a step waits for was freed by the step STAGES before
+        // it; MMAs complete in order, so the held block that the step overwrites, last read num_kb >= STAGES steps
+        // before (the launch sees to that), is free as well.
+        const bool load_a = !HOLD || u == first_unit || nt == 0;
+        const uint32_t expect = !load_a ? (PAIR ? 2 : 1) * L::B_BYTES : PAIR ? stage_bytes(0) + stage_bytes(1) : stage_bytes(0);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag)) {
             ok = false;
@@ -307,7 +321,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
           // the pair's barrier lives in CTA 0, which posts the byte count of both CTAs' loads
           if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], expect);
           const int k0 = kb * GEMM_BK;
-          uint8_t* a_dst = sA + stage * L::A_BYTES;
+          uint8_t* a_dst = sA + (HOLD ? kb : stage) * L::A_BYTES;
           uint8_t* b_dst = sB + stage * L::B_BYTES;
           const uint32_t fb = full_bar0 + stage * 8;
           auto load = [&](uint8_t* dst, const CUtensorMap* map, int c0, int c1) {
@@ -316,7 +330,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
           };
           if (A_MN) {
             for (int i = 0; i < a_sub; ++i) load(a_dst + i * (64 * GEMM_BK * 2), &tmA, a_row + i * 64, k0);
-          } else {
+          } else if (load_a) {
             load(a_dst, &tmA, k0, a_row);
           }
           if (B_MN) {
@@ -355,7 +369,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
           umma_commit(bar);
         }
       };
-      for (int u = first_unit; u < sh.num_units && ok; u += unit_step) {
+      for (int u = first_unit; u < end_unit && ok; u += unit_step) {
         int b, mt, nt, ks;
         decode_unit(u, sh, b, mt, nt, ks);
         const int kb0 = ks * sh.kb_per_split;
@@ -369,7 +383,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(sA + stage * L::A_BYTES);
+          const uint32_t a_addr = smem_u32(sA + (HOLD ? kb : stage) * L::A_BYTES);
           const uint32_t b_addr = smem_u32(sB + stage * L::B_BYTES);
 #pragma unroll
           for (int kk = 0; kk < GEMM_BK / 16; ++kk) {
@@ -448,7 +462,7 @@ __global__ void __launch_bounds__(gemm_threads(gemm_epi_warps(EPI)), 1)
         }
       }
     };
-    for (int u = first_unit; u < sh.num_units; u += unit_step) {
+    for (int u = first_unit; u < end_unit; u += unit_step) {
       int b, mt, nt, ks;
       decode_unit(u, sh, b, mt, nt, ks);
       const int row0 = mt * TILE_M + rank * GEMM_BM + quarter * 32;  // first output row of this warp
@@ -796,22 +810,23 @@ int make_tmap_bf16_3d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_
 }
 
 // Operand stages that fit beside EW warps' staging buffers (at most `want`).
-template <int BN, bool PAIR, int EW>
+template <int BN, bool PAIR, int EW, bool HOLD>
 constexpr int gemm_fit_stages(int want) {
-  using L1 = GemmSmem<BN, 1, PAIR, EW>;
-  const int fit = (int)((232448u - L1::EPI_BYTES - L1::BAR_BYTES - 1024u) / L1::STAGE_BYTES);
+  using L1 = GemmSmem<BN, 1, PAIR, EW, HOLD>;
+  const int fit = (int)((232448u - L1::HELD_BYTES - L1::EPI_BYTES - L1::BAR_BYTES - 1024u) / L1::STAGE_BYTES);
   return fit < want ? fit : want;
 }
 
-template <int BN, int STAGES_IN, int A_MN, int B_MN, int EPI, bool PAIR, int ACT = ACT_NONE>
+template <int BN, int STAGES_IN, int A_MN, int B_MN, int EPI, bool PAIR, int ACT = ACT_NONE, bool HOLD = false>
 static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const CUtensorMap& td2,
                        const GemmShape& sh, const EpiParams& ep, cudaStream_t stream, int dev) {
   constexpr int EW = gemm_epi_warps(EPI);
   constexpr int SW = gemm_staging_warps(EPI);
-  constexpr int STAGES = gemm_fit_stages<BN, PAIR, SW>(SW == 0 ? STAGES_IN + 2 : STAGES_IN);
+  constexpr int STAGES = gemm_fit_stages<BN, PAIR, SW, HOLD>(SW == 0 ? STAGES_IN + 2 : STAGES_IN);
   constexpr int THREADS = gemm_threads(EW);
-  auto kern = gemm_bf16_tc_kernel<BN, STAGES, A_MN, B_MN, EPI, PAIR, ACT>;
-  constexpr uint32_t smem = GemmSmem<BN, STAGES, PAIR, SW>::TOTAL;
+  auto kern = gemm_bf16_tc_kernel<BN, STAGES, A_MN, B_MN, EPI, PAIR, ACT, HOLD>;
+  constexpr uint32_t smem = GemmSmem<BN, STAGES, PAIR, SW, HOLD>::TOTAL;
+  static_assert(!HOLD || STAGES <= HOLD_MIN_KB, "a held block must be free when its slot is");
   static_assert(smem <= 232448, "GEMM shared memory exceeds the per-CTA limit");
   static bool attr_set[64] = {false};
   static int max_clusters[64] = {0};
@@ -888,6 +903,9 @@ static int dispatch_epi(int epi, const CUtensorMap& ta, const CUtensorMap& tb, c
     case RGPT_EPI_LSE_F32:
     case RGPT_EPI_SOFTMAX_GRAD_BF16:
       if constexpr (A_MN == 0 && B_MN == 0) {  // their entry points take K-major operands only
+        if constexpr (PAIR)
+          if (epi == RGPT_EPI_LSE_F32 && sh.hold_a)
+            return launch_gemm<BN, STAGES, 0, 0, RGPT_EPI_LSE_F32, true, ACT_NONE, true>(ta, tb, td, td2, sh, ep, s, dev);
         return epi == RGPT_EPI_LSE_F32
                    ? launch_gemm<BN, STAGES, 0, 0, RGPT_EPI_LSE_F32, PAIR>(ta, tb, td, td2, sh, ep, s, dev)
                    : launch_gemm<BN, STAGES, 0, 0, RGPT_EPI_SOFTMAX_GRAD_BF16, PAIR>(ta, tb, td, td2, sh, ep, s, dev);
@@ -1088,7 +1106,13 @@ static int gemm_entry(const void* A, int a_mn_major, long long lda, long long a_
   // column by column over ALL row tiles instead: A stays in L2 and B streams through once, where
   // groups of 8 row tiles would read the 51 MB lm_head weight once per group (m_tiles / 8 times).
   sh.group_m = GROUP_M;
-  if (sh.n_tiles >= 64 && (long long)M * K * 2 <= (32LL << 20)) sh.group_m = sh.m_tiles;
+  // LSE_F32 has no staging buffers, so up to 8 k-blocks of A fit beside a ring of B: each CTA pair then sweeps the column
+  // tiles of one row tile after another and loads half as much. B is read from L2 by pairs that are at different columns,
+  // so it has to fit there. Us, dealt out in turn / A held: 16368 x 50304, K 512 675 / 636, K 384 594 / 565; 2048 x 50304
+  // 93.5 / 90.9; 8192 x 65536 (64 MB of B) 442 / 436, 8192 x 80000 539 / 556, 8192 x 100000 673 / 724.
+  sh.hold_a = lsx && pair && sh.num_kb >= HOLD_MIN_KB && sh.num_kb <= HOLD_KB && (long long)N * K * 2 <= (64LL << 20);
+  if (sh.hold_a) sh.group_m = 1;
+  else if (sh.n_tiles >= 64 && (long long)M * K * 2 <= (32LL << 20)) sh.group_m = sh.m_tiles;
 
   // Operand maps. K-major: (inner=K, outer=rows); MN-major: (inner=rows, outer=K).
   CUtensorMap ta, tb, td, td2;

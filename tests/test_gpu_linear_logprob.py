@@ -43,7 +43,9 @@ def ref(x, w, labels):
 
 
 SHAPES = [(1, 1, 8, 0), (1, 50304, 512, 0), (3, 130, 64, 0), (16, 50257, 512, 0), (128, 129, 72, 8), (257, 1000, 1024, 0),
-          (300, 4097, 128, 64), (1000, 383, 512, 0), (513, 33000, 1032, 0), (5000, 300, 64, 0)]
+          (300, 4097, 128, 64), (1000, 383, 512, 0), (513, 33000, 1032, 0), (5000, 300, 64, 0),
+          # many tiles of K from 6 to 8 blocks of 64 (hidden states kept on chip), and one block less
+          (2100, 50304, 512, 0), (1601, 50257, 449, 7), (4500, 20001, 384, 8), (7000, 12800, 328, 0), (2100, 40000, 320, 0)]
 
 
 @pytest.mark.parametrize("M,V,K,stride", SHAPES)
@@ -59,7 +61,7 @@ def test_forward(cuda, M, V, K, stride):
     assert nv._lib.device_error() == 0
 
 
-@pytest.mark.parametrize("M,V,K", [(130, 1000, 64), (700, 50304, 512), (5, 50257, 512), (2100, 50304, 1024)])
+@pytest.mark.parametrize("M,V,K", [(130, 1000, 64), (700, 50304, 512), (5, 50257, 512), (2100, 50304, 1024), (2100, 50304, 512)])
 def test_rounded_products_give_what_stored_logits_give(cuda, M, V, K):
     """The same fp32 accumulators rounded the same way, so only the sums' own order differs."""
     x, w, labels = make(M, V, K)
