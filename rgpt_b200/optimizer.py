@@ -586,9 +586,9 @@ class Muon(torch.optim.Optimizer):
         ent = self._cache.get(key)
         if ent is None:
             dev = params[0].device
-            pieces = [(ti, s) for ti, p in enumerate(params) for s in range(0, p.numel(), _ADAM8_CHUNK)]
-            ent = (_table(rows, dev), torch.tensor([t for t, _ in pieces], dtype=torch.int32).to(dev),
-                   torch.tensor([s for _, s in pieces], dtype=torch.int64).to(dev))
+            starts = [torch.arange(0, p.numel(), _ADAM8_CHUNK) for p in params]
+            of = torch.cat([torch.full(s.shape, ti, dtype=torch.int32) for ti, s in enumerate(starts)])
+            ent = (_table(rows, dev), of.to(dev), torch.cat(starts).to(dev))
             self._cache[key] = ent
         table, ct, cs = ent
         return lambda: nv.adamw8(table, ct, cs, _ADAM8_CHUNK, lr, wd, beta1, beta2, eps, step_i, hp=self._hp(gi))
