@@ -447,14 +447,18 @@ struct LpStage {
   uint64_t* full;
   int n, pieces, slots, issued;
   bool ok;
-  __device__ __forceinline__ LpStage(const uint4* src_, int n_, void* smem, uint64_t* full_, int slots_)
+  const bool passing;  // its lines may leave L2 first
+  const uint64_t policy;
+  __device__ __forceinline__ LpStage(const uint4* src_, int n_, void* smem, uint64_t* full_, int slots_, bool passing_)
       : src(src_), place(reinterpret_cast<uint4*>(smem)), full(full_), n(n_), pieces((n_ + VECS - 1) / VECS),
-        slots(slots_), issued(0), ok(true) {}
+        slots(slots_), issued(0), ok(true), passing(passing_), policy(l2_evict_first()) {}
   __device__ __forceinline__ int size(int c) const { return min(VECS, n - c * VECS); }
   __device__ __forceinline__ void issue(int c) {  // thread 0
     const uint32_t bytes = 16u * (uint32_t)size(c);
     mbar_arrive_expect_tx(&full[c % slots], bytes);
-    bulk_load_1d(place + (c % slots) * VECS, src + (long long)c * VECS, bytes, &full[c % slots]);
+    uint4* at = place + (c % slots) * VECS;
+    if (passing) bulk_load_1d(at, src + (long long)c * VECS, bytes, &full[c % slots], policy);
+    else bulk_load_1d(at, src + (long long)c * VECS, bytes, &full[c % slots]);
     issued = c + 1;
   }
   // all threads, first
@@ -506,12 +510,12 @@ __device__ __forceinline__ void lp_add_piece(LpSum& sum, const uint4* v, int n) 
 
 // The sum of one row through shared memory, the same in every thread of its CTAs, all of which have read it on return.
 template <typename E, int W, int THREADS, int VECS, int SLOTS, typename F>
-__device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, LpRow* out,
-                                              F&& meanwhile) {
+__device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, bool passing,
+                                              LpRow* out, F&& meanwhile) {
   using L = LpType<E>;
   const int head = lp_head(x, V), nvec = (V - head) / L::VEC, rest = V - nvec * L::VEC;
   const int lo = sh.lo(nvec);
-  LpStage<VECS> st(reinterpret_cast<const uint4*>(x + head) + lo, sh.hi(nvec) - lo, smem, full, SLOTS);
+  LpStage<VECS> st(reinterpret_cast<const uint4*>(x + head) + lo, sh.hi(nvec) - lo, smem, full, SLOTS, passing);
   st.start();
   meanwhile();
   LpSum a;
@@ -526,11 +530,16 @@ __device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, voi
 }
 
 // ---------------------------------------------------------------------------- token log-probabilities
-// Forward for long rows: one CTA a row (or a share of it), 24 KB of it in flight; eight small CTAs an SM, each in its
+// Forward for long rows: one CTA a row (or a share of it), 16 KB of it in flight; eight small CTAs an SM, each in its
 // own phase, keep the copies and the exponentials going at the same time (4092 rows of 50304 bf16 logits, 2492 of them
-// scored: 46 us, 5.4 TB/s; 43 without the exponentials; twice the piece 52, half of it 52; four CTAs of 256 threads an
-// SM 7 us more, loads into registers 11 more).
-constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512, LP_FWD_SLOTS = 3;
+// scored: 46 us, 5.4 TB/s; 43 without the exponentials; a third slot 46, pieces of 4 KB 52, of 16 KB 46; four CTAs of 256
+// threads an SM 7 us more, loads into registers 11 more). Two slots, because an SM's split into shared memory and L1
+// outlasts the kernel: with three, the backward that follows at once finds little L1 to land its loads in (forward and
+// backward 162 us against 154; of 16368 rows 616 against 576).
+constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512, LP_FWD_SLOTS = 2;
+// Bytes of the last rows that the forward leaves to L2's usual care, the rows before them marked to go first: with the two
+// L2 halves that an SM's loads may go through, more than this does not stay (60 to 100 MB: 154 -> 150 us).
+constexpr unsigned long long LP_KEEP_BYTES = 80ull << 20;
 constexpr uint32_t LP_FWD_SMEM = LP_FWD_SLOTS * LP_FWD_VECS * 16u;
 template <typename E, int W>
 __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E* __restrict__ logits, LpRows lr, int V,
@@ -559,7 +568,9 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
   const E* x = logits + lr.offset(row);
   const float xl = first ? L::get(x[label]) : 0.f;
   LpRow r;
-  lp_staged_sum<E, W, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, &r, [] {});
+  // a backward begins with the last rows (see logp_bwd_kernel): those before make room for them
+  const bool passing = (unsigned long long)(gridDim.x / sh.parts - 1 - row) * V * sizeof(E) > LP_KEEP_BYTES;
+  lp_staged_sum<E, W, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, passing, &r, [] {});
   if (first) {
     const double lp = lp_label(xl, r);
     logps[row] = (float)lp;
@@ -610,7 +621,7 @@ __global__ void __launch_bounds__(LP_THREADS) logp_bwd_kernel(const E* logits, L
   griddep_wait();
   griddep_launch();
   const LpShare sh = lp_share<W>();
-  // the last rows first: the forward has left them in L2 (4092 rows of 100 KB: forward and backward 176 -> 166 us)
+  // the last rows first: the forward has left them in L2 (4092 rows of 100 KB: forward and backward 10 us less)
   const long long row = M - 1 - lp_row<W>(sh);
   if (row < 0) return;  // whole warps
   const long long label = labels[row];
@@ -934,7 +945,7 @@ __global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logi
   const float xl = L::get(x[label]);
   LpRow r;
   int2 n;
-  lp_staged_sum<E, W, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, &r, [&] {
+  lp_staged_sum<E, W, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, false, &r, [&] {
     n = policy_counts(p, lr, V, row, sh.part == 0, red);  // while the first pieces are on their way
   });
   if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
