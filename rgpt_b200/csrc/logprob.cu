@@ -278,14 +278,17 @@ __device__ __forceinline__ float2 lp_join(float2 a, LpShare sh, MERGE&& merge) {
   return r;
 }
 
+// M ln2 + log(s) for a normal s: log(s) from the mantissa in [0.75, 1.5) in fp32 (absolute error 2^-25) and the exponent
+// in fp64
+__device__ __forceinline__ double lp_log(double M, float s) {
+  constexpr double LN2 = 0.69314718055994530942;
+  const int e = (int)((__float_as_uint(s) - 0x3F400000u) & 0xFF800000u) >> 23;
+  const float f = __uint_as_float(__float_as_uint(s) - ((uint32_t)e << 23));
+  return fma(M + (double)e, LN2, (double)logf(f));
+}
 // The finished row from its joined (M, s).
 __device__ __forceinline__ LpRow lp_finish(float2 r) {
-  // lse = ln2 (M + log2 s); log(s) from the mantissa in [0.75, 1.5) in fp32 (absolute error 2^-25) and the exponent in fp64
-  constexpr double LN2 = 0.69314718055994530942;
-  const int e = (int)((__float_as_uint(r.y) - 0x3F400000u) & 0xFF800000u) >> 23;
-  const float f = __uint_as_float(__float_as_uint(r.y) - ((uint32_t)e << 23));
-  const double M = (double)r.x;
-  return LpRow{0.f, r.x, 1.f / r.y, fma(M + (double)e, LN2, (double)logf(f) - LP_EX2_MEAN)};
+  return LpRow{0.f, r.x, 1.f / r.y, lp_log((double)r.x, r.y) - LP_EX2_MEAN};
 }
 // The label's log-probability; rounding may not make a sure label more than sure.
 __device__ __forceinline__ double lp_label(float xl, const LpRow& r) {
@@ -300,11 +303,15 @@ __device__ __forceinline__ bool lp_plain(float2 r) {
 template <typename E, typename J>
 __device__ __noinline__ LpRow lp_careful(const E* x, int V, int t, int n, J join) {
   float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
   for (int j = t; j < V; j += n) top = fmaxf(top, LpType<E>::get(x[j]));
   const float ref = lp_ref(join(make_float2(top, 0.f), true).x);
+#pragma unroll 1
   for (int j = t; j < V; j += n) sum += ex2_approx((LpType<E>::get(x[j]) - ref) * LP_LOG2E);
   sum = join(make_float2(sum, 0.f), false).x;
-  return LpRow{ref, 0.f, 1.f / sum, (double)ref + log((double)sum)};
+  // a sum of 0 (nothing but -inf) gives -inf, an infinite or NaN one itself
+  const double l = sum > 0.f && sum < INFINITY ? lp_log(0.0, sum) : sum == 0.f ? -INFINITY : (double)sum;
+  return LpRow{ref, 0.f, 1.f / sum, (double)ref + l};
 }
 __device__ __forceinline__ float2 lp_merge(float2 p, float2 q) {
   LpSum t;
@@ -375,6 +382,33 @@ __device__ __forceinline__ void lp_at_label(F2 (&f)[L::VEC / 2], int at, float c
   for (int k = 0; k < L::VEC / 2; ++k) f[k] = f2_add(f[k], f2(2 * k == at ? coef : 0.f, 2 * k + 1 == at ? coef : 0.f));
 }
 
+// A vector of the gradient; the label is its element `at`.
+template <typename E>
+__device__ __forceinline__ uint4 lp_grad_vec(const uint4& u, int at, float coef, const LpProb& prob) {
+  using L = LpType<E>;
+  F2 f[L::VEC / 2];
+  L::unpack(u, f);
+#pragma unroll
+  for (int k = 0; k < L::VEC / 2; ++k) f[k] = prob(f[k]);
+  if (at >= 0 && at < L::VEC) lp_at_label<L>(f, at, coef);
+  return L::pack(f);
+}
+// Its elements i = from, from + step .. of those outside the vectors: `head` before them, then the ones behind.
+template <typename E>
+__device__ __forceinline__ void lp_write_rest(const E* x, E* d, int label, float coef, int head, int vec_elems, int from,
+                                              int to, int step, const LpProb& prob) {
+  using L = LpType<E>;
+  for (int i = from; i < to; i += step) {
+    const int j = i < head ? i : i + vec_elems;
+    const float g = prob.one(L::get(x[j]));
+    d[j] = L::put(j == label ? g + coef : g);
+  }
+}
+template <typename E>
+__device__ __forceinline__ bool lp_aligned(const E* x, const E* d) {
+  return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+}
+
 // This CTA's share of coef * ([j = label] - p(x_j)) over one row; prob gives -coef * p. d may be x: each thread reads
 // an element before it writes the same one. LAST: nobody reads the row after this, so its lines may leave L2 first.
 template <typename E, int W, bool LAST>
@@ -382,18 +416,10 @@ __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label
                                               const LpProb& prob) {
   using L = LpType<E>;
   constexpr int N = lp_size<W>(LP_THREADS);
-  const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
-  const int head = vec ? lp_head(x, V) : V, nvec = (V - head) / L::VEC;
+  const int head = lp_aligned(x, d) ? lp_head(x, V) : V, nvec = (V - head) / L::VEC;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   uint4* dv = reinterpret_cast<uint4*>(d + head);
-  auto one = [&](const uint4& u, int at) {
-    F2 f[L::VEC / 2];
-    L::unpack(u, f);
-#pragma unroll
-    for (int k = 0; k < L::VEC / 2; ++k) f[k] = prob(f[k]);
-    if (at >= 0 && at < L::VEC) lp_at_label<L>(f, at, coef);
-    return L::pack(f);
-  };
+  auto one = [&](const uint4& u, int at) { return lp_grad_vec<E>(u, at, coef, prob); };
   int v = sh.lo(nvec) + lp_rank<W>();
   const int vend = sh.hi(nvec);
   if constexpr (W == LP_WARP) {  // short rows: one step takes most of them, its last vectors from some lanes only
@@ -417,11 +443,7 @@ __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label
   }
   for (; v < vend; v += N) dv[v] = one(xv[v], label - head - v * L::VEC);
   const int rest = V - nvec * L::VEC;
-  for (int i = sh.lo(rest) + lp_rank<W>(); i < sh.hi(rest); i += N) {
-    const int j = i < head ? i : i + nvec * L::VEC;
-    const float g = prob.one(L::get(x[j]));
-    d[j] = L::put(j == label ? g + coef : g);
-  }
+  lp_write_rest<E>(x, d, label, coef, head, nvec * L::VEC, sh.lo(rest) + lp_rank<W>(), sh.hi(rest), N, prob);
 }
 
 template <typename E, int W>
@@ -447,7 +469,7 @@ struct LpStage {
   uint64_t* full;
   int n, pieces, slots, issued;
   bool ok;
-  const bool passing;  // its lines may leave L2 first
+  bool passing;  // its lines may leave L2 first
   const uint64_t policy;
   __device__ __forceinline__ LpStage(const uint4* src_, int n_, void* smem, uint64_t* full_, int slots_, bool passing_)
       : src(src_), place(reinterpret_cast<uint4*>(smem)), full(full_), n(n_), pieces((n_ + VECS - 1) / VECS),
@@ -484,6 +506,26 @@ struct LpStage {
     __syncthreads();
     if (threadIdx.x == 0 && ok) issue(c + slots);
   }
+  // A second time through, from the last piece to the first: the last ones are still in their places, the others are
+  // brought in again, each into its place. Piece c comes as the place's use number (last + (last - c)) / slots, from 0,
+  // where last is the place's last piece.
+  __device__ __forceinline__ uint32_t back_parity(int c) const {
+    const int last = pieces - 1 - (pieces - 1 - c) % slots;
+    return (uint32_t)(last / slots + (last - c) / slots) & 1u;
+  }
+  __device__ __forceinline__ const uint4* wait_back(int c) {
+    if (c < pieces - slots && ok && !mbar_wait(&full[c % slots], back_parity(c), nullptr)) {
+      ok = false;
+      if (threadIdx.x == 0)
+        for (int i = c - 1; i > c - slots && i >= 0; --i) mbar_wait(&full[i % slots], back_parity(i), nullptr);
+    }
+    return place + (c % slots) * VECS;
+  }
+  __device__ __forceinline__ void next_back(int c) {
+    if (c - slots < 0) return;
+    __syncthreads();
+    if (threadIdx.x == 0 && ok) issue(c - slots);
+  }
 };
 
 // Adds a piece of n vectors to a thread's sum, U vectors at a time; lanes past the end of the last ones add -inf.
@@ -509,13 +551,17 @@ __device__ __forceinline__ void lp_add_piece(LpSum& sum, const uint4* v, int n) 
 }
 
 // The sum of one row through shared memory, the same in every thread of its CTAs, all of which have read it on return.
-template <typename E, int W, int THREADS, int VECS, int SLOTS, typename F>
-__device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, void* smem, uint64_t* full, bool passing,
-                                              LpRow* out, F&& meanwhile) {
+template <int VECS, typename E>
+__device__ __forceinline__ LpStage<VECS> lp_stage(const E* x, int V, LpShare sh, void* smem, uint64_t* full, int slots,
+                                                  bool passing) {
+  const int head = lp_head(x, V), nvec = (V - head) / LpType<E>::VEC, lo = sh.lo(nvec);
+  return LpStage<VECS>(reinterpret_cast<const uint4*>(x + head) + lo, sh.hi(nvec) - lo, smem, full, slots, passing);
+}
+template <typename E, int W, int THREADS, int VECS, typename F>
+__device__ __forceinline__ void lp_staged_sum(LpStage<VECS>& st, const E* x, int V, LpShare sh, LpRow* out,
+                                              F&& meanwhile) {
   using L = LpType<E>;
   const int head = lp_head(x, V), nvec = (V - head) / L::VEC, rest = V - nvec * L::VEC;
-  const int lo = sh.lo(nvec);
-  LpStage<VECS> st(reinterpret_cast<const uint4*>(x + head) + lo, sh.hi(nvec) - lo, smem, full, SLOTS, passing);
   st.start();
   meanwhile();
   LpSum a;
@@ -529,18 +575,55 @@ __device__ __forceinline__ void lp_staged_sum(const E* x, int V, LpShare sh, voi
   *out = lp_plain(q) ? lp_finish(q) : lp_team_careful<E, W, THREADS>(x, V, sh);
 }
 
+// lp_write_grad by the threads and from the stage of lp_staged_sum, for d of x's alignment (mod 16).
+template <typename E, int THREADS, int VECS>
+__device__ __forceinline__ void lp_staged_grad(LpStage<VECS>& st, const E* x, E* d, int V, int label, float coef,
+                                               LpShare sh, const LpProb& prob) {
+  using L = LpType<E>;
+  constexpr int U = 4;
+  static_assert(VECS % (U * THREADS) == 0, "a whole piece takes whole steps");
+  const int head = lp_head(x, V), nvec = (V - head) / L::VEC, rest = V - nvec * L::VEC, lo = sh.lo(nvec);
+  uint4* dv = reinterpret_cast<uint4*>(d + head) + lo;
+  st.passing = true;  // nobody reads the row after this
+  for (int c = st.pieces - 1; c >= 0; --c) {
+    const uint4* v = st.wait_back(c);
+    const int n = st.size(c), first = c * VECS;
+    auto one = [&](uint4 u, int i) {
+      __stcs(&dv[first + i], lp_grad_vec<E>(u, label - head - (lo + first + i) * L::VEC, coef, prob));
+    };
+    if (n == VECS) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < VECS; i += U * THREADS) {
+        uint4 u[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) u[k] = v[i + k * THREADS];
+#pragma unroll
+        for (int k = 0; k < U; ++k) one(u[k], i + k * THREADS);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n; i += THREADS) one(v[i], i);
+    }
+    st.next_back(c);
+  }
+  lp_write_rest<E>(x, d, label, coef, head, nvec * L::VEC, sh.lo(rest) + (int)threadIdx.x, sh.hi(rest), THREADS, prob);
+}
+
 // ---------------------------------------------------------------------------- token log-probabilities
-// Forward for long rows: one CTA a row (or a share of it), 16 KB of it in flight; eight small CTAs an SM, each in its
-// own phase, keep the copies and the exponentials going at the same time (4092 rows of 50304 bf16 logits, 2492 of them
-// scored: 46 us, 5.4 TB/s; 43 without the exponentials; a third slot 46, pieces of 4 KB 52, of 16 KB 46; four CTAs of 256
-// threads an SM 7 us more, loads into registers 11 more). Two slots, because an SM's split into shared memory and L1
-// outlasts the kernel: with three, the backward that follows at once finds little L1 to land its loads in (forward and
-// backward 162 us against 154; of 16368 rows 616 against 576).
-constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512, LP_FWD_SLOTS = 2;
+// Forward for long rows: one CTA a row (or a share of it), 16 KB of it in flight; nine small CTAs an SM, each in its own
+// phase, keep the copies and the exponentials going at the same time (4092 rows of 50304 bf16 logits, 2492 of them
+// scored: 45 us, 5.6 TB/s; some 3 less without the exponentials; pieces of 4 KB 52; four CTAs of 256 threads an SM 7 us
+// more, loads into registers 11 more). Two slots, because an SM's split into shared memory and L1 outlasts the kernel:
+// with three, the backward that follows at once finds little L1 to land its loads in (forward and backward 162 us against
+// 154; of 16368 rows 616 against 576).
+constexpr int LP_FWD_THREADS = 128, LP_FWD_VECS = 512;
+template <int W>
+constexpr int LP_FWD_SLOTS = W == LP_CLUSTER ? 4 : 2;  // few rows: SMs that are not full (8 x 131072 fp32 8.4 -> 7.8 us)
 // Bytes of the last rows that the forward leaves to L2's usual care, the rows before them marked to go first: with the two
 // L2 halves that an SM's loads may go through, more than this does not stay (60 to 100 MB: 154 -> 150 us).
 constexpr unsigned long long LP_KEEP_BYTES = 80ull << 20;
-constexpr uint32_t LP_FWD_SMEM = LP_FWD_SLOTS * LP_FWD_VECS * 16u;
+template <int W>
+constexpr uint32_t LP_FWD_SMEM = LP_FWD_SLOTS<W> * LP_FWD_VECS * 16u;
 template <typename E, int W>
 __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E* __restrict__ logits, LpRows lr, int V,
                                                                         const long long* __restrict__ labels,
@@ -550,7 +633,7 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
                                                                         double* __restrict__ wide) {
   using L = LpType<E>;
   extern __shared__ __align__(128) uint8_t lp_smem[];
-  __shared__ uint64_t full[LP_FWD_SLOTS];
+  __shared__ uint64_t full[LP_FWD_SLOTS<W>];
   griddep_wait();
   griddep_launch();
   const LpShare sh = lp_share<W>();
@@ -570,7 +653,8 @@ __global__ void __launch_bounds__(LP_FWD_THREADS) logp_fwd_staged_kernel(const E
   LpRow r;
   // a backward begins with the last rows (see logp_bwd_kernel): those before make room for them
   const bool passing = (unsigned long long)(gridDim.x / sh.parts - 1 - row) * V * sizeof(E) > LP_KEEP_BYTES;
-  lp_staged_sum<E, W, LP_FWD_THREADS, LP_FWD_VECS, LP_FWD_SLOTS>(x, V, sh, lp_smem, full, passing, &r, [] {});
+  auto st = lp_stage<LP_FWD_VECS>(x, V, sh, lp_smem, full, LP_FWD_SLOTS<W>, passing);
+  lp_staged_sum<E, W, LP_FWD_THREADS>(st, x, V, sh, &r, [] {});
   if (first) {
     const double lp = lp_label(xl, r);
     logps[row] = (float)lp;
@@ -914,11 +998,12 @@ __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpR
   lp_write_grad<E, W, true>(x, d, V, (int)label, coef, sh, LpProb(r.a, r.b, -coef * r.inv));
 }
 
-// The same for long rows, by one CTA each (or a share of it), the first read by bulk copies. The second read finds the
-// row in L2 as long as few rows are on their way: three CTAs an SM (16368 rows of 50304 bf16 logits, of which 15 in 16
-// are scored: 463 us, 5.6 TB/s; nine smaller CTAs some 90 us more, their rows fill L2; without the hint that the second
-// read is the last 60 us more). Holding the row in shared memory instead allows two rows an SM, too few to cover their
-// phases' latencies: 80 us more at best.
+// The same for long rows, by one CTA each (or a share of it), both reads by bulk copies. The second goes backwards: what
+// the first read last is still in shared memory (all of a share that fits three pieces), and the rest it finds in L2 as
+// long as few rows are on their way, four CTAs an SM. 16368 rows of 50304 bf16 logits, 10000 of them scored: 459 us, 5.8
+// TB/s; 465 with plain loads for the second read; pieces of 8 KB, two slots or four 470 to 490. 64 such rows, a cluster
+// of four CTAs each: 12.9 us, 14.0 with plain loads. Holding whole rows of this length allows two an SM, too few to cover
+// their phases' latencies: 90 us more at best.
 constexpr int POL_VECS = 1024, POL_SLOTS = 3;
 constexpr uint32_t POL_SMEM = POL_SLOTS * POL_VECS * 16u;
 template <typename E, int W>
@@ -945,13 +1030,17 @@ __global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logi
   const float xl = L::get(x[label]);
   LpRow r;
   int2 n;
-  lp_staged_sum<E, W, LP_THREADS, POL_VECS, POL_SLOTS>(x, V, sh, lp_smem, full, false, &r, [&] {
+  auto st = lp_stage<POL_VECS>(x, V, sh, lp_smem, full, POL_SLOTS, false);
+  lp_staged_sum<E, W, LP_THREADS>(st, x, V, sh, &r, [&] {
     n = policy_counts(p, lr, V, row, sh.part == 0, red);  // while the first pieces are on their way
   });
   if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
   if (!d) return;
   __syncthreads();
-  lp_write_grad<E, W, true>(x, d, V, (int)label, s_coef, sh, LpProb(r.a, r.b, -s_coef * r.inv));
+  const float coef = s_coef;
+  const LpProb prob(r.a, r.b, -coef * r.inv);
+  if (lp_aligned(x, d)) lp_staged_grad<E, LP_THREADS>(st, x, d, V, (int)label, coef, sh, prob);
+  else lp_write_grad<E, W, true>(x, d, V, (int)label, coef, sh, prob);
 }
 
 // stats = {loss, policy term, KL, clipped share}: weighted sums over the tokens, from their log-probabilities, by one CTA
@@ -1086,8 +1175,9 @@ static int launch_logp_fwd(const void* logits, int dtype, LpRows lr, long long M
     if (lp_long(V, dtype)) {
       auto kern = c > 1 ? logp_fwd_staged_kernel<E, LP_CLUSTER> : logp_fwd_staged_kernel<E, LP_CTA>;
       static bool set[2][64] = {};
-      if ((rc = lp_smem(kern, LP_FWD_SMEM, set[c > 1])) == RGPT_OK)
-        launch_pdl(kern, dim3((unsigned)(M * c)), dim3(LP_FWD_THREADS), LP_FWD_SMEM, s, c, (const E*)logits, lr, V, labels,
+      const uint32_t smem = c > 1 ? LP_FWD_SMEM<LP_CLUSTER> : LP_FWD_SMEM<LP_CTA>;
+      if ((rc = lp_smem(kern, smem, set[c > 1])) == RGPT_OK)
+        launch_pdl(kern, dim3((unsigned)(M * c)), dim3(LP_FWD_THREADS), smem, s, c, (const E*)logits, lr, V, labels,
                    ignore_index, logps, lse, wide);
       return;
     }
