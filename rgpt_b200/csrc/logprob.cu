@@ -777,47 +777,59 @@ __device__ __forceinline__ void pref_terms(const PrefArgs& a, double h, double* 
   }
 }
 
-// One CTA per pair: the two sequences' log-probabilities in fp64, the margin h and the sequences' coefficients
-// d loss / d (a scored token's log-probability). A single CTA takes all pairs when they are few and short, and their
-// mean, which saves a launch.
+// A pair a warp, or for long sequences a CTA: the two sequences' log-probabilities in fp64, the margin h and the sequences'
+// coefficients d loss / d (a scored token's log-probability). Where one CTA takes all pairs it writes their mean loss as
+// well, which saves a launch.
 __global__ void __launch_bounds__(256) pref_pair_kernel(const double* __restrict__ logps,
                                                         const long long* __restrict__ labels, long long ignore_index,
-                                                        int V, int P, int T, const float* __restrict__ ref, PrefArgs a,
-                                                        float* __restrict__ seq_logps, float* __restrict__ margins,
-                                                        float* __restrict__ coef, float* __restrict__ loss_out) {
+                                                        int V, int P, int T, int by_warp, const float* __restrict__ ref,
+                                                        PrefArgs a, float* __restrict__ seq_logps,
+                                                        float* __restrict__ margins, float* __restrict__ coef,
+                                                        float* __restrict__ loss_out) {
   griddep_wait();
   griddep_launch();
   __shared__ double red[8];
-  double mean = 0.0;
-  for (int p = blockIdx.x; p < P; p += gridDim.x) {
+  const int p = by_warp ? (int)(blockIdx.x * 8 + (threadIdx.x >> 5)) : (int)blockIdx.x;
+  const int step = by_warp ? 32 : 256, t0 = (int)threadIdx.x % step;
+  double pair_loss = 0.0;
+  if (p < P) {  // whole warps, or the whole CTA
     double s[2], n[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const long long base = (long long)(p + k * P) * T;
-      double v = 0.0, c = 0.0;
-      for (int t = threadIdx.x; t < T; t += blockDim.x) {
+      double v = 0.0;
+      int c = 0;
+      for (int t = t0; t < T; t += step) {
         v += logps[base + t];
-        if (a.average) c += lp_scored(labels[base + t], ignore_index, V) ? 1.0 : 0.0;
+        if (a.average) c += lp_scored(labels[base + t], ignore_index, V) ? 1 : 0;
       }
-      s[k] = lp_block_sum(v, red);
-      n[k] = a.average ? fmax(lp_block_sum(c, red), 1.0) : 1.0;
-      s[k] /= n[k];
+      if (by_warp) {
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        c = __reduce_add_sync(0xffffffffu, c);
+      } else {
+        v = lp_block_sum(v, red);
+        if (a.average) c = (int)lp_block_sum((double)c, red);
+      }
+      n[k] = a.average ? (double)max(c, 1) : 1.0;
+      s[k] = v / n[k];
     }
-    if (threadIdx.x != 0) continue;
-    double d = s[0] - s[1];
-    if (ref) d = (s[0] - (double)ref[p]) - (s[1] - (double)ref[p + P]);
-    const double h = (double)a.beta * d - (double)a.margin;
-    double loss, dh;
-    pref_terms(a, h, &loss, &dh);
-    dh *= (double)a.beta * (double)a.grad_scale / P;
-    seq_logps[p] = (float)s[0];
-    seq_logps[p + P] = (float)s[1];
-    margins[p] = (float)h;
-    coef[p] = (float)(dh / n[0]);
-    coef[p + P] = (float)(-dh / n[1]);
-    mean += loss;
+    if (t0 == 0) {
+      double d = s[0] - s[1];
+      if (ref) d = (s[0] - (double)ref[p]) - (s[1] - (double)ref[p + P]);
+      const double h = (double)a.beta * d - (double)a.margin;
+      double dh;
+      pref_terms(a, h, &pair_loss, &dh);
+      dh *= (double)a.beta * (double)a.grad_scale / P;
+      seq_logps[p] = (float)s[0];
+      seq_logps[p + P] = (float)s[1];
+      margins[p] = (float)h;
+      coef[p] = (float)(dh / n[0]);
+      coef[p + P] = (float)(-dh / n[1]);
+    }
   }
-  if (gridDim.x == 1 && threadIdx.x == 0) loss_out[0] = (float)(mean / P);
+  if (gridDim.x > 1) return;
+  const double mean = lp_block_sum(pair_loss, red);
+  if (threadIdx.x == 0) loss_out[0] = (float)(mean / P);
 }
 
 // mean of the pairs' losses, from their margins
@@ -1242,9 +1254,12 @@ extern "C" int rgpt_preference_loss(const void* logits, int dtype, long long sb,
   const long long M = 2ll * P * T;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if ((rc = launch_logp_fwd(logits, dtype, lr, M, V, labels, ignore_index, token_logps, lse, scratch, s))) return rc;
-  const unsigned pair_ctas = (long long)P * T <= 512 ? 1u : (unsigned)P;
+  // A warp a pair up to 256 tokens (all three or four launches, bf16, pairs x tokens x vocabulary: 8 x 16 x 1000 7.9 us,
+  // 512 x 1 x 256 10.7, 1 x 256 x 2048 10.8; one CTA going through the pairs 20.6, 833, 10.1; at 512 tokens 11.6 / 10.4).
+  const int by_warp = T <= 256 ? 1 : 0;
+  const unsigned pair_ctas = by_warp ? (unsigned)((P + 7) / 8) : (unsigned)P;
   launch_pdl(pref_pair_kernel, dim3(pair_ctas), dim3(256), 0, s, 1, (const double*)scratch, labels, ignore_index, V, P, T,
-             ref_logps, a, seq_logps, margins, coef, loss);
+             by_warp, ref_logps, a, seq_logps, margins, coef, loss);
   if (pair_ctas > 1) launch_pdl(pref_loss_kernel, dim3(1), dim3(256), 0, s, 1, margins, P, a, loss);
   if (dlogits &&
       (rc = launch_logp_bwd(logits, dtype, lr, M, V, labels, ignore_index, lse, coef, 1, dlogits, LpRows{db, dt, T}, s)))

@@ -491,6 +491,11 @@ def token_logprobs_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Te
     _call_on(dev, "rgpt_token_logprobs_bwd", logits.data_ptr(), dt, sb, st, B, T, V, *args, *grad)
 
 
+def _preference_kernels(P: int, T: int, dlogits: torch.Tensor | None) -> int:
+    """Launches of preference_loss: rows, pairs (a warp or a CTA each), their mean unless one CTA has them all, gradient."""
+    return 2 + (P > (8 if T <= 256 else 1)) + (dlogits is not None)
+
+
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
                     token_logps: torch.Tensor, lse: torch.Tensor, seq_logps: torch.Tensor, margins: torch.Tensor,
                     coef: torch.Tensor, loss: torch.Tensor, dlogits: torch.Tensor | None = None,
@@ -517,7 +522,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         pairs, T = p[4] // 2, p[5]
         return _call_on(p[19], "rgpt_preference_loss", *p[:4], pairs, *p[5:8], int(ignore_index), p[8],
                         PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
-                        float(grad_scale), *p[9:19], kernels=2 + (pairs * T > 512) + (dlogits is not None))
+                        float(grad_scale), *p[9:19], kernels=_preference_kernels(pairs, T, dlogits))
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
     if logits.dim() != 3 or B % 2 or B == 0 or T == 0 or V == 0:
         raise ValueError(f"preference_loss needs logits [2P, T, V] of at least one pair and token, got {tuple(logits.shape)}")
@@ -534,7 +539,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
     _call_on(dev, "rgpt_preference_loss", logits.data_ptr(), dt, sb, st, P, T, V, lab, int(ignore_index), ref,
              PREFERENCE_KINDS[kind], float(beta), float(margin), float(label_smoothing), int(bool(average)),
              float(grad_scale), *outs, scratch.data_ptr(), *grad,
-             kernels=2 + (P * T > 512) + (dlogits is not None))
+             kernels=_preference_kernels(P, T, dlogits))
 
 
 def _policy_kernels(B: int, T: int, by_sequence: bool) -> int:

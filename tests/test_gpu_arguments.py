@@ -149,7 +149,15 @@ def test_linear_gradients_share_no_memory_with_what_they_read(cuda):
 
 
 def test_launches_are_counted(cuda):
-    """Few tokens are counted by the row kernel, others by kernels of their own."""
+    """Few tokens are counted by the row kernel, others by kernels of their own; few pairs' mean needs no kernel of its
+    own."""
+    for P, T, grad, want in ((1, 5, False, 2), (8, 5, True, 3), (9, 5, True, 4), (2, 300, True, 4), (1, 300, True, 3)):
+        before = nv._lib.launch_count
+        x, m, loss = torch.randn(2 * P, T, 40, device="cuda"), z(P), z(1)
+        nv.preference_loss(x, z(2 * P, T, dt=L), token_logps=z(2 * P, T), lse=z(2 * P, T), seq_logps=z(2 * P), margins=m,
+                           coef=z(2 * P), loss=loss, dlogits=x if grad else None, kind="squared")
+        assert nv._lib.launch_count - before == want
+        assert loss.item() == pytest.approx(((m.double() - 0.5) ** 2).mean().item(), rel=1e-6)
     for B, T, by_sequence, want in ((2, 9, False, 2), (33, 2, True, 4), (33, 2, False, 2), (5, 300, False, 4)):
         before = nv._lib.launch_count
         x = torch.randn(B, T, 40, device="cuda")

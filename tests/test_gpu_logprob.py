@@ -210,6 +210,9 @@ PREF = [
     dict(P=3, T=60, V=8203, dtype=torch.float16, kind="hinge", average=True, beta=1.0),
     dict(P=160, T=1, V=20001, dtype=torch.float32, kind="squared", layout="padded"),
     dict(P=2, T=9, V=500, dtype=torch.float32, kind="hinge", average=True, empty=True),
+    dict(P=100, T=5, V=250, dtype=torch.float32, kind="sigmoid", average=True, beta=1.0, smoothing=0.1),
+    dict(P=512, T=1, V=501, dtype=torch.float16, kind="squared", layout="padded"),
+    dict(P=1, T=450, V=1100, dtype=torch.bfloat16, kind="hinge", layout="shifted", free=True),
 ]
 
 
