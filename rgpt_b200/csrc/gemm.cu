@@ -1282,6 +1282,36 @@ __global__ void __launch_bounds__(ROWS == 1 ? 256 : 1024) lse_reduce_kernel(
   if (lse) lse[row] = (float)l;
 }
 
+// out = the sum of `splits` partial products, in their order.
+__global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ part, int splits, int M, int N, void* out,
+                                                        long long ldo, int f32) {
+  griddep_wait();
+  griddep_launch();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, ld = (N + 3) / 4 * 4;
+  const int row = (int)(i / ld), col = (int)(i % ld);
+  if (row >= M || col >= N) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) s += part[(long long)k * M * ld + i];
+  const long long at = (long long)row * ldo + col;
+  if (f32) reinterpret_cast<float*>(out)[at] = s;
+  else reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16(s);
+}
+
+extern "C" int rgpt_gemm_join(const float* part, int splits, int M, int N, void* out, long long ldo, int out_f32,
+                              void* stream) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int st = rgpt_check_device(dev);
+  if (st) return st;
+  if (splits < 1 || M < 1 || N < 1 || ldo < N || part == nullptr || out == nullptr)
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "gemm_join: splits=%d M=%d N=%d ldo=%lld or a null pointer", splits, M, N, ldo);
+  const long long n = (long long)M * ((N + 3) / 4 * 4);
+  launch_pdl(gemm_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1, part,
+             splits, M, N, out, ldo, out_f32);
+  return rgpt_check_launch("gemm_join_kernel");
+}
+
 static int logp_gemm_check(const char* what, const long long* labels) {
   return labels == nullptr ? rgpt_set_error(RGPT_ERR_BAD_SHAPE, "%s: null pointer", what) : RGPT_OK;
 }

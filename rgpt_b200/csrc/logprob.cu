@@ -404,6 +404,22 @@ __device__ __forceinline__ void lp_write_rest(const E* x, E* d, int label, float
     d[j] = L::put(j == label ? g + coef : g);
   }
 }
+// 16 bytes at an address of the type's alignment only: by 4-byte words, two bytes on where that address lies inside one (a
+// word is never split between what may be read and what may not).
+__device__ __forceinline__ uint4 lp_load_any(const float* p) {
+  return make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3]));
+}
+template <typename E>
+__device__ __forceinline__ uint4 lp_load_any(const E* p) {
+  static_assert(sizeof(E) == 2, "16-bit types");
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+  const uint32_t a = w[0], b = w[1], c = w[2], d = w[3];
+  if ((at & 2) == 0) return make_uint4(a, b, c, d);
+  const uint32_t e = w[4];
+  return make_uint4(__funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), __funnelshift_r(c, d, 16),
+                    __funnelshift_r(d, e, 16));
+}
 template <typename E>
 __device__ __forceinline__ bool lp_aligned(const E* x, const E* d) {
   return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
@@ -416,12 +432,22 @@ __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label
                                               const LpProb& prob) {
   using L = LpType<E>;
   constexpr int N = lp_size<W>(LP_THREADS);
-  const int head = lp_aligned(x, d) ? lp_head(x, V) : V, nvec = (V - head) / L::VEC;
+  const bool same = lp_aligned(x, d);
+  const int head = lp_head(d, V), nvec = (V - head) / L::VEC;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   uint4* dv = reinterpret_cast<uint4*>(d + head);
   auto one = [&](const uint4& u, int at) { return lp_grad_vec<E>(u, at, coef, prob); };
   int v = sh.lo(nvec) + lp_rank<W>();
   const int vend = sh.hi(nvec);
+  if (!same) {  // stores by vectors, loads by what x's alignment allows
+    for (; v < vend; v += 2 * N) {
+      const bool two = v + N < vend;
+      const uint4 a = lp_load_any(x + head + (long long)v * L::VEC);
+      const uint4 b = two ? lp_load_any(x + head + (long long)(v + N) * L::VEC) : a;
+      __stcs(&dv[v], one(a, label - head - v * L::VEC));
+      if (two) __stcs(&dv[v + N], one(b, label - head - (v + N) * L::VEC));
+    }
+  }
   if constexpr (W == LP_WARP) {  // short rows: one step takes most of them, its last vectors from some lanes only
     for (; v - lp_rank<W>() < vend; v += LP_UNROLL * N) {
       uint4 u[LP_UNROLL];
@@ -925,13 +951,17 @@ struct PolicyRows {
   float *logps, *lse, *coef;
 };
 
+// A token's inputs, loaded before its row is.
+struct PolicyIn {
+  float old, ref, adv;
+  __device__ __forceinline__ PolicyIn(const PolicyRows& p, LpRows lr, long long row)
+      : old(p.old[row]), ref(p.ref ? p.ref[row] : 0.f), adv(p.adv[p.a.adv_per_token ? row : lr.batch(row)]) {}
+};
 // What thread 0 does with a row's sum: the token's terms, the outputs, and the row's coefficient for the CTA.
-__device__ __forceinline__ float policy_row(const PolicyRows& p, LpRows lr, long long row, float xl, const LpRow& r,
-                                            int n, int total, bool first) {
+__device__ __forceinline__ float policy_row(const PolicyRows& p, const PolicyIn& in, long long row, float xl,
+                                            const LpRow& r, int n, int total, bool first) {
   const double lp = lp_label(xl, r);
-  const unsigned b = lr.batch(row);
-  const PolicyTerms t = policy_terms(p.a, lp, p.old[row], p.ref != nullptr, p.ref ? p.ref[row] : 0.f,
-                                     p.adv[p.a.adv_per_token ? row : b]);
+  const PolicyTerms t = policy_terms(p.a, lp, in.old, p.ref != nullptr, in.ref, in.adv);
   const float coef = t.d * policy_weight(p.a, n, total) * p.a.grad_scale;
   if (first) {
     p.logps[row] = (float)lp;
@@ -995,10 +1025,11 @@ __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpR
   }
   const E* x = logits + lr.offset(row);
   const float xl = LpType<E>::get(x[label]);  // before an in-place gradient
+  const PolicyIn in(p, lr, row);
   const int2 n = W == LP_WARP ? make_int2(p.counts[lr.batch(row)], *p.total) : policy_counts(p, lr, V, row, true, red);
   const LpRow r = lp_row_sum<E, W>(x, V);
   float coef = 0.f;
-  if (first) coef = policy_row(p, lr, row, xl, r, n.x, n.y, true);
+  if (first) coef = policy_row(p, in, row, xl, r, n.x, n.y, true);
   if (!d) return;
   if constexpr (W == LP_WARP) {
     coef = __shfl_sync(0xffffffffu, coef, 0);
@@ -1040,13 +1071,14 @@ __global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logi
   }
   const E* x = logits + lr.offset(row);
   const float xl = L::get(x[label]);
+  const PolicyIn in(p, lr, row);
   LpRow r;
   int2 n;
   auto st = lp_stage<POL_VECS>(x, V, sh, lp_smem, full, POL_SLOTS, false);
   lp_staged_sum<E, W, LP_THREADS>(st, x, V, sh, &r, [&] {
     n = policy_counts(p, lr, V, row, sh.part == 0, red);  // while the first pieces are on their way
   });
-  if (threadIdx.x == 0) s_coef = policy_row(p, lr, row, xl, r, n.x, n.y, sh.part == 0);
+  if (threadIdx.x == 0) s_coef = policy_row(p, in, row, xl, r, n.x, n.y, sh.part == 0);
   if (!d) return;
   __syncthreads();
   const float coef = s_coef;

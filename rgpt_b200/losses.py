@@ -119,8 +119,8 @@ class _LinearLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dlogps):
         x, w, labels, lse = ctx.saved_tensors
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(w.shape, device=w.device, dtype=w.dtype) if ctx.needs_input_grad[1] else None
+        dx, dw = (_new(t, t.shape[0], (t.shape[1] + 7) // 8 * 8, dtype=t.dtype)[:, :t.shape[1]] if need else None
+                  for t, need in zip((x, w), ctx.needs_input_grad))
         nv.linear_logprobs_bwd(x, w, labels, lse, dlogps.float().contiguous(), dx, dw, ignore_index=ctx.ignore_index)
         return dx, dw, None, None
 

@@ -629,6 +629,28 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
              int(bool(round_bf16)), part.data_ptr(), part.numel(), *outs, kernels=2)
 
 
+def _gemm_long(A: torch.Tensor, B: torch.Tensor, out: torch.Tensor) -> None:
+    """out = A @ B^T (bf16 or fp32, written). Where the output has tiles for half of the SMs at most and the contraction is
+    long, it is cut into parts whose fp32 products are joined in order (88 rows x 408 columns over 116602: 480 -> 30 us)."""
+    (M, C), N = A.shape, B.shape[0]
+    tiles = -(-M // 128) * -(-N // 256)
+    sms = torch.cuda.get_device_properties(out.device).multi_processor_count
+    splits = min(sms // tiles, C // 1024) if 2 * tiles <= sms else 1
+    epi = EPI_STORE_BF16 if out.dtype == torch.bfloat16 else EPI_STORE_F32
+    if splits < 2:
+        gemm(A, B, out, epi=epi)
+        return
+    each = -(-C // (64 * splits)) * 64
+    whole, splits = C // each, -(-C // each)
+    part = torch.empty(splits, M, (N + 3) // 4 * 4, device=out.device, dtype=torch.float32)
+    cut = [t.as_strided((whole, t.shape[0], each), (each * t.stride(1), t.stride(0), t.stride(1))) for t in (A, B)]
+    gemm(*cut, part[:whole, :, :N], epi=EPI_STORE_F32)
+    if whole < splits:
+        gemm(A[:, whole * each:], B[:, whole * each:], part[whole, :, :N], epi=EPI_STORE_F32)
+    _lib.call("rgpt_gemm_join", ptr(part), splits, M, N, ptr(out), out.stride(0), int(out.dtype == torch.float32),
+              _lib.stream_ptr(out.device))
+
+
 # Gradient rows of linear_logprobs_bwd in flight: at most this many bf16 logit gradients (1 GiB) at a time.
 LINEAR_CHUNK_ELEMS = 1 << 29
 
@@ -667,7 +689,7 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
         dl = torch.empty(rows, ld, device=dev, dtype=torch.bfloat16)[:, :V]
         acc = dw
         if dw is not None and dw.dtype == torch.bfloat16 and rows < M:
-            acc = torch.zeros(V, K, device=dev, dtype=torch.float32)
+            acc = torch.zeros(V, (K + 3) // 4 * 4, device=dev, dtype=torch.float32)[:, :K]
         for a in range(0, M, rows):
             n = min(rows, M - a)
             xa, d = x[a:a + n], dl[:n]
@@ -675,10 +697,10 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
                       ptr(labels[a:a + n]), int(ignore_index), ptr(lse[a:a + n]), ptr(dlogps[a:a + n]), ptr(d), ld,
                       _lib.stream_ptr(dev))
             if dx is not None:
-                gemm(d, w.t(), dx[a:a + n], epi=EPI_STORE_BF16 if dx.dtype == torch.bfloat16 else EPI_STORE_F32)
+                _gemm_long(d, w.t(), dx[a:a + n])
             if acc is not None:
                 if acc.dtype == torch.bfloat16:
-                    gemm(d.t(), xa.t(), acc)
+                    _gemm_long(d.t(), xa.t(), acc)
                 else:
                     gemm(d.t(), xa.t(), acc, epi=EPI_ACCUM_F32, splitk=0)
         if acc is not dw:

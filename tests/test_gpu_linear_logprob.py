@@ -75,15 +75,19 @@ def test_rounded_products_give_what_stored_logits_give(cuda, M, V, K):
 
 
 @pytest.mark.parametrize("M,V,K,stride,chunk", [(1, 9, 8, 0, None), (7, 50257, 512, 0, None), (300, 1001, 72, 8, None),
-                                               (300, 1001, 64, 0, 128), (1025, 5000, 512, 0, 256), (2047, 777, 1024, 0, 1000)])
+                                               (300, 1001, 64, 0, 128), (1025, 5000, 512, 0, 256), (2047, 777, 1024, 0, 1000),
+                                               # few output tiles and a long contraction, for dx and for dw
+                                               (88, 33001, 408, 0, None), (3, 20480, 72, 8, None), (129, 9999, 30, 2, 100),
+                                               (5000, 130, 72, 0, None), (4097, 129, 9, 7, None)])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
 def test_backward(cuda, M, V, K, stride, chunk, out):
     x, w, labels = make(M, V, K, stride=stride)
     lp, lse = torch.empty(M, device=cuda), torch.empty(M, device=cuda)
     nv.linear_logprobs(x, w, labels, lp, lse=lse)
     g = torch.randn(M, device=cuda) / M
-    dx = torch.full((M, K), 5.0, device=cuda, dtype=out)
-    dw = torch.full((V, K), 0.25, device=cuda, dtype=out)
+    ld = (K + 7) // 8 * 8
+    dx = torch.full((M, ld), 5.0, device=cuda, dtype=out)[:, :K]
+    dw = torch.full((V, ld), 0.25, device=cuda, dtype=out)[:, :K]
     nv.linear_logprobs_bwd(x, w, labels, lse, g, dx, dw, chunk_rows=chunk)
     on, z, want_lse, _, size = ref(x, w, labels)
     d = torch.softmax(z, 1)
@@ -105,8 +109,9 @@ def test_backward(cuda, M, V, K, stride, chunk, out):
     assert nv._lib.device_error() == 0
 
 
-def test_autograd_and_no_rows(cuda):
-    x, w, labels = make(70, 513, 64)
+@pytest.mark.parametrize("K", [64, 61])
+def test_autograd_and_no_rows(cuda, K):
+    x, w, labels = make(70, 513, K, stride=64 - K)
     x.requires_grad_(True), w.requires_grad_(True)
     lp = losses.linear_logprobs(x, w, labels)
     (lp * torch.linspace(-1, 1, 70, device=cuda)).sum().backward()
@@ -118,6 +123,6 @@ def test_autograd_and_no_rows(cuda):
         # bf16 gradient rows and a bf16 result: 2^-8 of the largest sum's size
         assert ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * want.abs().max()).all()
     nv.linear_logprobs(x.detach()[:0], w.detach(), labels[:0], torch.empty(0, device=cuda))
-    dw = torch.ones(513, 64, device=cuda, dtype=torch.bfloat16)
+    dw = torch.ones(513, 64, device=cuda, dtype=torch.bfloat16)[:, :K]
     nv.linear_logprobs_bwd(x.detach()[:0], w.detach(), labels[:0], torch.empty(0, device=cuda), torch.empty(0, device=cuda), None, dw)
     assert (dw == 0).all()
