@@ -439,14 +439,9 @@ __device__ __forceinline__ void lp_write_grad(const E* x, E* d, int V, int label
   auto one = [&](const uint4& u, int at) { return lp_grad_vec<E>(u, at, coef, prob); };
   int v = sh.lo(nvec) + lp_rank<W>();
   const int vend = sh.hi(nvec);
-  if (!same) {  // stores by vectors, loads by what x's alignment allows
-    for (; v < vend; v += 2 * N) {
-      const bool two = v + N < vend;
-      const uint4 a = lp_load_any(x + head + (long long)v * L::VEC);
-      const uint4 b = two ? lp_load_any(x + head + (long long)(v + N) * L::VEC) : a;
-      __stcs(&dv[v], one(a, label - head - v * L::VEC));
-      if (two) __stcs(&dv[v + N], one(b, label - head - (v + N) * L::VEC));
-    }
+  if (!same) {  // stores by vectors, loads by what x's alignment allows (4096 rows of 50257 bf16: 198 us; aligned 137)
+#pragma unroll 1
+    for (; v < vend; v += N) __stcs(&dv[v], one(lp_load_any(x + head + (long long)v * L::VEC), label - head - v * L::VEC));
   }
   if constexpr (W == LP_WARP) {  // short rows: one step takes most of them, its last vectors from some lanes only
     for (; v - lp_rank<W>() < vend; v += LP_UNROLL * N) {
@@ -1050,7 +1045,7 @@ __global__ void __launch_bounds__(LP_THREADS) policy_kernel(const E* logits, LpR
 constexpr int POL_VECS = 1024, POL_SLOTS = 3;
 constexpr uint32_t POL_SMEM = POL_SLOTS * POL_VECS * 16u;
 template <typename E, int W>
-__global__ void __launch_bounds__(LP_THREADS) policy_staged_kernel(const E* logits, LpRows lr, int V,
+__global__ void __launch_bounds__(LP_THREADS, 4) policy_staged_kernel(const E* logits, LpRows lr, int V,
                                                                     const PolicyRows p, E* dlogits, LpRows dr) {
   using L = LpType<E>;
   extern __shared__ __align__(128) uint8_t lp_smem[];
