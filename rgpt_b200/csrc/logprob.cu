@@ -1165,8 +1165,9 @@ static void lp_dispatch(int dtype, F&& f) {
 }
 
 // CTAs a row: doubled (up to the portable cluster of 8) while the grid stays within two CTAs an SM and each part keeps
-// at least 8 KB of the row. Policy loss of rows of 100 KB, us for 1 / 2 / 4 / 8 CTAs a row: 16 rows 20.5 / 20.5 / 18.4 /
-// 16.4, 64 rows 20.5 / 20.5 / 18.4 / 26.7, 148 rows 20.5 / 20.5 / 28.7 / 42.0, 300 rows 28.5 / 34.8 / 41.8 / 69.6.
+// at least 8 KB of the row. Rows of 100 KB, us for 1 / 2 / 4 / 8 CTAs a row, forward: 16 rows 8.5 / 6.8 / 5.7 / 5.2, 64 rows
+// 9.6 / 7.7 / 6.9 / 6.9, 148 rows 9.9 / 8.6 / 10.3 / 12.6, 300 rows 12.4 / 12.4 / 15.3 / 19.8; policy loss: 15.0 / 13.3 / 11.8 /
+// 11.5, 15.9 / 14.6 / 14.3 / 22.0, 16.8 / 18.0 / 25.1 / 37.6, 25.1 / 30.9 / 38.4 / 66.9.
 static int lp_parts(long long M, int V, int dtype) {
   int dev = 0;
   cudaGetDevice(&dev);
