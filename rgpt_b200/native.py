@@ -629,27 +629,32 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
              int(bool(round_bf16)), part.data_ptr(), part.numel(), *outs, kernels=2)
 
 
-def _gemm_long(A: torch.Tensor, B: torch.Tensor, out: torch.Tensor) -> None:
-    """out = A @ B^T (bf16 or fp32, written). Where the output has tiles for half of the SMs at most and the contraction is
-    long, it is cut into parts whose fp32 products are joined in order (88 rows x 408 columns over 116602: 536 -> 76 us, most
-    of those on the host)."""
-    (M, C), N = A.shape, B.shape[0]
+def _product(dev: int, A: tuple, B: tuple, M: int, N: int, C: int, D: tuple, *, batch: int = 1, epi: int, splitk: int = 1):
+    """D = A @ B^T, [M, N] over C: A and B are (address, 1 if rows are the contiguous side, row stride, batch stride), D is
+    (address, row stride, batch stride). gemm() without its checks, which take longer than a few rows' product."""
+    _call_on(dev, "rgpt_gemm_bf16", *A, *B, M, N, C, batch, epi, 0, 1.0, 0.0, *D, None, 0, 0, None, 0, 0, None, splitk, None)
+
+
+def _product_long(out: torch.Tensor, dev: int, A: tuple, B: tuple, M: int, N: int, C: int, D: int, ldd: int) -> None:
+    """D = A @ B^T as _product, written in out's type. Where D has tiles for half of the SMs at most and C is long, C is cut
+    into parts whose fp32 products are joined in order (88 rows x 408 columns over 116602 take 536 us otherwise, the whole
+    backward of such rows 112)."""
     tiles = -(-M // 128) * -(-N // 256)
-    sms = torch.cuda.get_device_properties(out.device).multi_processor_count
+    sms = torch.cuda.get_device_properties(dev).multi_processor_count
     splits = min(sms // tiles, C // 1024) if 2 * tiles <= sms else 1
-    epi = EPI_STORE_BF16 if out.dtype == torch.bfloat16 else EPI_STORE_F32
+    f32 = out.dtype is torch.float32
     if splits < 2:
-        gemm(A, B, out, epi=epi)
-        return
+        return _product(dev, (*A, 0), (*B, 0), M, N, C, (D, ldd, 0), epi=EPI_STORE_F32 if f32 else EPI_STORE_BF16)
     each = -(-C // (64 * splits)) * 64
-    whole, splits = C // each, -(-C // each)
-    part = torch.empty(splits, M, (N + 3) // 4 * 4, device=out.device, dtype=torch.float32)
-    cut = [t.as_strided((whole, t.shape[0], each), (each * t.stride(1), t.stride(0), t.stride(1))) for t in (A, B)]
-    gemm(*cut, part[:whole, :, :N], epi=EPI_STORE_F32)
+    whole, splits, ld = C // each, -(-C // each), (N + 3) // 4 * 4
+    part = torch.empty(splits * M * ld, device=out.device, dtype=torch.float32)
+    step = [each * (ldo if mn else 1) for _, mn, ldo in (A, B)]  # elements from one part to the next
+    P, size = part.data_ptr(), M * ld
+    _product(dev, (*A, step[0]), (*B, step[1]), M, N, each, (P, ld, size), batch=whole, epi=EPI_STORE_F32)
     if whole < splits:
-        gemm(A[:, whole * each:], B[:, whole * each:], part[whole, :, :N], epi=EPI_STORE_F32)
-    _lib.call("rgpt_gemm_join", ptr(part), splits, M, N, ptr(out), out.stride(0), int(out.dtype == torch.float32),
-              _lib.stream_ptr(out.device))
+        A, B = ((at + 2 * whole * st, mn, ldo, 0) for (at, mn, ldo), st in zip((A, B), step))
+        _product(dev, A, B, M, N, C - whole * each, (P + 4 * whole * size, ld, 0), epi=EPI_STORE_F32)
+    _call_on(dev, "rgpt_gemm_join", P, splits, M, N, D, ldd, int(f32))
 
 
 # Gradient rows of linear_logprobs_bwd in flight: at most this many bf16 logit gradients (1 GiB) at a time.
@@ -682,30 +687,32 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
         if dw is not None and dw.dtype == torch.bfloat16:
             dw.zero_()
         return
-    if not x.is_cuda:
+    index = x.get_device()
+    if index < 0:
         raise RuntimeError("librgpt_kernels only takes CUDA tensors (no CPU path)")
     ld = (V + 7) // 8 * 8
     rows = min(M, chunk_rows or max(256, LINEAR_CHUNK_ELEMS // ld // 256 * 256))
-    with torch.cuda.device(dev):
-        dl = torch.empty(rows, ld, device=dev, dtype=torch.bfloat16)[:, :V]
-        acc = dw
-        if dw is not None and dw.dtype == torch.bfloat16 and rows < M:
-            acc = torch.zeros(V, (K + 3) // 4 * 4, device=dev, dtype=torch.float32)[:, :K]
-        for a in range(0, M, rows):
-            n = min(rows, M - a)
-            xa, d = x[a:a + n], dl[:n]
-            _lib.call("rgpt_linear_logprobs_dlogits", ptr(xa), x.stride(0), ptr(w), w.stride(0), n, V, K,
-                      ptr(labels[a:a + n]), int(ignore_index), ptr(lse[a:a + n]), ptr(dlogps[a:a + n]), ptr(d), ld,
-                      _lib.stream_ptr(dev))
-            if dx is not None:
-                _gemm_long(d, w.t(), dx[a:a + n])
-            if acc is not None:
-                if acc.dtype == torch.bfloat16:
-                    _gemm_long(d.t(), xa.t(), acc)
-                else:
-                    gemm(d.t(), xa.t(), acc, epi=EPI_ACCUM_F32, splitk=0)
-        if acc is not dw:
-            dw.copy_(acc)
+    dl = torch.empty(rows * ld, device=dev, dtype=torch.bfloat16)
+    acc = dw
+    if dw is not None and dw.dtype is torch.bfloat16 and rows < M:
+        acc = torch.zeros(V, (K + 3) // 4 * 4, device=dev, dtype=torch.float32)
+    X, W, L, S, G, d = (t.data_ptr() for t in (x, w, labels, lse, dlogps, dl))
+    ldx, ldw = x.stride(0), w.stride(0)
+    for a in range(0, M, rows):
+        n, xa = min(rows, M - a), X + 2 * a * ldx
+        _call_on(index, "rgpt_linear_logprobs_dlogits", xa, ldx, W, ldw, n, V, K, L + 8 * a, int(ignore_index), S + 4 * a,
+                 G + 4 * a, d, ld)
+        if dx is not None:
+            _product_long(dx, index, (d, 0, ld), (W, 1, ldw), n, K, V, dx.data_ptr() + dx.element_size() * a * dx.stride(0),
+                          dx.stride(0))
+        if acc is not None:
+            if acc.dtype is torch.bfloat16:
+                _product_long(acc, index, (d, 1, ld), (xa, 1, ldx), V, K, n, acc.data_ptr(), acc.stride(0))
+            else:
+                _product(index, (d, 1, ld, 0), (xa, 1, ldx, 0), V, K, n, (acc.data_ptr(), acc.stride(0), 0), epi=EPI_ACCUM_F32,
+                         splitk=0)
+    if acc is not dw:
+        dw.copy_(acc[:, :K])
 
 
 # ----------------------------------------------------------------------------- optimizer
