@@ -3,7 +3,6 @@ same arguments and refuse the same calls."""
 import pytest
 import torch
 
-from rgpt_b200 import _fastargs  # noqa: F401  (built with the kernels)
 from rgpt_b200 import native as nv
 
 pytestmark = pytest.mark.gpu
@@ -84,6 +83,8 @@ def recorded(monkeypatch, call, pack, held):
 
 
 def test_same_arguments(cuda, monkeypatch):
+    from rgpt_b200 import _fastargs  # built with the kernels
+    assert nv._pack is _fastargs.pack
     for name, call in calls():
         held = []
         (packed, a), (_, b) = recorded(monkeypatch, call, True, held), recorded(monkeypatch, call, False, held)
