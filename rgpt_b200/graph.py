@@ -11,7 +11,8 @@ What a graph fixes at capture, and how this class keeps each step correct:
     before every replay (Muon.use_device_hparams / stage_device_hparams).
   * Buffers. The token ids live in a static device buffer; every call copies its batch there
     (from pinned host memory or from the device). Activations, gradients and optimizer state
-    are the engine's and optimizer's persistent buffers.
+    are the engine's and optimizer's persistent buffers. A replay counts as a pass over those
+    activations: a loss of the same batch shape that waits for its backward refuses it afterwards.
   * The loss. The returned 0-d tensor is the graph's static output: it holds the latest step's
     loss until the next call.
 The first `warmup` calls run eagerly. They are real training steps, and they create the
@@ -54,6 +55,7 @@ class GraphedTrainStep:
         self.launches: int | None = None  # native kernels in one replay (counted at capture)
         self.calls = 0
         self._loss: torch.Tensor | None = None
+        self._acts = None  # the activations that the captured step writes
         optimizer.use_device_hparams()
 
     def _body(self) -> torch.Tensor:
@@ -87,10 +89,12 @@ class GraphedTrainStep:
             mode = "thread_local" if _data_parallel() else "global"
             with torch.cuda.graph(g, capture_error_mode=mode):
                 self._loss = self._body()
+            self._acts = self.model.engine().acts(self.ids.shape[1], self.ids.shape[2] - 1)
             self.launches = _lib.launch_count - n0
             _lib.launch_count = n0
             self.graph = g
         self.graph.replay()
+        self._acts.number += 1
         _lib.launch_count += self.launches
         return self._loss
 
@@ -107,3 +111,4 @@ class GraphedTrainStep:
         holds collectives must be released before the process group is destroyed."""
         self.graph = None
         self._loss = None
+        self._acts = None

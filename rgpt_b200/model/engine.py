@@ -98,9 +98,13 @@ def qk_norm_spec(attn, qk: str, norm_eps: float) -> dict:
 
 
 class _Acts:
-    """Activation buffers for one (B, T) shape, reused across steps."""
+    """Activation buffers for one (B, T) shape, reused across steps, and what else the backward of the pass that
+    filled them needs: its token ids, whether dropout and the halting heads were active, and its number."""
 
     def __init__(self, eng, B, T, dev):
+        self.ids = None
+        self.drop_active = self.halting = False
+        self.number = 0  # of the latest pass: a backward is good for the pass whose activations are still here
         c = eng.cfg
         d, V, F = c["d_model"], c["vocab_size"], 4 * c["d_model"]
         H = c["n_heads"]
@@ -199,7 +203,6 @@ class Engine:
             # data-parallel ranks seeded alike still draw independent masks
             seed ^= (torch.distributed.get_rank() * 0x9E3779B97F4A7C15) & (2 ** 62 - 1)
         self.drop_seed = torch.tensor([seed], dtype=torch.int64).to(self.device)
-        self._drop_active = False
         self._rng_stream = None
         self._mask_events = []
         self.overlap_masks = True  # draw the dropout masks on a side stream (False: on the caller's)
@@ -346,20 +349,21 @@ class Engine:
         ids = input_ids.reshape(-1)
         if ids.dtype != torch.int64:
             ids = ids.long()
-        self._ids = ids.contiguous()
+        A.ids = ids.contiguous()
+        A.number += 1
         lab = None
         if labels is not None:
             lab = labels.reshape(-1)
             lab = (lab if lab.dtype == torch.int64 else lab.long()).contiguous()
         self._labels = lab
         # nn.Dropout is active in training mode (model/gpt.py:96, transformer_block.py:45,52, attention.py:57)
-        self._drop_active = m.training and self.p_drop > 0
-        if self._drop_active:
+        A.drop_active = m.training and self.p_drop > 0
+        if A.drop_active:
             self.drop_seed.add_(1)
             self._draw_masks(A)
-        nv.embedding_fwd(self._ids, m.embs.weight, A.x[0], drop=self._drop(A, "emb"))
+        nv.embedding_fwd(A.ids, m.embs.weight, A.x[0], drop=self._drop(A, "emb"))
         halting = self.halting and lab is not None
-        self._halting_active = halting
+        A.halting = halting
         app = 0
         for r in range(self.n_recur):
             for li, blk in enumerate(m.layers):
@@ -393,7 +397,7 @@ class Engine:
 
     def _drop(self, A, kind, app=0):
         """The Drop spec of one site, or None when dropout is off for this pass."""
-        if not self._drop_active:
+        if not A.drop_active:
             return None
         if kind == "emb":
             return nv.Drop(A.drop_emb, self.drop_seed, self.EMB_DROP_SITE, self.p_drop)
@@ -439,7 +443,7 @@ class Engine:
             # G1 gate = sigmoid(q_n Wg^T + bg), one [M*H, 64] x [64, 64] GEMM with a bias+sigmoid epilogue
             nv.gemm(A.qn[app].view(M * H, 64), W["wg"], A.gate[app].view(M * H, 64),
                     epi=nv.EPI_BIAS_SIGMOID_BF16, colscale=at.gate_proj.bias)
-        if self._drop_active:
+        if A.drop_active:
             torch.cuda.current_stream().wait_event(self._mask_events[app])
         nv.attn_fwd(A.qk[app], A.qkv[app], A.gate[app], A.o[app], A.og[app] if self.g1 else None, A.lse[app],
                     B, T, H, drop=self._drop(A, "attn_p", app))
@@ -458,11 +462,24 @@ class Engine:
                 drop=self._drop(A, "ff_out", app))
 
     # ------------------------------------------------------------------ backward
+    @staticmethod
+    def check_pass(A, number):
+        """Raise unless A still holds the activations of the pass with this number."""
+        if number != A.number:
+            raise RuntimeError(
+                "another pass of this model over a batch of the same shape has replaced the activations that this backward "
+                "needs. Call backward() before the model's next pass (gradients accumulate: loss1.backward(), then the "
+                "second forward and loss2.backward()), and score tokens before the loss or after its backward.")
+
     @torch.no_grad()
-    def backward(self, A, dlogits=None, alpha_dev=None):
+    def backward(self, A, dlogits=None, alpha_dev=None, number=None):
         """Backpropagate from dlogits (bf16 [M, V]; default: the in-place dlogits of the fused loss).
 
-        alpha_dev: optional device scalar scaling every gradient (the upstream loss gradient)."""
+        alpha_dev: optional device scalar scaling every gradient (the upstream loss gradient).
+        number: A.number after the forward this is the backward of (None: the latest); activations that a later
+        pass has replaced give no gradient."""
+        if number is not None:
+            self.check_pass(A, number)
         m = self.model
         G = self.grads
         dl = A.logits if dlogits is None else dlogits
@@ -475,7 +492,7 @@ class Engine:
         lnf_w = "ln_f.weight" if kind == nv.NORM_RMS_AFFINE else None
         lnf_t = "ln_f.temp" if kind == nv.NORM_L2_TEMP else None
         tval = 1.0
-        halting = self._halting_active
+        halting = A.halting
         need_gb_now = not halting
         # A data-parallel optimizer may hook the arena to reduce each gradient bucket as soon as the
         # backward has finished it (overlapping the collective with the rest of the backward). Buckets
@@ -523,7 +540,7 @@ class Engine:
                 if cut:
                     A.g.zero_()
                     A.gb.zero_()
-        nv.embedding_bwd(self._ids, A.g, G["embs.weight"], drop=self._drop(A, "emb"))
+        nv.embedding_bwd(A.ids, A.g, G["embs.weight"], drop=self._drop(A, "emb"))
         if sync is not None:
             if "pre" in self.grad_buckets:
                 sync.ready(self.grad_arena, *self.grad_buckets["pre"])

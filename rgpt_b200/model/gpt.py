@@ -16,6 +16,11 @@ Post-training: ``token_logprobs`` scores labels without storing logits, and
 
 Weight gradients are accumulated into a flat fp32 arena whose views are the
 parameters' ``.grad`` (use the optimizer's ``zero_grad`` to clear them).
+
+The engine keeps one set of activations for each batch shape in use, and every pass over that shape (a loss,
+``token_logprobs``, a replayed training step) overwrites it: call a loss's ``backward()`` before the model's next
+pass. A backward whose activations have been replaced raises RuntimeError. Several losses of one step take turns,
+``loss1.backward()`` before the second forward; their gradients add up.
 """
 import torch
 import torch.nn as nn
@@ -32,14 +37,14 @@ class _GPTLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input_ids, labels, eng, anchor):
         A = eng.forward(input_ids, labels, training=True, want_loss=True, grad_scale=1.0)
-        ctx.eng, ctx.acts = eng, A
+        ctx.eng, ctx.acts, ctx.number = eng, A, A.number
         total = A.losses[0].clone()
         return total, A.losses[1].clone(), (A.losses[2] + A.losses[3]).clone()
 
     @staticmethod
     def backward(ctx, g_total, g_tok, g_q):
         # token / q losses are returned for logging; gradients flow through the total only
-        ctx.eng.backward(ctx.acts, alpha_dev=g_total.reshape(1).float().contiguous())
+        ctx.eng.backward(ctx.acts, alpha_dev=g_total.reshape(1).float().contiguous(), number=ctx.number)
         return None, None, None, None
 
 
@@ -50,9 +55,9 @@ class _GPTForward(torch.autograd.Function):
     def forward(ctx, input_ids, labels, eng, anchor):
         A = eng.forward(input_ids, labels, training=True, want_loss=False)
         B, T = input_ids.shape
-        ctx.eng, ctx.acts, ctx.shape = eng, A, (B, T)
+        ctx.eng, ctx.acts, ctx.number, ctx.shape = eng, A, A.number, (B, T)
         logits = A.logits.view(B, T, -1).clone()
-        if eng._halting_active:
+        if A.halting:
             import torch.nn.functional as F
             R = eng.n_recur
             lab = eng._labels
@@ -72,9 +77,10 @@ class _GPTForward(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_logits, d_halt, d_qs, d_targets):
         eng, A = ctx.eng, ctx.acts
+        eng.check_pass(A, ctx.number)
         B, T = ctx.shape
         dl = d_logits.reshape(B * T, -1).to(torch.bfloat16).contiguous()
-        if eng._halting_active:
+        if A.halting:
             R = eng.n_recur
             M = B * T
             dq = torch.zeros(R, M, 2, device=dl.device, dtype=torch.float32)
@@ -96,13 +102,13 @@ class _GPTPostTraining(torch.autograd.Function):
         A = eng.forward(input_ids, None, training=True, want_loss=False)
         logits = A.logits.view(*input_ids.shape, -1)
         outs = loss_fn(logits, logits)
-        ctx.eng, ctx.acts = eng, A
+        ctx.eng, ctx.acts, ctx.number = eng, A, A.number
         ctx.mark_non_differentiable(*outs[1:])
         return outs
 
     @staticmethod
     def backward(ctx, g, *unused):
-        ctx.eng.backward(ctx.acts, alpha_dev=g.reshape(1).float().contiguous())
+        ctx.eng.backward(ctx.acts, alpha_dev=g.reshape(1).float().contiguous(), number=ctx.number)
         return None, None, None, None
 
 
@@ -182,7 +188,7 @@ class GPT(nn.Module):
         eng = self.engine()
         if torch.is_grad_enabled() and self.training:
             logits, halt, qs, targets = _GPTForward.apply(input_ids, labels, eng, self._anchor())
-            if not eng._halting_active:
+            if labels is None or not eng.halting:
                 return logits, halt, [], []
             return logits, halt, list(qs.unbind(0)), targets
         A = eng.forward(input_ids, labels, training=False, want_loss=False)
@@ -224,7 +230,8 @@ class GPT(nn.Module):
         """Paired preference loss (native.preference_loss) of input_ids, labels [2P, T]: the P chosen sequences, then
         the P rejected ones; labels == pad_token_id (prompts, padding) are not scored. ref_logps [2P]: the frozen
         reference's summed (averaged, with `average`) token_logprobs. Returns (loss, sequence log-probabilities [2P],
-        margins [P]); the loss is differentiable in training mode. Halting losses are not part of it."""
+        margins [P]); the loss is differentiable in training mode, until the model's next pass over this batch shape. Halting
+        losses are not part of it."""
         labels = labels.long().contiguous()
         new = lambda *s: torch.empty(*s, device=labels.device, dtype=torch.float32)  # noqa: E731
 
@@ -244,7 +251,8 @@ class GPT(nn.Module):
         """Clipped policy loss with a KL term (native.policy_loss) of input_ids, labels [B, T] (the sampled tokens;
         pad_token_id where not scored); old_logps and ref_logps [B, T]: token_logprobs of the sampling policy and of
         the frozen reference; advantages [B] or [B, T]. Returns (loss, stats [4], token log-probabilities [B, T]); the
-        loss is differentiable in training mode. Halting losses are not part of it."""
+        loss is differentiable in training mode, until the model's next pass over this batch shape. Halting losses are not
+        part of it."""
         labels = labels.long().contiguous()
         new = lambda *s, dt=torch.float32: torch.empty(*s, device=labels.device, dtype=dt)  # noqa: E731
 
