@@ -203,8 +203,10 @@ struct LpSum {
   }
 };
 
-// What a row's sum comes to: probabilities e^{x - lse} = 2^{c (x - a) - b} * inv. a = 0 and b = M, or after a careful
-// pass a = max and b = 0; the subtraction of a 0 is exact, so one form serves both.
+// What a row's sum comes to: probabilities e^{x - lse} = 2^{c (x - a) - b} * inv. The subtraction comes first, so that
+// what fp32 leaves of c and of the product goes with x - a and not with x (2^{c x - M} / sum, in one fused operation an
+// element, makes every probability of a row of logits near 1000 some 1e-5 too small). After the plain pass a is lse
+// rounded to fp32 and b the rest of it in base 2, after a careful pass a = max and b = 0.
 struct LpRow {
   float a, b, inv;
   double lse;
@@ -288,7 +290,9 @@ __device__ __forceinline__ double lp_log(double M, float s) {
 }
 // The finished row from its joined (M, s).
 __device__ __forceinline__ LpRow lp_finish(float2 r) {
-  return LpRow{0.f, r.x, 1.f / r.y, lp_log((double)r.x, r.y) - LP_EX2_MEAN};
+  const double lse = lp_log((double)r.x, r.y) - LP_EX2_MEAN;
+  const float a = (float)lse;
+  return LpRow{a, (float)((lse - (double)a) * 1.4426950408889634), 1.f, lse};
 }
 // The label's log-probability; rounding may not make a sure label more than sure.
 __device__ __forceinline__ double lp_label(float xl, const LpRow& r) {
