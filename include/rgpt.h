@@ -254,7 +254,9 @@ int rgpt_preference_loss(const void* logits, int dtype, long long sb, long long 
  *   loss = sum_t w (pg + kl_coef kl),  w = 1 / (scored tokens), or with by_sequence
  *   1 / (sequences with a scored token * scored tokens of the token's sequence).
  * old_logps, ref_logps [B, T]; advantages [B], or [B, T] with adv_per_token. Writes token_logps [B, T], counts [B]
- * (scored tokens of each sequence), stats [4] = {loss, sum w pg, sum w kl, weighted share of clipped tokens}, the
+ * (scored tokens of each sequence), stats [4] = {loss, sum w pg, sum w kl, weighted share of clipped tokens} of these
+ * token_logps (summed in fp64; coef and dlogits have the log-probabilities before their rounding to fp32, and clip the
+ * same tokens), the
  * optional lse [B, T] and coef [B, T] (grad_scale * d loss / d lp, 0 where not scored), and, when dlogits is not null,
  * grad_scale * d loss / d logits. Without any scored token everything is 0. */
 int rgpt_policy_loss(const void* logits, int dtype, long long sb, long long st, int B, int T, int V,

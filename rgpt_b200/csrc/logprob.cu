@@ -896,7 +896,9 @@ __device__ __forceinline__ float kl_term(float q, float e) {
 }
 
 // Terms of one token from its log-probability lp: r = e^{lp - old}; -min(r A, clip(r) A); e^q - q - 1, q = ref - lp.
-// The differences are taken, and compared with the clip's borders, in fp64; the exponentials of them in fp32.
+// The differences are taken in fp64, their exponentials in fp32 (1e-7 of a term). Whether a ratio lies past a border is
+// decided, in fp64, from the log-probability as it is returned, rounded to fp32: the gradient has lp before that, the
+// statistics after it, and both must count the same tokens as clipped.
 struct PolicyTerms {
   float pg, kl, cut, d;  // d = d (pg + kl_coef * kl) / d lp
 };
@@ -904,7 +906,8 @@ __device__ __forceinline__ PolicyTerms policy_terms(const PolicyArgs& a, double 
                                                     float adv) {
   PolicyTerms t;
   const double lr = lp - (double)old;
-  const bool cut = (adv > 0.f && lr > a.log_high) || (adv < 0.f && lr < a.log_low);
+  const double at = (double)(float)lp - (double)old;
+  const bool cut = (adv > 0.f && at > a.log_high) || (adv < 0.f && at < a.log_low);
   const float r = expf((float)lr);
   t.pg = -(cut ? (adv > 0.f ? 1.f + a.high : 1.f - a.low) : r) * adv;
   t.d = cut ? 0.f : -r * adv;
