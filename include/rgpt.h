@@ -242,7 +242,8 @@ int rgpt_token_logprobs_bwd(const void* logits, int dtype, long long sb, long lo
  *   SQUARED: (h - 1/2)^2;   loss[0] = mean over the pairs.
  * Writes token_logps, lse [2P, T], seq_logps [2P] (s), margins [P] (h), coef [2P] (grad_scale * d loss / d a scored
  * token's log-probability) and, when dlogits is not null, grad_scale * d loss / d logits. scratch [2P, T] fp64: the
- * log-probabilities before their rounding to fp32, whose errors the difference of two long sums would show. */
+ * log-probabilities before their rounding to fp32, whose errors the difference of two long sums would show; many pairs'
+ * losses take the places of some of them on their way to the mean, which is rounded once. */
 enum RgptPreference { RGPT_PREF_SIGMOID = 0, RGPT_PREF_HINGE = 1, RGPT_PREF_SQUARED = 2 };
 int rgpt_preference_loss(const void* logits, int dtype, long long sb, long long st, int P, int T, int V,
                          const long long* labels, long long ignore_index, const float* ref_logps, int kind, float beta,

@@ -804,8 +804,9 @@ __device__ __forceinline__ void pref_terms(const PrefArgs& a, double h, double* 
 
 // A pair a warp, or for long sequences a CTA: the two sequences' log-probabilities in fp64, the margin h and the sequences'
 // coefficients d loss / d (a scored token's log-probability). Where one CTA takes all pairs it writes their mean loss as
-// well, which saves a launch.
-__global__ void __launch_bounds__(256) pref_pair_kernel(const double* __restrict__ logps,
+// well, which saves a launch; else a pair's loss, in fp64, takes the place of its first log-probability, which only this
+// pair reads and has read.
+__global__ void __launch_bounds__(256) pref_pair_kernel(double* logps,
                                                         const long long* __restrict__ labels, long long ignore_index,
                                                         int V, int P, int T, int by_warp, const float* __restrict__ ref,
                                                         PrefArgs a, float* __restrict__ seq_logps,
@@ -850,6 +851,7 @@ __global__ void __launch_bounds__(256) pref_pair_kernel(const double* __restrict
       margins[p] = (float)h;
       coef[p] = (float)(dh / n[0]);
       coef[p + P] = (float)(-dh / n[1]);
+      if (gridDim.x > 1) logps[(long long)p * T] = pair_loss;
     }
   }
   if (gridDim.x > 1) return;
@@ -857,18 +859,14 @@ __global__ void __launch_bounds__(256) pref_pair_kernel(const double* __restrict
   if (threadIdx.x == 0) loss_out[0] = (float)(mean / P);
 }
 
-// mean of the pairs' losses, from their margins
-__global__ void __launch_bounds__(256) pref_loss_kernel(const float* __restrict__ margins, int P, PrefArgs a,
+// mean of the pairs' losses, one every `step` places
+__global__ void __launch_bounds__(256) pref_loss_kernel(const double* __restrict__ pair_loss, int P, long long step,
                                                         float* __restrict__ loss) {
   griddep_wait();
   griddep_launch();
   __shared__ double red[8];
   double v = 0.0;
-  for (int p = threadIdx.x; p < P; p += blockDim.x) {
-    double l, dh;
-    pref_terms(a, (double)margins[p], &l, &dh);
-    v += l;
-  }
+  for (int p = threadIdx.x; p < P; p += blockDim.x) v += pair_loss[p * step];
   v = lp_block_sum(v, red);
   if (threadIdx.x == 0) loss[0] = (float)(v / P);
 }
@@ -1308,9 +1306,9 @@ extern "C" int rgpt_preference_loss(const void* logits, int dtype, long long sb,
   // 512 x 1 x 256 10.7, 1 x 256 x 2048 10.8; one CTA going through the pairs 20.6, 833, 10.1; at 512 tokens 11.6 / 10.4).
   const int by_warp = T <= 256 ? 1 : 0;
   const unsigned pair_ctas = by_warp ? (unsigned)((P + 7) / 8) : (unsigned)P;
-  launch_pdl(pref_pair_kernel, dim3(pair_ctas), dim3(256), 0, s, 1, (const double*)scratch, labels, ignore_index, V, P, T,
+  launch_pdl(pref_pair_kernel, dim3(pair_ctas), dim3(256), 0, s, 1, scratch, labels, ignore_index, V, P, T,
              by_warp, ref_logps, a, seq_logps, margins, coef, loss);
-  if (pair_ctas > 1) launch_pdl(pref_loss_kernel, dim3(1), dim3(256), 0, s, 1, margins, P, a, loss);
+  if (pair_ctas > 1) launch_pdl(pref_loss_kernel, dim3(1), dim3(256), 0, s, 1, (const double*)scratch, P, (long long)T, loss);
   if (dlogits &&
       (rc = launch_logp_bwd(logits, dtype, lr, M, V, labels, ignore_index, lse, coef, 1, dlogits, LpRows{db, dt, T}, s)))
     return rc;
