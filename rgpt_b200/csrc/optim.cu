@@ -119,6 +119,9 @@ constexpr float A8_R_UNIT = 256.0f;
 __device__ __forceinline__ float a8_decode_r(uint32_t q) {
   return __half2float(__ushort_as_half((unsigned short)(q << 5)));
 }
+// The bits of |v|: compared as whole numbers they order like the values, with NaN above infinity, so that a block with a
+// NaN has it as its largest (floating-point maxima drop it).
+__device__ __forceinline__ uint32_t a8_size(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 __device__ __forceinline__ float2 a8_decode_m2(uint32_t q2) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q2, __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(A8_THREADS, 20) adamw8_kernel(const RgptAdamw8
         cr[k >> 2] |= (inside(k) ? (uint32_t)t.vq[at(k)] : 0u) << (8 * (k & 3));
       }
     }
-    float am = 0.f, ar = 0.f;
+    uint32_t most_m = 0u, most_r = 0u;
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
       const float2 c = a8_decode_m2((cm[k >> 2] >> (8 * (k & 3))) & 0xFFFFu);
@@ -184,13 +187,13 @@ __global__ void __launch_bounds__(A8_THREADS, 20) adamw8_kernel(const RgptAdamw8
       r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(q, q), beta2), __fmul_rn(__fmul_rn(g[k], g[k]), w2)));
       const float u = __fmul_rn(m[k], rcp_approx(fmaf(r[k], inv_sqrt_bc2, eps)));
       p[k] = fmaf(u, step, __fmul_rn(p[k], decay));
-      am = fmaxf(am, fabsf(m[k]));
-      ar = fmaxf(ar, r[k]);
+      most_m = max(most_m, a8_size(m[k]));
+      most_r = max(most_r, a8_size(r[k]));
     }
-    am = warp_max(am);
-    ar = warp_max(ar);
-    if (!(am > A8_TINY)) am = 0.f;
-    if (!(ar > A8_TINY)) ar = 0.f;
+    float am = __uint_as_float(__reduce_max_sync(0xffffffffu, most_m));
+    float ar = __uint_as_float(__reduce_max_sync(0xffffffffu, most_r));
+    if (am <= A8_TINY) am = 0.f;  // a NaN stays, and gives the block NaN scales
+    if (ar <= A8_TINY) ar = 0.f;
     const float im = am > 0.f ? __fmul_rn(__frcp_rn(am), A8_M_TOP) : 0.f;
     const float ir = ar > 0.f ? __fmul_rn(__frcp_rn(ar), A8_R_TOP) : 0.f;
     cm[0] = cm[1] = cr[0] = cr[1] = 0u;
