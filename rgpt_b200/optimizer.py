@@ -32,6 +32,11 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)  # optimizer.py:19
 _ADAM_CHUNK = 16384
 _ADAM8_CHUNK = 2048
 ADAM8_MIN_NUMEL = 4096  # smaller parameters keep fp32 moments under adam_state_bits=8
+# Codes of sqrt(v) lie 1.6 to 3.1 % apart and round to nearest; a step of a fallen gradient lowers sqrt(v) by
+# 1 - sqrt(beta2) at most. Where that is far below half a code's distance the codes stop following: with the gradient of
+# every second element ten times smaller for 8 / (1 - beta2) steps, the 8-bit v of these is 1.01 times the fp32 one at 0.98
+# (median; 95 % below 1.12), 1.13 (1.36) at 0.99, 8 at 0.995 and 91 at 0.999.
+ADAM8_MAX_BETA2 = 0.98
 _HP_RING = 4  # pinned host slots for the per-step scalars (copies in flight before a slot is reused)
 
 
@@ -268,6 +273,7 @@ class Muon(torch.optim.Optimizer):
         """adam_state_bits (also per group): 32 keeps the AdamW moments in fp32; 8 keeps both in 8-bit codes with fp32
         scales for blocks of 256 elements (rgpt_adamw8 has the format) for parameters of at least 4096 elements, with
         state keys exp_avg_q8, exp_avg_scale, exp_avg_sq_q8, exp_avg_sq_scale: 2 bytes a parameter instead of 8.
+        Their codes follow second-moment decays beta2 of at most 0.98; slower ones are refused.
         ns_precision: "bf16" iterates Newton-Schulz in bf16 as the reference does (optimizer.py:20-44);
         "fp32" iterates it at fp32 accuracy (hi/lo bf16 operands, fp32 accumulation) from the same bf16
         input, the update still rounded to bf16 as the reference rounds it (optimizer.py:68)."""
@@ -280,6 +286,8 @@ class Muon(torch.optim.Optimizer):
                         ns_steps=ns_steps, ns_coeffs=tuple(ns_coeffs), ns_precision=ns_precision,
                         adam_state_bits=adam_state_bits)
         super().__init__(params, defaults)
+        for group in self.param_groups:
+            self._check_adam8(group)
         self._cache: Dict[Any, Any] = {}
         self._hp_dev: Optional[torch.Tensor] = None
         # Independent update jobs (each Newton-Schulz shape class, each AdamW group) run on their own
@@ -288,6 +296,15 @@ class Muon(torch.optim.Optimizer):
         # overlap each other's tails. Set to False to issue everything on the caller's stream.
         self.concurrent = True
         self._streams: List[torch.cuda.Stream] = []
+
+    @staticmethod
+    def _check_adam8(group) -> None:
+        """Refuse a second-moment decay that the group's 8-bit codes cannot follow."""
+        beta2 = float(group["adam_betas"][1])
+        if (beta2 > ADAM8_MAX_BETA2 and group.get("adam_state_bits", 32) == 8 and not group.get("use_muon", False)
+                and any(p.numel() >= ADAM8_MIN_NUMEL for p in group["params"])):
+            raise ValueError(f"adam_state_bits=8 needs beta2 <= {ADAM8_MAX_BETA2}, got {beta2}: 8-bit second moments do not "
+                             "fall as slowly (use adam_state_bits=32)")
 
     # ------------------------------------------------------------------ device scalars
     def use_device_hparams(self) -> None:
@@ -311,6 +328,8 @@ class Muon(torch.optim.Optimizer):
         are rounded exactly as the by-value path rounds them, so both paths update identically."""
         if self._hp_dev is None:
             raise RuntimeError("stage_device_hparams() needs use_device_hparams() first")
+        for group in self.param_groups:
+            self._check_adam8(group)
         slot = self._hp_slot
         if self._hp_done[slot] is not None:
             self._hp_done[slot].synchronize()  # the copy that last read this pinned slot has run
@@ -509,6 +528,7 @@ class Muon(torch.optim.Optimizer):
             return []
         lr = float(group["lr"])
         wd = float(group["weight_decay"])
+        self._check_adam8(group)
         beta1, beta2 = group["adam_betas"]
         eps = float(group["adam_eps"])
         step_i = int(group.get("_adam_step", 0))
