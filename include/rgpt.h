@@ -273,8 +273,10 @@ int rgpt_linear_logprobs(const void* X, long long ldx, const void* W, long long 
                          const long long* labels, long long ignore_index, int round_bf16, float* part,
                          long long part_floats, float* logps, float* lse, void* stream);
 /* out [M, N] (row stride ldo; bf16, or fp32 with out_f32) = sum over s of part[s] [M, N] fp32 with rows of N rounded up to
- * 4, in the order of s: joins products whose contraction was cut, rounded once. */
-int rgpt_gemm_join(const float* part, int splits, int M, int N, void* out, long long ldo, int out_f32, void* stream);
+ * 4, in the order of s: joins products whose contraction was cut, rounded once. add (fp32 only): out += that sum. part is
+ * 16-byte aligned. */
+int rgpt_gemm_join(const float* part, int splits, int M, int N, void* out, long long ldo, int out_f32, int add,
+                   void* stream);
 /* The gradient of those logits for M rows, from the recomputed product: dlogits [M, >= V] bf16 =
  * dlogps * ([j = label] - e^{logit_j - lse}), zero rows where not scored. The gradients of X and W follow by
  * rgpt_gemm_bf16 (dX = dlogits W, dW += dlogits^T X). */

@@ -79,7 +79,7 @@ _SIGNATURES: dict[str, list] = {
     ],
     "rgpt_linear_logprobs": [_c_vp, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_vp, _c_ll,
                              _c_vp, _c_vp, _c_vp],
-    "rgpt_gemm_join": [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_vp],
+    "rgpt_gemm_join": [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_int, _c_int, _c_vp],
     "rgpt_linear_logprobs_dlogits": [_c_vp, _c_ll, _c_vp, _c_ll, _c_int, _c_int, _c_int, _c_vp, _c_ll, _c_vp, _c_vp,
                                      _c_vp, _c_ll, _c_vp],
     "rgpt_adamw8": [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_float, _c_float, _c_float, _c_float, _c_float, _c_int,

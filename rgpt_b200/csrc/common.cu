@@ -76,4 +76,4 @@ extern "C" int rgpt_device_error(void) {
   return RGPT_OK;
 }
 
-extern "C" int rgpt_version(void) { return 101; }
+extern "C" int rgpt_version(void) { return 102; }

@@ -1282,33 +1282,60 @@ __global__ void __launch_bounds__(ROWS == 1 ? 256 : 1024) lse_reduce_kernel(
   if (lse) lse[row] = (float)l;
 }
 
-// out = the sum of `splits` partial products, in their order.
-__global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ part, int splits, int M, int N, void* out,
-                                                        long long ldo, int f32) {
+// out = the sum of `splits` partial products, in their order, or with `add` out + that sum. Four columns a thread; whole:
+// out's rows start on their four elements' boundary.
+__global__ void __launch_bounds__(256) gemm_join_kernel(const float4* __restrict__ part, int splits, int M, int N, void* out,
+                                                        long long ldo, int f32, int add, int whole) {
   griddep_wait();
   griddep_launch();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, ld = (N + 3) / 4 * 4;
-  const int row = (int)(i / ld), col = (int)(i % ld);
-  if (row >= M || col >= N) return;
-  float s = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < splits; ++k) s += part[(long long)k * M * ld + i];
-  const long long at = (long long)row * ldo + col;
-  if (f32) reinterpret_cast<float*>(out)[at] = s;
-  else reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16(s);
+  const unsigned quads = (unsigned)(N + 3) / 4;
+  const long long q = (long long)blockIdx.x * 256 + threadIdx.x, size = (long long)M * quads;
+  if (q >= size) return;
+  const long long row = size <= 0xFFFFFFFFll ? (long long)((unsigned)q / quads) : q / quads;
+  const int col = 4 * (int)(q - row * quads), n = min(4, N - col);
+  const long long at = row * ldo + col;
+  const bool vec = whole && n == 4;
+  float* o = reinterpret_cast<float*>(out) + at;
+  float4 old = make_float4(0.f, 0.f, 0.f, 0.f), s = old;
+  if (add && vec) old = *reinterpret_cast<const float4*>(o);
+  for (int k0 = 0; k0 < splits; k0 += 4) {  // four loads on their way
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k0 + k < splits) v[k] = __ldcs(&part[(k0 + k) * size + q]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k0 + k < splits) s.x += v[k].x, s.y += v[k].y, s.z += v[k].z, s.w += v[k].w;
+  }
+  if (vec) {
+    if (f32) *reinterpret_cast<float4*>(o) = make_float4(old.x + s.x, old.y + s.y, old.z + s.z, old.w + s.w);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(out) + at) =
+             make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+    return;
+  }
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  for (int j = 0; j < n; ++j) {
+    if (!f32) reinterpret_cast<__nv_bfloat16*>(out)[at + j] = __float2bfloat16(v[j]);
+    else o[j] = add ? o[j] + v[j] : v[j];
+  }
 }
 
-extern "C" int rgpt_gemm_join(const float* part, int splits, int M, int N, void* out, long long ldo, int out_f32,
+extern "C" int rgpt_gemm_join(const float* part, int splits, int M, int N, void* out, long long ldo, int out_f32, int add,
                               void* stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   const int st = rgpt_check_device(dev);
   if (st) return st;
-  if (splits < 1 || M < 1 || N < 1 || ldo < N || part == nullptr || out == nullptr)
-    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "gemm_join: splits=%d M=%d N=%d ldo=%lld or a null pointer", splits, M, N, ldo);
-  const long long n = (long long)M * ((N + 3) / 4 * 4);
-  launch_pdl(gemm_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1, part,
-             splits, M, N, out, ldo, out_f32);
+  if (splits < 1 || M < 1 || N < 1 || ldo < N || part == nullptr || out == nullptr || (add && !out_f32))
+    return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "gemm_join: splits=%d M=%d N=%d ldo=%lld, a null pointer, or a sum added to bf16",
+                          splits, M, N, ldo);
+  if ((reinterpret_cast<uintptr_t>(part) & 15) != 0)
+    return rgpt_set_error(RGPT_ERR_MISALIGNED, "gemm_join: the partial products are not 16-byte aligned");
+  const long long ctas = ((long long)M * ((N + 3) / 4) + 255) / 256;
+  if (ctas > 0x7fffffffll) return rgpt_set_error(RGPT_ERR_BAD_SHAPE, "gemm_join: M=%d N=%d are too large", M, N);
+  const int whole = ldo % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (out_f32 ? 16 : 8) == 0 ? 1 : 0;
+  launch_pdl(gemm_join_kernel, dim3((unsigned)ctas), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), 1,
+             reinterpret_cast<const float4*>(part), splits, M, N, out, ldo, out_f32, add, whole);
   return rgpt_check_launch("gemm_join_kernel");
 }
 

@@ -635,18 +635,35 @@ def _product(dev: int, A: tuple, B: tuple, M: int, N: int, C: int, D: tuple, *, 
     _call_on(dev, "rgpt_gemm_bf16", *A, *B, M, N, C, batch, epi, 0, 1.0, 0.0, *D, None, 0, 0, None, 0, 0, None, splitk, None)
 
 
-def _product_long(out: torch.Tensor, dev: int, A: tuple, B: tuple, M: int, N: int, C: int, D: int, ldd: int) -> None:
-    """D = A @ B^T as _product, written in out's type. Where D has tiles for half of the SMs at most and C is long, C is cut
-    into parts whose fp32 products are joined in order (88 rows x 408 columns over 116602 take 536 us otherwise, the whole
-    backward of such rows 112)."""
+def _cuts(M: int, N: int, C: int, sms: int, add: bool) -> int:
+    """Parts that _product_long cuts a contraction of C into."""
     tiles = -(-M // 128) * -(-N // 256)
-    sms = torch.cuda.get_device_properties(dev).multi_processor_count
-    splits = min(sms // tiles, C // 1024) if 2 * tiles <= sms else 1
+    if 2 * tiles <= sms:
+        return min(sms // tiles, C // 1024)
+    if not add:
+        return 1
+    # More tiles: rounds of them (0.43 us for 64 of C, and eight such for the epilogue) against the join (4 us, and 2.4e-6
+    # an element and 0.45e-6 for each of its parts). dw of 5000 x 1024 over 16368, 160 tiles on 148 SMs: 221 us in one part,
+    # 154 + 25 in four; of 10000 x 1024 over 12000, 316 tiles: 252 in one, 205 + 42 in four.
+    def us(s: int) -> float:
+        return -(-tiles * s // sms) * (-(-C // (64 * s)) + 8) * 0.43 + (s > 1) * (4 + M * N * (2.4e-6 + 0.45e-6 * s))
+
+    return min(range(1, max(1, min(8, C // 1024, LINEAR_CHUNK_ELEMS // (2 * M * N))) + 1), key=us)
+
+
+def _product_long(out: torch.Tensor, dev: int, A: tuple, B: tuple, M: int, N: int, C: int, D: int, ldd: int,
+                  add: bool = False) -> None:
+    """D = A @ B^T as _product, written in out's type, or with `add` (fp32) added to D. Where D has tiles for half of the SMs
+    at most and C is long, C is cut into parts whose fp32 products are joined in order (88 rows x 408 columns over 116602
+    take 536 us otherwise, the whole backward of such rows 112). Each element of D gets one sum, in a fixed order: equal calls
+    give equal bits (the GEMM's own split of C adds its parts as they arrive)."""
+    splits = _cuts(M, N, C, torch.cuda.get_device_properties(dev).multi_processor_count, add)
     f32 = out.dtype is torch.float32
     if splits < 2:
-        return _product(dev, (*A, 0), (*B, 0), M, N, C, (D, ldd, 0), epi=EPI_STORE_F32 if f32 else EPI_STORE_BF16)
-    each = -(-C // (64 * splits)) * 64
-    whole, splits, ld = C // each, -(-C // each), (N + 3) // 4 * 4
+        return _product(dev, (*A, 0), (*B, 0), M, N, C, (D, ldd, 0),
+                        epi=EPI_ACCUM_F32 if add else EPI_STORE_F32 if f32 else EPI_STORE_BF16)
+    each = C // splits if A[1] and B[1] else C // (8 * splits) * 8  # of a K-major operand a part starts on 16 bytes
+    whole, splits, ld = C // each, -(-C // each), (N + 3) // 4 * 4  # equal parts, and perhaps what is left of fewer than 8 * splits
     part = torch.empty(splits * M * ld, device=out.device, dtype=torch.float32)
     step = [each * (ldo if mn else 1) for _, mn, ldo in (A, B)]  # elements from one part to the next
     P, size = part.data_ptr(), M * ld
@@ -654,7 +671,7 @@ def _product_long(out: torch.Tensor, dev: int, A: tuple, B: tuple, M: int, N: in
     if whole < splits:
         A, B = ((at + 2 * whole * st, mn, ldo, 0) for (at, mn, ldo), st in zip((A, B), step))
         _product(dev, A, B, M, N, C - whole * each, (P + 4 * whole * size, ld, 0), epi=EPI_STORE_F32)
-    _call_on(dev, "rgpt_gemm_join", P, splits, M, N, D, ldd, int(f32))
+    _call_on(dev, "rgpt_gemm_join", P, splits, M, N, D, ldd, int(f32), int(add))
 
 
 # Gradient rows of linear_logprobs_bwd in flight: at most this many bf16 logit gradients (1 GiB) at a time.
@@ -706,11 +723,8 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
             _product_long(dx, index, (d, 0, ld), (W, 1, ldw), n, K, V, dx.data_ptr() + dx.element_size() * a * dx.stride(0),
                           dx.stride(0))
         if acc is not None:
-            if acc.dtype is torch.bfloat16:
-                _product_long(acc, index, (d, 1, ld), (xa, 1, ldx), V, K, n, acc.data_ptr(), acc.stride(0))
-            else:
-                _product(index, (d, 1, ld, 0), (xa, 1, ldx, 0), V, K, n, (acc.data_ptr(), acc.stride(0), 0), epi=EPI_ACCUM_F32,
-                         splitk=0)
+            _product_long(acc, index, (d, 1, ld), (xa, 1, ldx), V, K, n, acc.data_ptr(), acc.stride(0),
+                          add=acc.dtype is torch.float32)
     if acc is not dw:
         dw.copy_(acc[:, :K])
 
