@@ -712,7 +712,7 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
     dl = torch.empty(rows * ld, device=dev, dtype=torch.bfloat16)
     acc = dw
     if dw is not None and dw.dtype is torch.bfloat16 and rows < M:
-        acc = torch.zeros(V, (K + 3) // 4 * 4, device=dev, dtype=torch.float32)
+        acc = torch.empty(V, (K + 3) // 4 * 4, device=dev, dtype=torch.float32)  # the sum over the chunks
     X, W, L, S, G, d = (t.data_ptr() for t in (x, w, labels, lse, dlogps, dl))
     ldx, ldw = x.stride(0), w.stride(0)
     for a in range(0, M, rows):
@@ -724,9 +724,9 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
                           dx.stride(0))
         if acc is not None:
             _product_long(acc, index, (d, 1, ld), (xa, 1, ldx), V, K, n, acc.data_ptr(), acc.stride(0),
-                          add=acc.dtype is torch.float32)
+                          add=acc.dtype is torch.float32 and (acc is dw or a > 0))
     if acc is not dw:
-        dw.copy_(acc[:, :K])
+        _call_on(index, "rgpt_gemm_join", acc.data_ptr(), 1, V, K, dw.data_ptr(), dw.stride(0), 0, 0)
 
 
 # ----------------------------------------------------------------------------- optimizer
