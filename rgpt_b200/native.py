@@ -383,12 +383,30 @@ def _call_on(index: int, name: str, *args, kernels: int = 1) -> None:
 
 # The operators below check their arguments twice over: _fastargs.pack (csrc/fastargs.cpp) in one step, giving the
 # entry point's arguments when all is well, and otherwise here, where a refusal says what was wrong. (Where only the
-# kernel library has been built, the checks here serve alone.)
-try:
-    from ._fastargs import pack as _pack
-except ImportError:
-    def _pack(kinds: str, tensors: tuple):
-        return None
+# kernel library has been built, the checks here serve alone.) The extension is loaded by the first call, as the kernel
+# library is: importing this module maps neither.
+def _load_pack():
+    global _pack
+    try:
+        from ._fastargs import pack as _pack
+    except ImportError:
+        def _pack(kinds: str, tensors: tuple):
+            return None
+    return _pack
+
+
+def __getattr__(name: str):
+    if name == "_pack":
+        return _load_pack()
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def _packed(kinds: str, tensors: tuple):
+    """The entry point's arguments, or None where the checks here have to say what is wrong."""
+    try:
+        return _pack(kinds, tensors)
+    except NameError:
+        return _load_pack()(kinds, tensors)
 
 
 def _flat(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int) -> int:
@@ -460,7 +478,7 @@ def token_logprobs(logits: torch.Tensor, labels: torch.Tensor, logps: torch.Tens
     """logps = log softmax(logits)[label], 0 for tokens that are not scored (label ignore_index or outside the
     vocabulary); lse (optional, for token_logprobs_bwd) = logsumexp. logits [M, V] or [B, T, V] in bf16, fp16 or fp32
     with unit stride along the vocabulary and any other strides; labels int64, logps and lse fp32 of the leading shape."""
-    p = _pack("LyfF", (logits, labels, logps, lse))
+    p = _packed("LyfF", (logits, labels, logps, lse))
     if p is not None:
         return _call_on(p[10], "rgpt_token_logprobs", *p[:8], int(ignore_index), p[8], p[9])
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
@@ -478,7 +496,7 @@ def token_logprobs_bwd(logits: torch.Tensor, labels: torch.Tensor, lse: torch.Te
                        dlogits: torch.Tensor, *, ignore_index: int = -100) -> None:
     """dlogits = dlogps * (onehot(label) - softmax(logits)), zero rows for tokens that are not scored. dlogits: the
     logits themselves (overwritten) or another tensor of their type and shape."""
-    p = _pack("LyffG", (logits, labels, lse, dlogps, dlogits))
+    p = _packed("LyffG", (logits, labels, lse, dlogps, dlogits))
     if p is not None and dlogits is not None:
         return _call_on(p[13], "rgpt_token_logprobs_bwd", *p[:8], int(ignore_index), *p[8:13])
     dt, sb, st, B, T, V = _logit_rows(logits, "logits")
@@ -516,7 +534,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, ref_logps: torch
         raise ValueError("preference_loss: label_smoothing must be in [0, 0.5], and 0 unless kind is 'sigmoid'")
     if not 0.0 < beta < float("inf"):
         raise ValueError(f"preference_loss: beta must be positive and finite, got {beta}")
-    p = _pack("LyRffbhb1WG", (logits, labels, ref_logps, token_logps, lse, seq_logps, margins, coef, loss, scratch,
+    p = _packed("LyRffbhb1WG", (logits, labels, ref_logps, token_logps, lse, seq_logps, margins, coef, loss, scratch,
                               dlogits))
     if p is not None and logits.dim() == 3:
         pairs, T = p[4] // 2, p[5]
@@ -564,7 +582,7 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_logps: torch.Ten
         raise ValueError(f"policy_loss: clip_low must be in [0, 1] and clip_high >= 0, got {clip_low} and {clip_high}")
     if kl_coef != 0.0 and ref_logps is None:
         raise ValueError("policy_loss: kl_coef needs ref_logps")
-    p = _pack("LyfFafc4FFG", (logits, labels, old_logps, ref_logps, advantages, token_logps, counts, stats, lse, coef,
+    p = _packed("LyfFafc4FFG", (logits, labels, old_logps, ref_logps, advantages, token_logps, counts, stats, lse, coef,
                               dlogits))
     if p is not None:
         return _call_on(p[20], "rgpt_policy_loss", *p[:8], int(ignore_index), *p[8:12], float(clip_low),
@@ -609,7 +627,7 @@ def linear_logprobs(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, logp
     lse [M] (optional, for linear_logprobs_bwd) is written for every row. round_bf16: the products are rounded to bf16
     first, which gives what token_logprobs gives on stored bf16 logits. part: fp32 scratch of at least
     4 * M * ceil(V/128) elements (allocated when None)."""
-    p = _pack("XXyPfF", (x, w, labels, part, logps, lse))
+    p = _packed("XXyPfF", (x, w, labels, part, logps, lse))
     if p is not None:
         return _call_on(p[9], "rgpt_linear_logprobs", *p[:4], *x.shape[:1], *w.shape, p[4], int(ignore_index),
                         int(bool(round_bf16)), *p[5:9], kernels=2)
@@ -755,7 +773,7 @@ def adamw8(table: torch.Tensor, chunk_tensor: torch.Tensor, chunk_start: torch.T
 
 def adamw8_moments(p: torch.Tensor, mq: torch.Tensor, m_scale: torch.Tensor, vq: torch.Tensor, v_scale: torch.Tensor):
     """(m, v), fp32 of p's shape: the moments of parameter p that 8-bit codes and their scales stand for."""
-    a = _pack("zususNN", (p, mq, m_scale, vq, v_scale, None, None))
+    a = _packed("zususNN", (p, mq, m_scale, vq, v_scale, None, None))
     if a is not None:
         _call_on(a[6], "rgpt_adamw8_moments", *a[:6], mq.shape[0])
         return a[7], a[8]
