@@ -360,8 +360,9 @@ PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 
 _entries: dict = {}  # bound entry points by name
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# (a torch without CUDA has neither, and no tensor that would need them)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _call_on(index: int, name: str, *args, kernels: int = 1) -> None:
