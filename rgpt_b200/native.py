@@ -455,8 +455,14 @@ def _end(t: torch.Tensor) -> int:
     return t.data_ptr() + last * t.element_size()
 
 
+def _rows_apart(sb: int, st: int, B: int, T: int, width: int) -> bool:
+    """Whether rows of `width` elements at these strides share no element, batch first or time first."""
+    return ((T == 1 or st >= width) and (B == 1 or sb >= (T - 1) * st + width)) or (sb >= width and st >= (B - 1) * sb + width)
+
+
 def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):
-    """(address, batch stride, token stride) of the gradient's rows: the logits themselves, or memory apart from them."""
+    """(address, batch stride, token stride) of the gradient's rows: the logits themselves, or memory apart from them
+    (elsewhere, or in turn with their rows at the same strides)."""
     if dlogits is None:
         return None, 0, 0
     if dlogits.dtype is not logits.dtype or dlogits.shape != logits.shape or dlogits.get_device() != logits.get_device():
@@ -466,11 +472,13 @@ def _grad_rows(dlogits: torch.Tensor | None, logits: torch.Tensor):
     if dlogits.is_contiguous():
         end = at + B * T * V * dlogits.element_size()
     else:
-        if not ((T == 1 or st >= V) and (B == 1 or sb >= (T - 1) * st + V)) and not (sb >= V and st >= (B - 1) * sb + V):
+        if not _rows_apart(sb, st, B, T, V):
             raise ValueError(f"the rows of dlogits overlap (strides {dlogits.stride()})")
         end = _end(dlogits)
     if (at != of or dlogits.stride() != logits.stride()) and at < _end(logits) and of < end:
-        raise ValueError("dlogits must be the logits themselves or share no memory with them")
+        off, odd = divmod(abs(at - of), dlogits.element_size())
+        if dlogits.stride() != logits.stride() or odd or off < V or not _rows_apart(sb, st, B, T, off + V):
+            raise ValueError("dlogits must be the logits themselves or share no memory with them")
     return at, sb, st
 
 
