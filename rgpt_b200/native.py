@@ -710,7 +710,9 @@ def linear_logprobs_bwd(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, 
                         chunk_rows: int | None = None) -> None:
     """The gradients of linear_logprobs (round_bf16=False): dx [M, K] written in bf16 or fp32; dw [V, K] written when
     bf16, ACCUMULATED when fp32. Either may be None. The logits' gradient exists for chunk_rows rows at a time (default:
-    as many as fit 1 GiB): its tiles come from the recomputed product, rounded to bf16 for the two GEMMs that follow."""
+    as many as fit 1 GiB): its tiles come from the recomputed product, rounded to bf16 for the two GEMMs that follow, as the
+    cross entropy's gradient is (the tensor cores' type; an element in two bf16 halves would double both products, for 2.3e-3
+    of error in dx and dw against 64 bits, of which their own bf16 makes 1.7e-3). Equal calls give equal bits."""
     M, V, K = _linear_operands(x, w)
     dev = x.device
     for t, n, dtype in ((labels, "labels", torch.int64), (lse, "lse", torch.float32), (dlogps, "dlogps", torch.float32)):
